@@ -65,6 +65,7 @@ enum { OCL_LAYOUT_GGUF = 0, OCL_LAYOUT_TILED16 = 1 };
 typedef struct ocl_ctx ocl_ctx;   /* one device + stream + scratch */
 typedef struct ocl_qbuf ocl_qbuf; /* a quantized weight resident in HBM */
 typedef struct ocl_tpcomm ocl_tpcomm; /* tensor-parallel peer buffers of one rank */
+typedef struct ocl_rope ocl_rope; /* rotation steps of a model's position encoding, on the device */
 
 /* ---- context ------------------------------------------------------------ */
 
@@ -273,7 +274,8 @@ OCL_API int ocl_argmax_f32(ocl_ctx* ctx, const float* logits_dev, size_t rows, s
 OCL_API int ocl_q_embed_rows(ocl_ctx* ctx, const ocl_qbuf* table, const int32_t* ids_dev, size_t n_ids,
                      float* out_dev);
 /* Read and clear the context's device-side error counters (synchronises the
- * stream): embedding ids that were out of range, and bounded device waits that
+ * stream): ids that were out of range (embedding rows; cache places and pages;
+ * history and bias tokens), and bounded device waits that
  * gave up (a GEMV whose shared-memory stream stalled for ~1 s, or a fused
  * all-reduce whose peers did not signal in ~1 s; that output is then
  * incomplete).  Either pointer may be NULL.  Returns OCL_ERR_TIMEOUT (after
@@ -281,6 +283,112 @@ OCL_API int ocl_q_embed_rows(ocl_ctx* ctx, const ocl_qbuf* table, const int32_t*
  * the status still sees the failure (KernelError in the reference's terms,
  * crates/core/src/lib.rs:75-80). */
 OCL_API int ocl_take_device_errors(ocl_ctx* ctx, unsigned int* bad_ids, unsigned int* timeouts);
+
+/* ---- between the linear layers of a decoder -------------------------------- */
+
+/* Element types of a key/value cache (GGUF tensor-type tags). */
+enum { OCL_KV_F16 = 1, OCL_KV_BF16 = 30 };
+
+/* A paged key/value cache of one layer, owned by the caller
+ * (PagedKvCacheLayout, crates/core/src/lib.rs:578-665).  Token t of a sequence
+ * lies in page block_table[seq][t / page_size], slot t % page_size; k and v have
+ * the same strides, in elements, with head_dim elements of one head side by side.
+ * head_dim 64, 96, 128 or 256; k_dev / v_dev 16-byte aligned, strides multiples of
+ * 8; any page_size. */
+typedef struct ocl_kv_cache {
+    void* k_dev;
+    void* v_dev;
+    int dtype; /* OCL_KV_F16 or OCL_KV_BF16 */
+    size_t n_pages, page_size, n_kv_heads, head_dim;
+    size_t page_stride, head_stride, token_stride;
+} ocl_kv_cache;
+
+/* Where the rows of a call stand (device memory): row r is token positions_dev[r]
+ * of sequence seqs_dev[r], or of sequence r when seqs_dev is NULL (then rows <=
+ * n_seqs).  A negative position is a padding row.  block_table_dev is int32
+ * [n_seqs, max_pages] with rows table_stride apart; entries behind a sequence's
+ * last page are not read.  max_pages * page_size bounds a sequence's length. */
+typedef struct ocl_kv_rows {
+    const int32_t* positions_dev;
+    const int32_t* seqs_dev;
+    const int32_t* block_table_dev;
+    size_t n_seqs, max_pages, table_stride;
+} ocl_kv_rows;
+
+/* Rotation of a head's first rot_dim elements: pair i turns by
+ * position * base^(-2i / rot_dim) / factors_host[i] (factors NULL = all 1;
+ * GGUF rope_freqs.weight).  interleaved 0: pairs (i, i + rot_dim / 2); 1: pairs
+ * (2i, 2i + 1).  rot_dim a multiple of 8, at most 256.  The angle is kept as a
+ * 64-bit fixed-point fraction of a revolution, exact at far positions. */
+OCL_API int ocl_rope_create(ocl_ctx* ctx, size_t rot_dim, double base, const float* factors_host, int interleaved,
+                            ocl_rope** out);
+OCL_API int ocl_rope_free(ocl_rope* rope);
+
+/* Norm of q and k per head, rotation, and the cache write, in one launch
+ * (crates/kernels/src/rmsnorm.rs, rope.rs and the cache write of
+ * crates/models/src/qwen/qwen2_5/decode.rs:83-91).  qkv_dev f32 [rows, (n_heads +
+ * 2 n_kv_heads) * head_dim], rows qkv_stride floats apart: q heads, k heads, v
+ * heads, as the fused projection gives them.  q_norm_dev / k_norm_dev f32
+ * [head_dim] or NULL (no norm): x * rsqrt(mean(x^2) + eps) * w.  rope NULL = no
+ * rotation.  q_out_dev f32 [rows, n_heads, head_dim]; k and v are rounded to the
+ * cache's type at the row's place.  A padding row's q is zeros and nothing is
+ * cached.  A position, sequence or page out of range caches nothing and bumps the
+ * counter that ocl_take_device_errors reports as bad ids.  Rows of one call must
+ * stand at different places.  qkv, norms and q_out 16-byte aligned, qkv_stride a
+ * multiple of 4. */
+OCL_API int ocl_qk_norm_rope(ocl_ctx* ctx, const float* qkv_dev, size_t qkv_stride, size_t rows, size_t n_heads,
+                             const ocl_kv_cache* cache, const ocl_kv_rows* at, const float* q_norm_dev,
+                             const float* k_norm_dev, float eps, const ocl_rope* rope, float* q_out_dev);
+
+/* Attention over the paged cache (scaled_dot_product_attention of
+ * crates/models/src/qwen/qwen2_5/decode.rs:96-105 for cached decode): row r sees
+ * tokens 0..positions[r] of its sequence, its own included, so that several rows of
+ * one sequence (drafted tokens, a prompt) are causal.  Query head h reads k/v head
+ * h / (n_heads / n_kv_heads).  q_dev f32 [rows, n_heads, head_dim], rows q_stride
+ * floats apart; out_dev f32 [rows, n_heads, head_dim].  scale > 0.  Accuracy: f32
+ * (q and the softmax weights are not rounded to 16 bits).  Padding rows give zeros.
+ * Tokens whose page is out of range are left out and counted as bad ids (a row with
+ * none left is zeros), as are rows whose sequence is (zeros) and positions past the
+ * block table (the tokens that it can hold are used).  The lengths are read on the
+ * device: a captured launch follows them.  Uses a fixed workspace of the context,
+ * so launches of one context must not overlap on the GPU. */
+OCL_API int ocl_paged_attention(ocl_ctx* ctx, const float* q_dev, size_t q_stride, size_t rows, size_t n_heads,
+                                const ocl_kv_cache* cache, const ocl_kv_rows* at, float scale, float* out_dev);
+
+/* Rules on the logits of one call, all in device memory; a NULL member is off.
+ * In this order, each step rounded to f32, for token t of row r with c = times t
+ * stands in the generated part of the row's history:
+ *   t anywhere in the history:  l = l > 0 ? l / repetition[r] : l * repetition[r]
+ *   c > 0:                      l = (l - frequency[r] * c) - presence[r]
+ *   t among the biases:         l = l + (the sum of its biases, in list order)
+ *   t not allowed:              l = -inf
+ * history int32 [rows, history_max], rows history_stride apart: row r's first
+ * history_lens[r] tokens (at most history_max), of which the first prompt_lens[r]
+ * (NULL = none) are the prompt.  bias_ids / bias_values [rows, bias_count], rows
+ * bias_stride apart.  Negative ids are unused places; ids >= vocab
+ * are skipped and counted as bad ids.  allowed: uint32 [rows, allowed_stride],
+ * token t is bit t % 32 of word t / 32. */
+typedef struct ocl_logit_rules {
+    const int32_t* history_dev;
+    size_t history_stride, history_max;
+    const int32_t* history_lens_dev;
+    const int32_t* prompt_lens_dev;
+    const float* repetition_dev;
+    const float* frequency_dev;
+    const float* presence_dev;
+    const int32_t* bias_ids_dev;
+    const float* bias_values_dev;
+    size_t bias_stride, bias_count;
+    const uint32_t* allowed_dev;
+    size_t allowed_stride;
+} ocl_logit_rules;
+
+/* Apply the rules to logits_dev f32 [rows, vocab] (rows in_stride floats apart)
+ * and write the result to out_dev (rows out_stride apart; may be logits_dev itself
+ * with the same stride) and / or its greedy pick to ids_dev, as ocl_argmax_f32
+ * would make it.  One of out_dev and ids_dev may be NULL.  rows <= 65535. */
+OCL_API int ocl_logits_process(ocl_ctx* ctx, const float* logits_dev, size_t in_stride, size_t rows, size_t vocab,
+                               const ocl_logit_rules* rules, float* out_dev, size_t out_stride, int32_t* ids_dev);
 
 #ifdef __cplusplus
 }

@@ -14,4 +14,7 @@ def __getattr__(name):
     if name in ("CudaKernelBackend", "DeviceTensor", "QuantBuffer"):
         from . import backend
         return getattr(backend, name)
+    if name in ("LogitRules", "PagedKvCache", "RopeTable"):
+        from . import decode
+        return getattr(decode, name)
     raise AttributeError(name)

@@ -21,6 +21,27 @@ OCL_ERR_TIMEOUT = -5
 _vp = C.c_void_p
 _sz = C.c_size_t
 
+
+class KvCacheDesc(C.Structure):
+    """ocl_kv_cache"""
+    _fields_ = [("k_dev", _vp), ("v_dev", _vp), ("dtype", C.c_int)] + [(n, _sz) for n in (
+        "n_pages", "page_size", "n_kv_heads", "head_dim", "page_stride", "head_stride", "token_stride")]
+
+
+class KvRowsDesc(C.Structure):
+    """ocl_kv_rows"""
+    _fields_ = [("positions_dev", _vp), ("seqs_dev", _vp), ("block_table_dev", _vp), ("n_seqs", _sz),
+                ("max_pages", _sz), ("table_stride", _sz)]
+
+
+class LogitRulesDesc(C.Structure):
+    """ocl_logit_rules"""
+    _fields_ = [("history_dev", _vp), ("history_stride", _sz), ("history_max", _sz),
+                ("history_lens_dev", _vp), ("prompt_lens_dev", _vp),
+                ("repetition_dev", _vp), ("frequency_dev", _vp), ("presence_dev", _vp), ("bias_ids_dev", _vp),
+                ("bias_values_dev", _vp), ("bias_stride", _sz), ("bias_count", _sz), ("allowed_dev", _vp), ("allowed_stride", _sz)]
+
+
 # name -> (restype, argtypes); every symbol include/ocelotl_cuda.h declares.
 SIGNATURES = {
     "ocl_cuda_init": (C.c_int, [C.c_int, C.POINTER(_vp)]),
@@ -55,6 +76,13 @@ SIGNATURES = {
     "ocl_q_gemm_gated_bf16": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _sz, _vp]),
     "ocl_argmax_f32": (C.c_int, [_vp, _vp, _sz, _sz, _vp]),
     "ocl_q_embed_rows": (C.c_int, [_vp, _vp, _vp, _sz, _vp]),
+    "ocl_rope_create": (C.c_int, [_vp, _sz, C.c_double, _vp, C.c_int, C.POINTER(_vp)]),
+    "ocl_rope_free": (C.c_int, [_vp]),
+    "ocl_qk_norm_rope": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(KvCacheDesc), C.POINTER(KvRowsDesc), _vp, _vp,
+                                   C.c_float, _vp, _vp]),
+    "ocl_paged_attention": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(KvCacheDesc), C.POINTER(KvRowsDesc), C.c_float,
+                                      _vp]),
+    "ocl_logits_process": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(LogitRulesDesc), _vp, _sz, _vp]),
     "ocl_take_device_errors": (C.c_int, [_vp, C.POINTER(C.c_uint), C.POINTER(C.c_uint)]),
 }
 

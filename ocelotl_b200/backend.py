@@ -23,6 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .decode import LogitRules, PagedKvCache, RopeTable, check_tensor
 from .errors import KernelError, UnsupportedError
 from .ggml import GgmlType, byte_len, geometry
 
@@ -154,6 +155,7 @@ class CudaKernelBackend:
             msg = self._lib.ocl_last_error(None).decode()
             raise (UnsupportedError("device", message=msg) if rc == _lib.OCL_ERR_UNSUPPORTED else _kernel_err(msg))
         self._ctx = ctx
+        self._stream = 0
         self.device_index = device
         self.torch_device = torch.device("cuda", device)
 
@@ -182,6 +184,7 @@ class CudaKernelBackend:
 
     def set_stream(self, stream: torch.cuda.Stream | None) -> None:
         self._check(self._lib.ocl_set_stream(self._ctx, C.c_void_p(stream.cuda_stream if stream else 0)))
+        self._stream = stream.cuda_stream if stream else 0
 
     def use_current_stream(self) -> None:
         """Launch on torch's current stream of this device."""
@@ -434,14 +437,188 @@ class CudaKernelBackend:
                 self.synchronize()
                 temp.quant.free()
 
+    # -- between the linear layers ------------------------------------------------
+    def kv_cache(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16) -> PagedKvCache:
+        """A zeroed paged cache of one layer: k and v [n_pages, n_kv_heads, page_size, head_dim]."""
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        return PagedKvCache(torch.zeros(shape, dtype=dtype, device=self.torch_device),
+                            torch.zeros(shape, dtype=dtype, device=self.torch_device))
+
+    def kv_cache_view(self, k: torch.Tensor, v: torch.Tensor) -> PagedKvCache:
+        """A cache over existing tensors [n_pages, n_kv_heads, page_size, head_dim], of any page and token strides."""
+        cache = PagedKvCache(k, v)
+        if k.device != self.torch_device:
+            raise _kernel_err(f"kv cache lives on {k.device} but the backend is on {self.torch_device}")
+        return cache
+
+    def rope_table(self, rot_dim: int, base: float, factors=None, interleaved: bool = False) -> RopeTable:
+        """Rotation of a head's first rot_dim elements; pair i turns by position * base^(-2i/rot_dim) / factors[i].
+
+        interleaved: pairs (2i, 2i+1) instead of (i, i + rot_dim/2).
+        """
+        f = None
+        if factors is not None:
+            f = np.ascontiguousarray(factors, dtype=np.float32).reshape(-1)
+            if f.size != rot_dim // 2:
+                raise _kernel_err(f"rope_table factors len {f.size} does not match rot_dim/2={rot_dim // 2}")
+        h = C.c_void_p()
+        self._check(self._lib.ocl_rope_create(self._ctx, rot_dim, base, None if f is None else f.ctypes.data,
+                                              1 if interleaved else 0, C.byref(h)))
+        return RopeTable(self, h.value, rot_dim)
+
+    def logit_rules(self, **parts) -> LogitRules:
+        """The rules of a batch of requests (see LogitRules), as process_logits and greedy_sample take them."""
+        return LogitRules(self.torch_device, **parts)
+
+    def _empty(self, shape, dtype=torch.float32) -> torch.Tensor:
+        """Device memory for an output, allocated on the stream that the kernels run on."""
+        s = self._stream
+        if torch.cuda.current_stream(self.torch_device).cuda_stream == s:
+            return torch.empty(shape, dtype=dtype, device=self.torch_device)
+        stream = torch.cuda.default_stream(self.torch_device) if s == 0 else \
+            torch.cuda.ExternalStream(s, device=self.torch_device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=self.torch_device)
+
+    def _out(self, out, shape: tuple, op: str) -> torch.Tensor:
+        if out is None:
+            return self._empty(shape)
+        if out.dtype != torch.float32 or out.device != self.torch_device or tuple(out.shape) != shape \
+                or not out.is_contiguous():
+            raise _kernel_err(f"{op} out must be a contiguous f32 {list(shape)} tensor on {self.torch_device}")
+        return out
+
+    def _rows(self, op: str, rows: int, cache: PagedKvCache, positions, block_table, seqs) -> _lib.KvRowsDesc:
+        dev = self.torch_device
+        if not isinstance(cache, PagedKvCache) or cache.k.device != dev:
+            raise _kernel_err(f"{op} cache must be a PagedKvCache on {dev}")
+        check_tensor(positions, f"{op} positions", torch.int32, dev, 1)
+        check_tensor(block_table, f"{op} block_table", torch.int32, dev, 2)
+        if positions.shape[0] != rows:
+            raise _kernel_err(f"{op} positions.len()={positions.shape[0]} does not match rows={rows}")
+        n_seqs, max_pages = block_table.shape
+        stride = block_table.stride(0) if n_seqs > 1 else max_pages
+        if seqs is not None:
+            check_tensor(seqs, f"{op} seqs", torch.int32, dev, 1)
+            if seqs.shape[0] != rows:
+                raise _kernel_err(f"{op} seqs.len()={seqs.shape[0]} does not match rows={rows}")
+            return _lib.KvRowsDesc(positions.data_ptr(), seqs.data_ptr(), block_table.data_ptr(), n_seqs, max_pages, stride)
+        return _lib.KvRowsDesc(positions.data_ptr(), None, block_table.data_ptr(), n_seqs, max_pages, stride)
+
+    def qk_norm_rope(self, qkv: torch.Tensor, cache: PagedKvCache, positions: torch.Tensor, block_table: torch.Tensor,
+                     rope: RopeTable | None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                     eps: float = 1e-6, seqs: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+        """Norm of q and k per head, position rotation, k and v into the cache: q f32 [rows, n_heads, head_dim].
+
+        qkv f32 [rows, (n_heads + 2 n_kv_heads) * head_dim] as `qkv()` gives it;
+        row r is token positions[r] of sequence seqs[r] (r when None), whose pages
+        block_table [n_seqs, max_pages] names.  A negative position is a padding row
+        (zeros, nothing cached).  Places out of range cache nothing and count as bad
+        ids (take_device_errors).  Rows of one call must stand at different places.
+        """
+        check_tensor(qkv, "qk_norm_rope qkv", torch.float32, self.torch_device, 2)
+        rows, width = qkv.shape
+        at = self._rows("qk_norm_rope", rows, cache, positions, block_table, seqs)
+        dim = cache.head_dim
+        heads = width // dim - 2 * cache.n_kv_heads
+        if width % dim or heads <= 0:
+            raise _kernel_err(f"qk_norm_rope qkv width {width} is not (n_heads + 2*{cache.n_kv_heads})*{dim}")
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None:
+                check_tensor(w, "qk_norm_rope " + name, torch.float32, self.torch_device, 1)
+                if w.shape[0] != dim:
+                    raise _kernel_err(f"qk_norm_rope {name}.len()={w.shape[0]} does not match head_dim={dim}")
+        out = self._out(out, (rows, heads, dim), "qk_norm_rope")
+        rc = self._lib.ocl_qk_norm_rope(
+            self._ctx, qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, cache.ref, C.byref(at),
+            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+            None if rope is None else rope.handle, out.data_ptr())
+        if rc:
+            self._check(rc)
+        return out
+
+    def paged_attention(self, q: torch.Tensor, cache: PagedKvCache, positions: torch.Tensor, block_table: torch.Tensor,
+                        scale: float | None = None, seqs: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of row r over tokens 0..positions[r] of its sequence: f32 [rows, n_heads, head_dim].
+
+        q f32 [rows, n_heads, head_dim] (rows may be strided); scale defaults to
+        head_dim^-0.5; positions, block_table and seqs as for qk_norm_rope.  A
+        negative position gives zeros.
+        """
+        check_tensor(q, "paged_attention q", torch.float32, self.torch_device, 3)
+        rows, heads, dim = q.shape
+        at = self._rows("paged_attention", rows, cache, positions, block_table, seqs)
+        if dim != cache.head_dim or (heads > 1 and q.stride(1) != dim):
+            raise _kernel_err(f"paged_attention q must hold heads of head_dim={cache.head_dim} side by side")
+        out = self._out(out, (rows, heads, dim), "paged_attention")
+        rc = self._lib.ocl_paged_attention(
+            self._ctx, q.data_ptr(), q.stride(0) if rows > 1 else heads * dim, rows, heads, cache.ref, C.byref(at),
+            dim ** -0.5 if scale is None else scale, out.data_ptr())
+        if rc:
+            self._check(rc)
+        return out
+
+    def _logits_call(self, op: str, logits: torch.Tensor, rules: LogitRules, out, ids) -> None:
+        check_tensor(logits, f"{op} logits", torch.float32, self.torch_device, 2)
+        if not isinstance(rules, LogitRules) or rules.device != self.torch_device:
+            raise _kernel_err(f"{op} rules must be LogitRules on {self.torch_device}")
+        rows, vocab = logits.shape
+        if rules.rows is not None and rules.rows != rows:
+            raise _kernel_err(f"{op} rules are for {rules.rows} rows, logits have {rows}")
+        if rules.words is not None and rules.words * 32 < vocab:
+            raise _kernel_err(f"{op} allowed mask has {rules.words} words a row, {vocab} tokens need {(vocab + 31) // 32}")
+        if out is not None:
+            check_tensor(out, f"{op} out", torch.float32, self.torch_device, 2)
+            if out.shape != logits.shape:
+                raise _kernel_err(f"{op} out {list(out.shape)} does not match logits {list(logits.shape)}")
+        if ids is not None:
+            check_tensor(ids, f"{op} ids", torch.int32, self.torch_device, 1)
+            if ids.shape[0] != rows:
+                raise _kernel_err(f"{op} ids.len()={ids.shape[0]} does not match rows={rows}")
+        rc = self._lib.ocl_logits_process(
+            self._ctx, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, rules.ref,
+            None if out is None else out.data_ptr(),
+            0 if out is None else out.stride(0) if rows > 1 else vocab, None if ids is None else ids.data_ptr())
+        if rc:
+            self._check(rc)
+
+    def process_logits(self, logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None,
+                       ids: torch.Tensor | None = None) -> torch.Tensor:
+        """Penalties, biases and the allowed-token mask on f32 [rows, vocab]; returns `out` (new when None).
+
+        out may be `logits` itself.  With ids (int32 [rows]) the greedy pick of the
+        result is written there in the same launch.
+        """
+        if out is None:
+            check_tensor(logits, "process_logits logits", torch.float32, self.torch_device, 2)
+            out = self._empty(tuple(logits.shape))
+        self._logits_call("process_logits", logits, rules, out, ids)
+        return out
+
     # -- greedy sampling (crates/runtime/src/sampling.rs:29) ----------------------
-    def greedy_sample(self, logits, out: torch.Tensor | None = None):
+    def greedy_sample(self, logits, out: torch.Tensor | None = None, rules: LogitRules | None = None):
         """Argmax per row of f32 logits with greedy_sample's tie and NaN rules.
+
+        With rules, the pick of the logits under them (see process_logits), in one
+        launch that leaves the logits as they are; then a [rows, vocab] or [vocab]
+        device tensor is wanted.
 
         logits: a contiguous f32 tensor on this device ([vocab] or [rows, vocab]),
         returning int32 ids on the device; or a host f32 array of one row,
         returning the id as an int (copied in and out).
         """
+        if rules is not None:
+            check_tensor(logits, "greedy_sample logits", torch.float32, self.torch_device,
+                         logits.dim() if isinstance(logits, torch.Tensor) and logits.dim() == 1 else 2)
+            if logits.dim() == 1:
+                logits = logits.unsqueeze(0)
+            if out is None:
+                out = self._empty((logits.shape[0],), torch.int32)
+            self._logits_call("greedy_sample", logits, rules, None, out)
+            return out
         if not isinstance(logits, torch.Tensor):
             arr = np.ascontiguousarray(logits, dtype=np.float32).reshape(-1)
             if arr.size == 0:

@@ -4,6 +4,7 @@
 // "unsupported before launch" rule of the reference's kernel design.
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -37,6 +38,8 @@ struct ocl_ctx {
     unsigned int* host_flags_dev = nullptr;  // the device address of host_flags
     uint16_t* xbf = nullptr;  // bf16 copy of x for the prefill GEMM form, grown on demand
     size_t xbf_bytes = 0;
+    float* attn_part = nullptr;             // attention: partial results of rows that several CTAs share
+    unsigned int* attn_counters = nullptr;  // attention: arrivals per shared row, zero between launches
     size_t gemm_min_rows = 64;  // rows at which ocl_q_linear switches to the tcgen05 GEMM (0 = never)
 };
 
@@ -55,6 +58,13 @@ struct ocl_qbuf {
     size_t n_rows = 0, k = 0, bytes = 0;
     void* dev = nullptr;
     bool gated = false;  // interleaved gate/up row tiles; n_rows = gate (= up) rows
+};
+
+struct ocl_rope {
+    int device = 0;
+    unsigned long long* steps = nullptr;  // [rot / 2], 2^64 * revolutions per position
+    int rot = 0;
+    bool interleaved = false;
 };
 
 namespace {
@@ -324,6 +334,79 @@ int take_timeouts(ocl_ctx* ctx, const char* op) {
                 "incomplete", op, n);
 }
 
+// Per-row slots and counters of the greedy pick (argmax and logit rules).
+int ensure_argmax(ocl_ctx* ctx) {
+    if (ctx->amax_counters) return OCL_OK;
+    const size_t sb = ocl::kArgmaxRowsMax * sizeof(unsigned long long), cb = ocl::kArgmaxRowsMax * sizeof(unsigned int);
+    if (!ctx->amax_slots) OCL_CUDA(ctx, cudaMalloc((void**)&ctx->amax_slots, sb), "cudaMalloc(argmax slots)");
+    OCL_CUDA(ctx, cudaMemsetAsync(ctx->amax_slots, 0, sb, ctx->stream), "memset argmax slots");
+    unsigned int* counters = nullptr;
+    OCL_CUDA(ctx, cudaMalloc((void**)&counters, cb), "cudaMalloc(argmax counters)");
+    const cudaError_t e = cudaMemsetAsync(counters, 0, cb, ctx->stream);
+    if (e != cudaSuccess) {
+        cudaFree(counters);
+        return cuda_fail(ctx, e, "memset argmax counters");
+    }
+    ctx->amax_counters = counters;
+    return OCL_OK;
+}
+
+bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+
+// Whether two [rows, width] f32 blocks share memory (by their whole extents).
+bool overlap(const float* a, size_t a_stride, const float* b, size_t b_stride, size_t rows, size_t a_width, size_t b_width) {
+    const uintptr_t a0 = (uintptr_t)a, a1 = a0 + ((rows - 1) * a_stride + a_width) * 4;
+    const uintptr_t b0 = (uintptr_t)b, b1 = b0 + ((rows - 1) * b_stride + b_width) * 4;
+    return a0 < b1 && b0 < a1;
+}
+
+// The cache, and where the rows stand, of the calls between the linear layers.
+int check_cache(ocl_ctx* ctx, const char* op, const ocl_kv_cache* c, const ocl_kv_rows* at, size_t rows,
+                size_t n_heads) {
+    if (!c || !at) return fail(ctx, OCL_ERR_INVALID, "%s cache / rows description is null", op);
+    if (c->dtype != OCL_KV_F16 && c->dtype != OCL_KV_BF16)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `cache type` (requested `%d`): supported = [F16(1), BF16(30)]",
+                    c->dtype);
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `head_dim` (requested `%zu`): supported = [64, 96, 128, 256]",
+                    c->head_dim);
+    if (!c->k_dev || !c->v_dev) return fail(ctx, OCL_ERR_INVALID, "%s cache pointer is null", op);
+    if (misaligned(c->k_dev) || misaligned(c->v_dev))
+        return fail(ctx, OCL_ERR_INVALID, "%s cache pointer is not 16-byte aligned", op);
+    if (c->n_pages == 0 || c->page_size == 0 || c->n_kv_heads == 0)
+        return fail(ctx, OCL_ERR_INVALID, "%s cache n_pages, page_size and n_kv_heads must be > 0", op);
+    if (c->n_pages > 0x7fffffff || c->page_size > 0x7fffffff || c->n_kv_heads > 65535)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `cache size` (requested `%zu pages of %zu, %zu heads`): "
+                    "supported = [< 2^31 pages, < 2^31 tokens a page, <= 65535 heads]", c->n_pages, c->page_size,
+                    c->n_kv_heads);
+    if (c->page_stride % 8 || c->head_stride % 8 || c->token_stride % 8 || c->token_stride < c->head_dim ||
+        (c->n_kv_heads > 1 && c->head_stride < c->head_dim) || (c->n_pages > 1 && c->page_stride < c->head_dim))
+        return fail(ctx, OCL_ERR_INVALID, "%s cache strides %zu, %zu, %zu must be multiples of 8 and at least head_dim=%zu",
+                    op, c->page_stride, c->head_stride, c->token_stride, c->head_dim);
+    if (n_heads == 0 || n_heads % c->n_kv_heads || n_heads > 65535)
+        return fail(ctx, OCL_ERR_INVALID, "%s n_heads=%zu is not a multiple of n_kv_heads=%zu up to 65535", op, n_heads,
+                    c->n_kv_heads);
+    if (rows > 0x3fffff)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `%s rows` (requested `%zu`): supported = [< 2^22]", op, rows);
+    if (rows && (!at->positions_dev || !at->block_table_dev)) return fail(ctx, OCL_ERR_INVALID, "%s positions / block table is null", op);
+    if (rows && (at->n_seqs == 0 || at->max_pages == 0)) return fail(ctx, OCL_ERR_INVALID, "%s block table is empty", op);
+    if (at->n_seqs > 0x7fffffff || at->max_pages > 0x7fffffff || at->table_stride < at->max_pages)
+        return fail(ctx, OCL_ERR_INVALID, "%s block table %zu x %zu with stride %zu is out of range", op, at->n_seqs,
+                    at->max_pages, at->table_stride);
+    if (!at->seqs_dev && rows > at->n_seqs)
+        return fail(ctx, OCL_ERR_INVALID, "%s rows=%zu exceed the block table's %zu sequences (and seqs is null)", op, rows,
+                    at->n_seqs);
+    return OCL_OK;
+}
+ocl::KvCache cache_of(const ocl_kv_cache* c) {
+    return {c->k_dev, c->v_dev, c->dtype, (int64_t)c->n_pages, (int64_t)c->page_size, (int64_t)c->n_kv_heads,
+            (int64_t)c->head_dim, (int64_t)c->page_stride, (int64_t)c->head_stride, (int64_t)c->token_stride};
+}
+ocl::KvRows rows_of(const ocl_kv_rows* at) {
+    return {at->positions_dev, at->seqs_dev, at->block_table_dev, (int64_t)at->n_seqs, (int64_t)at->max_pages,
+            (int64_t)at->table_stride};
+}
+
 }  // namespace
 
 namespace ocl {
@@ -359,8 +442,16 @@ int ocl_cuda_init(int device, ocl_ctx** out) {
     if (e == cudaSuccess) e = cudaMemset(ctx->dev_flags, 0, 64);
     if (e == cudaSuccess) e = cudaHostAlloc((void**)&ctx->host_flags, 64, cudaHostAllocMapped);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer((void**)&ctx->host_flags_dev, ctx->host_flags, 0);
+    // The attention workspace has one size for every call (a few MB): made here,
+    // it never moves under a captured launch.
+    if (e == cudaSuccess) e = cudaMalloc((void**)&ctx->attn_part, ocl::attention_part_bytes(ctx->sms));
+    if (e == cudaSuccess) e = cudaMalloc((void**)&ctx->attn_counters, ocl::attention_counters(ctx->sms) * 4);
+    if (e == cudaSuccess) e = cudaMemset(ctx->attn_counters, 0, ocl::attention_counters(ctx->sms) * 4);
     if (e != cudaSuccess) {
         if (ctx->dev_flags) cudaFree(ctx->dev_flags);
+        if (ctx->host_flags) cudaFreeHost(ctx->host_flags);
+        if (ctx->attn_part) cudaFree(ctx->attn_part);
+        if (ctx->attn_counters) cudaFree(ctx->attn_counters);
         delete ctx;
         return cuda_fail(nullptr, e, "context allocation");
     }
@@ -382,6 +473,8 @@ void ocl_cuda_destroy(ocl_ctx* ctx) {
         if (ctx->dev_flags) cudaFree(ctx->dev_flags);
         if (ctx->host_flags) cudaFreeHost(ctx->host_flags);
         if (ctx->xbf) cudaFree(ctx->xbf);
+        if (ctx->attn_part) cudaFree(ctx->attn_part);
+        if (ctx->attn_counters) cudaFree(ctx->attn_counters);
     }
     delete ctx;
 }
@@ -856,20 +949,163 @@ int ocl_argmax_f32(ocl_ctx* ctx, const float* logits_dev, size_t rows, size_t vo
                     "unsupported feature `argmax shape` (requested `%zu x %zu`): supported = [rows <= %d, vocab < 2^31]",
                     rows, vocab, ocl::kArgmaxRowsMax);
     DeviceGuard guard(ctx->device);
-    if (!ctx->amax_slots) {
-        OCL_CUDA(ctx, cudaMalloc((void**)&ctx->amax_slots, ocl::kArgmaxRowsMax * sizeof(unsigned long long)),
-                 "cudaMalloc(argmax slots)");
-        OCL_CUDA(ctx, cudaMalloc((void**)&ctx->amax_counters, ocl::kArgmaxRowsMax * sizeof(unsigned int)),
-                 "cudaMalloc(argmax counters)");
-        OCL_CUDA(ctx, cudaMemsetAsync(ctx->amax_slots, 0, ocl::kArgmaxRowsMax * sizeof(unsigned long long), ctx->stream),
-                 "memset argmax slots");
-        OCL_CUDA(ctx, cudaMemsetAsync(ctx->amax_counters, 0, ocl::kArgmaxRowsMax * sizeof(unsigned int), ctx->stream),
-                 "memset argmax counters");
-    }
+    const int rc = ensure_argmax(ctx);
+    if (rc) return rc;
     OCL_CUDA(ctx,
              ocl::launch_argmax(logits_dev, (int64_t)rows, (int64_t)vocab, ids_dev, ctx->amax_slots,
                                 ctx->amax_counters, ctx->stream),
              "argmax launch");
+    return OCL_OK;
+}
+
+int ocl_rope_create(ocl_ctx* ctx, size_t rot_dim, double base, const float* factors, int interleaved, ocl_rope** out) {
+    if (!ctx) return OCL_ERR_INVALID;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (!out) return fail(ctx, OCL_ERR_INVALID, "rope_create: out is null");
+    *out = nullptr;
+    if (rot_dim == 0 || rot_dim % 8 || rot_dim > 256)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `rot_dim` (requested `%zu`): supported = [multiples of 8 up to 256]",
+                    rot_dim);
+    if (!(base > 0) || !std::isfinite(base)) return fail(ctx, OCL_ERR_INVALID, "rope_create: base must be positive and finite");
+    unsigned long long steps[128];
+    for (size_t i = 0; i < rot_dim / 2; ++i) {
+        const float f = factors ? factors[i] : 1.0f;
+        if (!(f > 0) || !std::isfinite(f)) return fail(ctx, OCL_ERR_INVALID, "rope_create: factor %zu must be positive and finite", i);
+        // revolutions per position, modulo 1 (positions are whole), in 64-bit mantissas
+        const long double pi = 3.14159265358979323846264338327950288L;
+        long double turn = powl((long double)base, -2.0L * (long double)i / (long double)rot_dim) / (long double)f / (2 * pi);
+        turn -= floorl(turn);
+        const long double scaled = roundl(ldexpl(turn, 64));
+        steps[i] = scaled >= ldexpl(1.0L, 64) ? 0ull : (unsigned long long)scaled;
+    }
+    DeviceGuard guard(ctx->device);
+    ocl_rope* r = new ocl_rope();
+    r->device = ctx->device;
+    r->rot = (int)rot_dim;
+    r->interleaved = interleaved != 0;
+    cudaError_t e = cudaMalloc((void**)&r->steps, sizeof steps);
+    if (e == cudaSuccess) e = cudaMemcpy(r->steps, steps, rot_dim / 2 * sizeof steps[0], cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+        if (r->steps) cudaFree(r->steps);
+        delete r;
+        return cuda_fail(ctx, e, "rope_create");
+    }
+    *out = r;
+    return OCL_OK;
+}
+
+int ocl_rope_free(ocl_rope* r) {
+    if (!r) return OCL_OK;
+    DeviceGuard guard(r->device);
+    if (r->steps) cudaFree(r->steps);
+    delete r;
+    return OCL_OK;
+}
+
+int ocl_qk_norm_rope(ocl_ctx* ctx, const float* qkv, size_t qkv_stride, size_t rows, size_t n_heads,
+                     const ocl_kv_cache* cache, const ocl_kv_rows* at, const float* q_norm, const float* k_norm, float eps,
+                     const ocl_rope* rope, float* q_out) {
+    if (!ctx) return OCL_ERR_INVALID;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    const int rc = check_cache(ctx, "qk_norm_rope", cache, at, rows, n_heads);
+    if (rc) return rc;
+    const size_t width = (n_heads + 2 * cache->n_kv_heads) * cache->head_dim;
+    if (qkv_stride < width || qkv_stride % 4)
+        return fail(ctx, OCL_ERR_INVALID, "qk_norm_rope qkv row stride %zu must be a multiple of 4 and at least "
+                    "(n_heads + 2*n_kv_heads)*head_dim=%zu", qkv_stride, width);
+    if (!(eps >= 0)) return fail(ctx, OCL_ERR_INVALID, "qk_norm_rope eps must be >= 0");
+    if (rope && rope->device != ctx->device)
+        return fail(ctx, OCL_ERR_INVALID, "rope table lives on device %d but the context is on device %d", rope->device,
+                    ctx->device);
+    if (rope && (size_t)rope->rot > cache->head_dim)
+        return fail(ctx, OCL_ERR_INVALID, "qk_norm_rope rot_dim=%d exceeds head_dim=%zu", rope->rot, cache->head_dim);
+    if (rows == 0) return OCL_OK;
+    if (!qkv || !q_out) return fail(ctx, OCL_ERR_INVALID, "qk_norm_rope qkv/out pointer is null");
+    if (misaligned(qkv) || misaligned(q_out) || misaligned(q_norm) || misaligned(k_norm))
+        return fail(ctx, OCL_ERR_INVALID, "qk_norm_rope qkv, norms and out must be 16-byte aligned");
+    if (overlap(qkv, qkv_stride, q_out, n_heads * cache->head_dim, rows, width, n_heads * cache->head_dim))
+        return fail(ctx, OCL_ERR_INVALID, "qk_norm_rope out overlaps qkv");
+    DeviceGuard guard(ctx->device);
+    ocl::RopeTable t{nullptr, 0, false};
+    if (rope) t = {rope->steps, rope->rot, rope->interleaved};
+    OCL_CUDA(ctx,
+             ocl::launch_qk_norm_rope(qkv, (int64_t)qkv_stride, (int64_t)rows, (int64_t)n_heads, cache_of(cache),
+                                      rows_of(at), q_norm, k_norm, eps, t, q_out, ctx->dev_flags, ctx->sms, ctx->pdl,
+                                      ctx->stream),
+             "qk_norm_rope launch");
+    return OCL_OK;
+}
+
+int ocl_paged_attention(ocl_ctx* ctx, const float* q, size_t q_stride, size_t rows, size_t n_heads,
+                        const ocl_kv_cache* cache, const ocl_kv_rows* at, float scale, float* out) {
+    if (!ctx) return OCL_ERR_INVALID;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    const int rc = check_cache(ctx, "paged_attention", cache, at, rows, n_heads);
+    if (rc) return rc;
+    if (q_stride < n_heads * cache->head_dim || q_stride % 4)
+        return fail(ctx, OCL_ERR_INVALID, "paged_attention q row stride %zu must be a multiple of 4 and at least "
+                    "n_heads*head_dim=%zu", q_stride, n_heads * cache->head_dim);
+    if (!(scale > 0) || !std::isfinite(scale)) return fail(ctx, OCL_ERR_INVALID, "paged_attention scale must be positive and finite");
+    if (rows == 0) return OCL_OK;
+    if (!q || !out) return fail(ctx, OCL_ERR_INVALID, "paged_attention q/out pointer is null");
+    if (misaligned(q) || misaligned(out)) return fail(ctx, OCL_ERR_INVALID, "paged_attention q and out must be 16-byte aligned");
+    const size_t width = n_heads * cache->head_dim;
+    if (overlap(q, q_stride, out, width, rows, width, width))
+        return fail(ctx, OCL_ERR_INVALID, "paged_attention out overlaps q");
+    DeviceGuard guard(ctx->device);
+    OCL_CUDA(ctx,
+             ocl::launch_paged_attention(q, (int64_t)q_stride, (int64_t)rows, (int64_t)n_heads, cache_of(cache),
+                                         rows_of(at), scale, out, ctx->attn_part, ctx->attn_counters, ctx->dev_flags,
+                                         ctx->sms, ctx->pdl, ctx->stream),
+             "paged_attention launch");
+    return OCL_OK;
+}
+
+int ocl_logits_process(ocl_ctx* ctx, const float* logits, size_t in_stride, size_t rows, size_t vocab,
+                       const ocl_logit_rules* r, float* out, size_t out_stride, int32_t* ids) {
+    if (!ctx) return OCL_ERR_INVALID;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (vocab == 0) return fail(ctx, OCL_ERR_INVALID, "process_logits requires at least one logit");
+    if (!r) return fail(ctx, OCL_ERR_INVALID, "process_logits rules are null");
+    if (rows > (size_t)ocl::kArgmaxRowsMax || vocab > 0x7FFFFFFFu)
+        return fail(ctx, OCL_ERR_UNSUPPORTED,
+                    "unsupported feature `process_logits shape` (requested `%zu x %zu`): supported = [rows <= %d, vocab < 2^31]",
+                    rows, vocab, ocl::kArgmaxRowsMax);
+    if (in_stride < vocab || (out && out_stride < vocab))
+        return fail(ctx, OCL_ERR_INVALID, "process_logits row stride is below vocab=%zu", vocab);
+    if ((r->history_dev != nullptr) != (r->history_lens_dev != nullptr))
+        return fail(ctx, OCL_ERR_INVALID, "process_logits history and history_lens go together");
+    if (!r->history_dev && (r->prompt_lens_dev || r->repetition_dev || r->frequency_dev || r->presence_dev))
+        return fail(ctx, OCL_ERR_INVALID, "process_logits penalties need a history");
+    if ((r->bias_ids_dev != nullptr) != (r->bias_values_dev != nullptr))
+        return fail(ctx, OCL_ERR_INVALID, "process_logits bias ids and values go together");
+    if (r->allowed_dev && r->allowed_stride < (vocab + 31) / 32)
+        return fail(ctx, OCL_ERR_INVALID, "process_logits allowed mask has %zu words a row, %zu tokens need %zu",
+                    r->allowed_stride, vocab, (vocab + 31) / 32);
+    if (r->history_max > 0x7FFFFFFFu || r->bias_count > 0x7FFFFFFFu)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `process_logits history` (requested `%zu` tokens, `%zu` "
+                    "biases): supported = [< 2^31]", r->history_max, r->bias_count);
+    if ((r->history_dev && r->history_stride < r->history_max) || (r->bias_ids_dev && r->bias_stride < r->bias_count))
+        return fail(ctx, OCL_ERR_INVALID, "process_logits history / bias row stride is below the row's length");
+    if (rows == 0) return OCL_OK;
+    if (!logits) return fail(ctx, OCL_ERR_INVALID, "process_logits logits pointer is null");
+    if (!out && !ids) return fail(ctx, OCL_ERR_INVALID, "process_logits needs an output: logits, ids or both");
+    if (out == logits ? out_stride != in_stride
+                      : out && overlap(logits, in_stride, out, out_stride, rows, vocab, vocab))
+        return fail(ctx, OCL_ERR_INVALID, "process_logits out overlaps logits; in place needs the same pointer and row stride");
+    DeviceGuard guard(ctx->device);
+    if (ids) {
+        const int rc = ensure_argmax(ctx);
+        if (rc) return rc;
+    }
+    const ocl::LogitRules rules{r->history_dev, (int64_t)r->history_stride, (int64_t)r->history_max, r->history_lens_dev, r->prompt_lens_dev,
+                                r->repetition_dev, r->frequency_dev, r->presence_dev, r->bias_ids_dev,
+                                r->bias_values_dev, (int64_t)r->bias_stride, (int64_t)r->bias_count, r->allowed_dev, (int64_t)r->allowed_stride};
+    OCL_CUDA(ctx,
+             ocl::launch_logit_rules(logits, (int64_t)in_stride, (int64_t)rows, (int64_t)vocab, rules, out,
+                                     (int64_t)out_stride, ids, ctx->amax_slots, ctx->amax_counters, ctx->dev_flags,
+                                     ctx->sms, ctx->pdl, ctx->stream),
+             "process_logits launch");
     return OCL_OK;
 }
 

@@ -14,6 +14,7 @@
 // resets the slot and the counter for the next launch.
 #include <cuda_runtime.h>
 
+#include "device.cuh"
 #include "internal.cuh"
 
 namespace ocl {
@@ -21,12 +22,6 @@ namespace ocl {
 namespace {
 
 constexpr int kThreads = 256, kPerThread = 16, kChunk = kThreads * kPerThread;
-
-__device__ __forceinline__ unsigned long long key_of(float v, uint32_t idx) {
-    uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);  // -0.0 -> +0.0
-    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);       // monotone in v
-    return ((unsigned long long)b << 32) | (unsigned long long)(0xFFFFFFFFu - idx);
-}
 
 __global__ void __launch_bounds__(kThreads) argmax_kernel(const float* __restrict__ logits, int64_t vocab,
                                                           int32_t* __restrict__ ids,
@@ -51,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) argmax_kernel(const float* __restric
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (!isnan(v[e])) {
-                const unsigned long long k = key_of(v[e], (uint32_t)(i + e));
+                const unsigned long long k = greedy_key(v[e], (uint32_t)(i + e));
                 best = k > best ? k : best;
             }
     }

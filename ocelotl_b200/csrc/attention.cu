@@ -1,0 +1,526 @@
+// attention.cu -- attention of new tokens over the paged key/value cache.
+//
+// Row r holds token p = positions[r] of its sequence and sees tokens 0..p; query
+// head h reads k/v head h / G:
+//     s_j = scale * q . k_j,   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j
+// in one pass over the cache with a running m, sum and o.
+//
+// Bound: the cache is read once, 4 * head_dim bytes a token and k/v head, against
+// 4 * G * head_dim flops: HBM.  At f32 quality the flops do not fit the FMA units
+// beside that stream (G = 8: 52 TFLOP/s at 6.5 TB/s, plus the conversions), so they
+// run on the tensor cores: mma.sync m16n8k16 with the up to 8 query heads of a k/v
+// head as rows.  Half of the 16 rows would be empty; they carry the rest of the
+// precision instead.  A f32 factor (q, and the weights p_j) is cut into 16-bit
+// pieces that add up to it -- rows 0-7 the leading piece, rows 8-15 the next one,
+// for bf16 a third in a second MMA -- so every product is exact and the sum has f32
+// quality although q and p are never rounded to 16 bits:
+//     bf16: 3 pieces of 8 bits = 24 bits;   f16: 2 pieces of 11 bits = 22 bits
+// (q scaled by a power of two per head, p by 2^14, so that f16's range is enough).
+// The tensor core truncates when it adds; chains are kept short (two chains over
+// head_dim, one 16-token step for p.v) and joined with rounding f32 adds.
+//
+// Work split: the tiles (64 tokens of one row and k/v head) of all rows, in order,
+// are cut into equal runs, one per resident CTA, from the positions in device
+// memory -- so one captured launch stays balanced while the lengths grow.  Each of
+// the 4 warps streams its own 16 tokens of a tile through a private ring of
+// cp.async stages and needs no barrier inside a run.  A row whose tiles lie in
+// several CTAs is joined by the last of them to arrive, in CTA order: the result
+// does not depend on which one it is.  Nothing waits on another CTA.
+#include "device.cuh"
+#include "internal.cuh"
+
+namespace ocl {
+
+namespace {
+
+constexpr int kWarps = kTileWarps, kThreads = 32 * kWarps;
+constexpr int kHeads = 8;  // query heads of one k/v head worked on together
+
+constexpr int stages(int d) { return d <= 96 ? 4 : d == 128 ? 3 : 2; }
+constexpr int ctas_per_sm(int d) { return d == 64 ? 3 : d == 256 ? 1 : 2; }
+constexpr int max_ctas_per_sm = 3;
+constexpr int stage_bytes(int d) { return kWarpTok * d * 2 * 2; }  // k and v of 16 tokens
+constexpr bool q_in_smem(int d) { return d > 128; }
+constexpr int q_bytes(int d) { return q_in_smem(d) ? d / 16 * 32 * 24 : 0; }
+constexpr int slot_floats(int d) { return kHeads * d + 2 * kHeads; }
+constexpr int smem_bytes(int d) {
+    return kWarps * stages(d) * stage_bytes(d) + kWarps * kHeads * d * 4 + q_bytes(d);
+}
+
+struct AttnArgs {
+    const float* q;
+    int64_t q_stride;
+    int rows, n_heads, n_kv, group, head_groups;
+    KvCache kv;
+    KvRows at;
+    int cap;      // tokens a row of the block table can hold
+    float scale;  // in units of log2
+    float* out;
+    float* part;
+    unsigned int* counters;
+    unsigned int* err;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // bytes < 16: the rest is zero
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <class T> constexpr int kPieces = 3;
+template <> constexpr int kPieces<__half> = 2;
+template <class T> constexpr float kShift = 0.f;  // p is scaled by 2^kShift
+template <> constexpr float kShift<__half> = 14.f;
+
+// Two floats as N packed pairs of 16-bit pieces, leading piece first.
+template <int N, class T>
+__device__ __forceinline__ void cut(uint32_t (&w)[N], float a, float b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w[i] = pack16(a, b, T());
+        const float2 t = unpack16(w[i], T());
+        a -= t.x;
+        b -= t.y;
+    }
+}
+
+// 16-byte chunk of row `r` where chunk `c` is kept, so that 8 rows of one chunk
+// column (an ldmatrix) fall into different banks.
+template <int D>
+__device__ __forceinline__ int swizzle(int c, int r) {
+    return D % 64 == 0 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+}
+
+template <int D, class T>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D)) attention_kernel(const AttnArgs p) {
+    constexpr int S = stages(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
+    constexpr int kStage = stage_bytes(D);
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ long long scan[kWarps];
+    __shared__ int first_row, last_in;
+    __shared__ long long first_at;
+    __shared__ uint32_t valid[kWarps][S];
+    __shared__ float merge_m[kWarps][kHeads], merge_l[kWarps][kHeads];
+    float* merge_o = reinterpret_cast<float*>(smem + kWarps * S * kStage);
+    uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem + kWarps * S * kStage + kWarps * kHeads * D * 4);
+
+    grid_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
+    const int items = p.n_kv * p.head_groups;
+
+    // ---- this CTA's run of tiles
+    const int per = (p.rows + kThreads - 1) / kThreads;
+    const int r0 = min(tid * per, p.rows), r1 = min(r0 + per, p.rows);
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) mine += tiles_of(row_tokens(p.at, p.cap, r));
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += t;
+    }
+    if (lane == 31) scan[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += scan[w];
+        total += scan[w];
+    }
+    total *= items;
+    const long long P = total < (long long)gridDim.x ? total : (long long)gridDim.x;
+    const long long cta = blockIdx.x;
+    const long long begin = cta < P ? run_begin(total, P, cta) : total, end = cta < P ? run_begin(total, P, cta + 1) : total;
+    {
+        const long long b = (upto - mine) * items, e = upto * items;
+        if (begin < end && begin >= b && begin < e) {
+            long long at = b;
+            int r = r0;
+            for (;; ++r) {
+                const long long n = (long long)tiles_of(row_tokens(p.at, p.cap, r)) * items;
+                if (begin < at + n) break;
+                at += n;
+            }
+            first_row = r;
+            first_at = begin - at;
+        }
+    }
+    __syncthreads();
+
+    // rows without tokens are zeros; rows whose place is out of range are counted
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const int tokens = row_tokens(p.at, p.cap, r), pos = p.at.positions[r];
+        if (tid == 0 && pos >= 0 && pos >= tokens) atomicAdd(p.err, 1u);
+        if (tokens == 0)
+            for (int i = tid; i < p.n_heads * D; i += kThreads) p.out[(int64_t)r * p.n_heads * D + i] = 0.f;
+    }
+    if (begin >= end) return;
+
+    Cursor ld, cc;  // the tile to load next, the tile to compute next
+    ld.row = first_row;
+    ld.tokens = row_tokens(p.at, p.cap, ld.row);
+    ld.tiles = tiles_of(ld.tokens);
+    ld.item = (int)(first_at / ld.tiles);
+    ld.tile = (int)(first_at % ld.tiles);
+    cc = ld;
+    const int count = (int)(end - begin);
+    int to_load = count;
+
+    unsigned char* ring = smem + warp * S * kStage;
+    const T* kbase = static_cast<const T*>(p.kv.k);
+    const T* vbase = static_cast<const T*>(p.kv.v);
+
+    // Page of this lane's token (lanes 0-15) of the tile at `ld`: looked up one
+    // tile ahead of its loads.  -1: past the row's tokens, or no such page.
+    int page = -1, in_page = 0, head = 0;
+    auto look_up = [&]() {
+        page = -1;
+        if (to_load <= 0) return;
+        const int tok = ld.tile * kTileTok + warp * kWarpTok + (lane & 15);
+        if (tok < ld.tokens && !place_of(p.at, p.kv.n_pages, (int)p.kv.page_size, sequence_of(p.at, ld.row), tok, page, in_page)) {
+            page = -1;
+            if (ld.item == 0 && lane < 16) atomicAdd(p.err, 1u);
+        }
+        head = ld.item / p.head_groups;
+    };
+    auto load = [&](int stage) {
+        if (to_load > 0) {
+            const int64_t off = page < 0 ? -1
+                                         : (int64_t)page * p.kv.page_stride + (int64_t)in_page * p.kv.token_stride +
+                                               (int64_t)head * p.kv.head_stride;
+            const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+            if (lane == 0) valid[warp][stage] = have;
+            if (have) {
+                const uint32_t dk = smem_u32(ring + stage * kStage), dv = dk + kWarpTok * D * 2;
+#pragma unroll
+                for (int i = 0; i < kWarpTok * C / 32; ++i) {
+                    const int idx = i * 32 + lane, r = idx / C, ch = idx % C;
+                    const int64_t ro = __shfl_sync(0xffffffffu, off, r);
+                    const uint32_t at = (uint32_t)(r * D * 2 + swizzle<D>(ch, r) * 16);
+                    const int64_t el = ro < 0 ? 0 : ro + ch * 8;
+                    cp_async16(dk + at, kbase + el, ro < 0 ? 0 : 16);
+                    cp_async16(dv + at, vbase + el, ro < 0 ? 0 : 16);
+                }
+            }
+            --to_load;
+            if (++ld.tile == ld.tiles && to_load > 0) next_item(p.at, p.rows, p.cap, items, ld);
+            look_up();
+        }
+        cp_commit();
+    };
+
+    look_up();
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) load(s);
+
+    uint32_t qa[q_in_smem(D) ? 1 : KS][N * 2];  // A fragments: pieces of (k = 2c, 2c+1) and (k = 2c+8, 2c+9)
+    int stage = 0;
+    long long done = 0;  // tiles of the run behind cc
+    while (done < count) {
+        // ---- one item: query heads h0..h0+nh of a row, tiles [cc.tile, cc.tile + n)
+        const int n = (int)min((long long)(cc.tiles - cc.tile), (long long)count - done);
+        const int kvh = cc.item / p.head_groups, hg = cc.item % p.head_groups;
+        const int h0 = kvh * p.group + hg * kHeads, nh = min(kHeads, p.group - hg * kHeads);
+        float scale = p.scale;
+        {
+            const float* qr = p.q + (int64_t)cc.row * p.q_stride + (int64_t)(h0 + (g < nh ? g : 0)) * D + c4 * 2;
+            float2 x[KS][2];
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    x[k][j] = g < nh ? *reinterpret_cast<const float2*>(qr + k * 16 + j * 8) : make_float2(0.f, 0.f);
+                    top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
+                }
+            if constexpr (N == 2) {
+                // f16 pieces: bring the head's largest |q| into [2^7, 2^8)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = max(-100, min(100, 134 - (int)((__float_as_uint(top) >> 23) & 255)));
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                scale *= __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) x[k][j].x *= up, x[k][j].y *= up;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t w[2][N];
+                cut<N, T>(w[0], x[k][0].x, x[k][0].y);
+                cut<N, T>(w[1], x[k][1].x, x[k][1].y);
+                if constexpr (q_in_smem(D)) {
+                    if (k % kWarps == warp) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) q_frag[((k * N + i) * 2 + j) * 32 + lane] = w[j][i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) qa[k][2 * i] = w[0][i], qa[k][2 * i + 1] = w[1][i];
+                }
+            }
+        }
+        __syncthreads();  // q_frag is written; the previous item's merge buffers are read
+
+        float o[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = 0.f;
+        float m = -INFINITY, l = 0.f;  // running maximum (scaled, less kShift) and this lane's part of the sum
+
+        for (int t = 0; t < n; ++t) {
+            cp_wait<S - 2>();
+            __syncwarp();
+            const int cur = stage;
+            load(stage == 0 ? S - 1 : stage - 1);  // the stage that the previous tile freed
+            stage = stage + 1 == S ? 0 : stage + 1;
+            const uint32_t have = valid[warp][cur];
+            if (have == 0) continue;
+            const uint32_t sk = smem_u32(ring + cur * kStage), sv = sk + kWarpTok * D * 2;
+
+            // ---- s = q . k for 16 tokens: two 8-token MMA columns
+            float acc[2][2][4] = {}, low[2][4] = {};
+            {
+                const int r = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t b[4], a[N * 2];
+                    ldmatrix4(b, sk + r * D * 2 + swizzle<D>(2 * k + hi, r) * 16);
+                    if constexpr (q_in_smem(D)) {
+#pragma unroll
+                        for (int i = 0; i < N * 2; ++i) a[i] = q_frag[(k * N * 2 + i) * 32 + lane];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < N * 2; ++i) a[i] = qa[k][i];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        mma(acc[j][k & 1], a[0], a[2], a[1], a[3], b[2 * j], b[2 * j + 1], T());
+                        if constexpr (N == 3) mma(low[j], a[4], 0u, a[5], 0u, b[2 * j], b[2 * j + 1], T());
+                    }
+                }
+            }
+            float s[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = i >> 1, e = i & 1;
+                s[i] = (acc[j][0][e] + acc[j][1][e]) + ((acc[j][0][e + 2] + acc[j][1][e + 2]) + low[j][e]);
+                if (!((have >> (8 * j + 2 * c4 + e)) & 1)) s[i] = -INFINITY;
+            }
+            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m, top * scale - kShift<T>);
+            const float ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = exp2f(m - ref);
+            m = m_new;
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = exp2f(fmaf(s[i], scale, -ref));
+            l = l * alpha + ((w[0] + w[1]) + (w[2] + w[3]));
+
+            // ---- o = o * alpha + p . v
+            uint32_t pa[2][N];
+            cut<N, T>(pa[0], w[0], w[1]);
+            cut<N, T>(pa[1], w[2], w[3]);
+            {
+                const int r = lane & 15, hi = lane >> 4;
+#pragma unroll
+                for (int c = 0; c < NT; c += 2) {
+                    uint32_t b[4];
+                    ldmatrix4_t(b, sv + r * D * 2 + swizzle<D>(c + hi, r) * 16);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float d[4] = {};
+                        if constexpr (N == 3) mma(d, pa[0][2], 0u, pa[1][2], 0u, b[2 * j], b[2 * j + 1], T());
+                        mma(d, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b[2 * j], b[2 * j + 1], T());
+                        o[c + j][0] = fmaf(o[c + j][0], alpha, d[0] + d[2]);
+                        o[c + j][1] = fmaf(o[c + j][1], alpha, d[1] + d[3]);
+                    }
+                }
+            }
+        }
+
+        // ---- join the four warps
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (c4 == 0) merge_m[warp][g] = m, merge_l[warp][g] = l;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            *reinterpret_cast<float2*>(merge_o + (warp * kHeads + g) * D + ((t * 8 + c4 * 2) ^ ((g & 3) << 3))) =
+                make_float2(o[t][0], o[t][1]);
+        __syncthreads();
+        const long long item_begin = begin + done - cc.tile, item_end = item_begin + cc.tiles;
+        const long long c0 = run_of(total, P, item_begin), c1 = run_of(total, P, item_end - 1);
+        const bool whole = c0 == c1;
+        float* slot = p.part + (2 * cta + (cta == c0 ? 1 : 0)) * slot_floats(D);
+#pragma unroll
+        for (int i = 0; i < (kHeads * D / 4 + kThreads - 1) / kThreads; ++i) {
+            const int idx = i * kThreads + tid;
+            if (idx >= kHeads * D / 4) break;
+            const int h = idx / (D / 4), col = idx % (D / 4) * 4;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge_m[w][h]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = exp2f(merge_m[w][h] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(merge_o + (w * kHeads + h) * D + (col ^ ((h & 3) << 3)));
+                sum += merge_l[w][h] * f;
+                a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
+            }
+            if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                if (h < nh)
+                    *reinterpret_cast<float4*>(p.out + ((int64_t)cc.row * p.n_heads + h0 + h) * D + col) =
+                        make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            } else if (h < nh) {
+                __stcg(reinterpret_cast<float4*>(slot + h * D + col), a);
+                if (col == 0) {
+                    __stcg(slot + kHeads * D + h, top);
+                    __stcg(slot + kHeads * D + kHeads + h, sum);
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                last_in = atomicAdd(p.counters + c0, 1u) == (unsigned)(c1 - c0);
+                if (last_in) p.counters[c0] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (last_in) {
+                // ---- this CTA is the last one of the item: join all, in CTA order
+                const int parts = (int)(c1 - c0) + 1;
+                const float* first = p.part + (2 * c0 + 1) * slot_floats(D);
+                const float* rest = p.part + 2 * c0 * slot_floats(D);
+                auto part_of = [&](int i) { return i == 0 ? first : rest + (int64_t)2 * i * slot_floats(D); };
+                for (int h = warp; h < nh; h += kWarps) {
+                    float top = -INFINITY;
+                    for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(part_of(i) + kHeads * D + h));
+#pragma unroll
+                    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    float sum = 0.f;
+                    for (int i = lane; i < parts; i += 32)
+                        sum += __ldcg(part_of(i) + kHeads * D + kHeads + h) * exp2f(__ldcg(part_of(i) + kHeads * D + h) - ref);
+#pragma unroll
+                    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+                    if (lane == 0) merge_m[0][h] = ref, merge_l[0][h] = sum == 0.f ? 0.f : 1.0f / sum;
+                }
+                __syncthreads();
+                for (int idx = tid; idx < nh * (D / 4); idx += kThreads) {
+                    const int h = idx / (D / 4), col = idx % (D / 4) * 4;
+                    const float ref = merge_m[0][h], inv = merge_l[0][h];
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int i = 0; i < parts; ++i) {
+                        const float f = exp2f(__ldcg(part_of(i) + kHeads * D + h) - ref);
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(i) + h * D + col));
+                        a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
+                    }
+                    *reinterpret_cast<float4*>(p.out + ((int64_t)cc.row * p.n_heads + h0 + h) * D + col) =
+                        make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+                }
+            }
+        }
+        done += n;
+        if (done < count) next_item(p.at, p.rows, p.cap, items, cc);
+    }
+    cp_wait<0>();
+}
+
+template <int D, class T>
+cudaError_t launch_typed(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
+    static bool configured[kMaxDevices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= kMaxDevices || !configured[dev]) {
+        e = cudaFuncSetAttribute(attention_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
+        if (e != cudaSuccess) return e;
+        if (dev < kMaxDevices) configured[dev] = true;
+    }
+    const int64_t tiles = (int64_t)a.rows * a.n_kv * a.head_groups * ((a.cap + kTileTok - 1) / kTileTok);
+    const int64_t ctas = (int64_t)sms * ctas_per_sm(D);
+    return launch_kernel(attention_kernel<D, T>, dim3((unsigned)(tiles < ctas ? tiles : ctas)), kThreads, smem_bytes(D),
+                         pdl, s, a);
+}
+
+template <int D>
+cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
+    return a.kv.type == kKvBf16 ? launch_typed<D, __nv_bfloat16>(a, sms, pdl, s) : launch_typed<D, __half>(a, sms, pdl, s);
+}
+
+}  // namespace
+
+size_t attention_part_bytes(int sms) {
+    size_t most = 0;
+    for (int d : {64, 96, 128, 256}) {
+        const size_t b = (size_t)sms * ctas_per_sm(d) * 2 * slot_floats(d) * 4;
+        most = b > most ? b : most;
+    }
+    return most;
+}
+size_t attention_counters(int sms) { return (size_t)sms * max_ctas_per_sm; }
+
+cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t rows, int64_t n_heads, const KvCache& kv,
+                                   const KvRows& at, float scale, float* out, float* part, unsigned int* counters,
+                                   unsigned int* err, int sms, bool pdl, cudaStream_t s) {
+    AttnArgs a{};
+    a.q = q;
+    a.q_stride = q_stride;
+    a.rows = (int)rows;
+    a.n_heads = (int)n_heads;
+    a.n_kv = (int)kv.n_kv;
+    a.group = (int)(n_heads / kv.n_kv);
+    a.head_groups = (a.group + kHeads - 1) / kHeads;
+    a.kv = kv;
+    a.at = at;
+    const int64_t cap = at.max_pages * kv.page_size;
+    a.cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
+    a.scale = scale * 1.4426950408889634f;
+    a.out = out;
+    a.part = part;
+    a.counters = counters;
+    a.err = err;
+    switch (kv.head_dim) {
+        case 64: return launch_dim<64>(a, sms, pdl, s);
+        case 96: return launch_dim<96>(a, sms, pdl, s);
+        case 128: return launch_dim<128>(a, sms, pdl, s);
+        case 256: return launch_dim<256>(a, sms, pdl, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace ocl

@@ -5,6 +5,7 @@
 #include <cstdint>
 
 #include "layout.cuh"
+#include "paging.cuh"
 
 namespace ocl {
 
@@ -132,6 +133,60 @@ cudaError_t launch_gemv_gated(int type, const void* tiles, int64_t n_gate, int64
 constexpr int kArgmaxRowsMax = 65535;
 cudaError_t launch_argmax(const float* logits, int64_t rows, int64_t vocab, int32_t* ids,
                           unsigned long long* slots, unsigned int* counters, cudaStream_t s);
+
+// ---- decode-step operators between the linear layers -----------------------
+
+constexpr int kKvF16 = 1, kKvBf16 = 30;  // cache element types (GGUF tensor-type tags)
+
+// A paged key/value cache: token t of a sequence sits in page
+// table[seq][t / page_size], slot t % page_size; strides in elements.
+struct KvCache {
+    void *k, *v;
+    int type;
+    int64_t n_pages, page_size, n_kv, head_dim;
+    int64_t page_stride, head_stride, token_stride;
+};
+// Rotation of pairs i < rot/2 by positions * 2 pi * steps[i] / 2^64.
+struct RopeTable {
+    const unsigned long long* steps;
+    int rot;
+    bool interleaved;
+};
+
+// q f32 [rows, n_heads, head_dim] = rotate(norm(q of qkv)), and the same of k
+// with v (plain) rounded into the cache.  qkv rows are q | k | v heads.
+cudaError_t launch_qk_norm_rope(const float* qkv, int64_t qkv_stride, int64_t rows, int64_t n_heads, const KvCache& kv,
+                                const KvRows& at, const float* q_norm, const float* k_norm, float eps,
+                                const RopeTable& rope, float* q_out, unsigned int* err, int sms, bool pdl,
+                                cudaStream_t s);
+
+// out f32 [rows, n_heads, head_dim]: attention of row r over tokens
+// 0..positions[r] of its sequence.  part / counters: workspace of the joined
+// lengths (attention_workspace_bytes; counters zero between launches).
+size_t attention_part_bytes(int sms);
+size_t attention_counters(int sms);
+cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t rows, int64_t n_heads, const KvCache& kv,
+                                   const KvRows& at, float scale, float* out, float* part, unsigned int* counters,
+                                   unsigned int* err, int sms, bool pdl, cudaStream_t s);
+
+// Penalties, biases and the allowed-token mask of one call; null = off.
+struct LogitRules {
+    const int32_t* history;       // [rows, history_max], row r's first history_lens[r] tokens count
+    int64_t history_stride, history_max;
+    const int32_t *history_lens, *prompt_lens;
+    const float *repetition, *frequency, *presence;  // [rows]
+    const int32_t* bias_ids;      // [rows, bias_count], negative = unused
+    const float* bias_values;
+    int64_t bias_stride, bias_count;
+    const uint32_t* allowed;      // [rows, allowed_stride] words, bit t % 32 of word t / 32
+    int64_t allowed_stride;
+};
+// out (may be logits itself, or null) = the ruled logits; ids (or null) = their
+// greedy pick, with slots / counters as for launch_argmax.
+cudaError_t launch_logit_rules(const float* logits, int64_t in_stride, int64_t rows, int64_t vocab,
+                               const LogitRules& rules, float* out, int64_t out_stride, int32_t* ids,
+                               unsigned long long* slots, unsigned int* counters, unsigned int* err, int sms, bool pdl,
+                               cudaStream_t s);
 
 // Prefill GEMM: y bf16 [M, N] = x bf16 [M, K] . W^T on tcgen05 (K a multiple of 256).
 // gated_n_out > 0: W is an interleaved gate/up pair with N = 2 * 16 * row tiles

@@ -1,0 +1,189 @@
+// rope.cu -- norms of q and k per head, position rotation and the cache write in one pass.
+//
+// Row r of qkv (the fused projection's output) is n_heads q heads, n_kv k heads
+// and n_kv v heads of head_dim floats.  For each q and k head x:
+//     y = x * rsqrt(mean(x^2) + eps) * w            (no norm when w is null)
+//     (y_a, y_b) of pair i < rot/2 turned by t = position * freq_i, where the pair is
+//     (i, i + rot/2), or (2i, 2i + 1) when interleaved; the rest passes through.
+// q goes out in f32 (the attention's input), k and v into their page, rounded to
+// nearest even.
+//
+// The angle: freq_i is held in revolutions as a 64-bit fixed-point fraction, so
+// position * step wraps modulo one revolution exactly and the phase is good to
+// position * 2^-65 revolutions at any 31-bit position; an f32 product loses
+// 2^-24 of the whole angle instead (0.008 rad at position 131072).
+//
+// One warp per head, one or more CTAs per row (the host splits the heads of few
+// rows over CTAs); the row's cos and sin are computed once per CTA.
+#include "device.cuh"
+#include "internal.cuh"
+
+namespace ocl {
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+
+struct RopeArgs {
+    const float* qkv;
+    int64_t qkv_stride;
+    int n_heads, n_kv, groups;  // groups: CTAs per row
+    KvCache kv;
+    KvRows at;
+    const float *q_norm, *k_norm;
+    float eps;
+    RopeTable rope;
+    float* q_out;
+    unsigned int* err;
+};
+
+template <int V>
+__device__ __forceinline__ void load_vec(float (&d)[V], const float* p) {
+    if constexpr (V == 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p);
+        d[0] = t.x; d[1] = t.y; d[2] = t.z; d[3] = t.w;
+    } else if constexpr (V == 2) {
+        const float2 t = *reinterpret_cast<const float2*>(p);
+        d[0] = t.x; d[1] = t.y;
+    } else {
+        d[0] = *p;
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(float* p, const float (&d)[V]) {
+    if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(d[0], d[1], d[2], d[3]);
+    else if constexpr (V == 2) *reinterpret_cast<float2*>(p) = make_float2(d[0], d[1]);
+    else *p = d[0];
+}
+template <int V, class T>
+__device__ __forceinline__ void store_vec(T* p, const float (&d)[V]) {
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack16(d[0], d[1], T()), pack16(d[2], d[3], T()));
+    else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = pack16(d[0], d[1], T());
+    else *p = T(d[0]);
+}
+
+// A lane holds V pairs of its head: V elements at `a` and V at `b`.
+template <int D, int V, class T>
+__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p) {
+    static_assert(D / 2 <= 32 * V, "one lane step covers a head");
+    __shared__ float2 turn[D / 2];
+    grid_wait();
+    const int64_t row = blockIdx.x / p.groups;
+    const int group = blockIdx.x % p.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pos = p.at.positions[row];
+    const int half = p.rope.rot / 2;
+    if ((int)threadIdx.x < half) {
+        const unsigned long long phase = (unsigned long long)(long long)pos * p.rope.steps[threadIdx.x];
+        float s, c;
+        sincospif((float)(long long)phase * 0x1p-63f, &s, &c);  // phase as a signed fraction of a revolution
+        turn[threadIdx.x] = make_float2(c, s);
+    }
+    // the row's page: -1 when nothing is to be cached
+    int64_t slot = -1;
+    if (pos >= 0) {
+        const int64_t seq = sequence_of(p.at, row);
+        int page = -1, in_page = 0;
+        const bool ok = seq >= 0 && place_of(p.at, p.kv.n_pages, (int)p.kv.page_size, seq, pos, page, in_page);
+        slot = page * p.kv.page_stride + in_page * p.kv.token_stride;
+        if (!ok) {
+            slot = -1;
+            if (threadIdx.x == 0 && group == 0) atomicAdd(p.err, 1u);
+        }
+    }
+    __syncthreads();
+    const int i0 = lane * V;  // first pair
+    const int heads = p.n_heads + 2 * p.n_kv;
+    const bool active = i0 < D / 2;  // other lanes only take part in the reductions
+    for (int h = group * kWarps + warp; h < heads; h += p.groups * kWarps) {
+        const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.n_kv;
+        const bool turned = !is_v && i0 < half, halves = turned && !p.rope.interleaved;
+        const int a = halves ? i0 : 2 * i0, b = halves ? i0 + half : 2 * i0 + V;
+        float x[V] = {}, y[V] = {};
+        if (active && pos >= 0) {
+            const float* src = p.qkv + row * p.qkv_stride + (int64_t)h * D;
+            load_vec<V>(x, src + a);
+            load_vec<V>(y, src + b);
+        }
+        const float* w = is_v || pos < 0 ? nullptr : is_q ? p.q_norm : p.k_norm;
+        if (w) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
+            if (active) {
+                float wa[V], wb[V];
+                load_vec<V>(wa, w + a);
+                load_vec<V>(wb, w + b);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[e] *= inv * wa[e];
+                    y[e] *= inv * wb[e];
+                }
+            }
+        }
+        if (turned && !p.rope.interleaved) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float2 t = turn[i0 + e];
+                const float u = x[e], v = y[e];
+                x[e] = u * t.x - v * t.y;
+                y[e] = v * t.x + u * t.y;
+            }
+        } else if (turned) {
+            float z[2 * V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] = x[e], z[V + e] = y[e];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float2 t = turn[i0 + e];
+                const float u = z[2 * e], v = z[2 * e + 1];
+                z[2 * e] = u * t.x - v * t.y;
+                z[2 * e + 1] = v * t.x + u * t.y;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = z[e], y[e] = z[V + e];
+        }
+        if (!active) continue;
+        if (is_q) {
+            float* dst = p.q_out + (row * p.n_heads + h) * D;
+            store_vec<V>(dst + a, x);
+            store_vec<V>(dst + b, y);
+        } else if (slot >= 0) {
+            T* dst = static_cast<T*>(is_v ? p.kv.v : p.kv.k) + slot +
+                     (int64_t)(h - p.n_heads - (is_v ? p.n_kv : 0)) * p.kv.head_stride;
+            store_vec<V>(dst + a, x);
+            store_vec<V>(dst + b, y);
+        }
+    }
+}
+
+template <int D, int V>
+cudaError_t launch_dim(const RopeArgs& a, int64_t rows, bool pdl, cudaStream_t s) {
+    const dim3 grid((unsigned)(rows * a.groups));
+    return a.kv.type == kKvBf16 ? launch_kernel(qk_norm_rope_kernel<D, V, __nv_bfloat16>, grid, kThreads, 0, pdl, s, a)
+                                : launch_kernel(qk_norm_rope_kernel<D, V, __half>, grid, kThreads, 0, pdl, s, a);
+}
+
+}  // namespace
+
+cudaError_t launch_qk_norm_rope(const float* qkv, int64_t qkv_stride, int64_t rows, int64_t n_heads, const KvCache& kv,
+                                const KvRows& at, const float* q_norm, const float* k_norm, float eps,
+                                const RopeTable& rope, float* q_out, unsigned int* err, int sms, bool pdl,
+                                cudaStream_t s) {
+    RopeArgs a{qkv, qkv_stride, (int)n_heads, (int)kv.n_kv, 1, kv, at, q_norm, k_norm, eps, rope, q_out, err};
+    const int64_t most = (n_heads + 2 * kv.n_kv + kWarps - 1) / kWarps;  // CTAs a row can use
+    const int64_t want = (sms + rows - 1) / rows;
+    a.groups = (int)(want < most ? want : most);
+    if (rows * a.groups > 0x7fffffff) return cudaErrorInvalidValue;
+    switch (kv.head_dim) {
+        case 64: return launch_dim<64, 1>(a, rows, pdl, s);
+        case 96: return launch_dim<96, 2>(a, rows, pdl, s);
+        case 128: return launch_dim<128, 2>(a, rows, pdl, s);
+        case 256: return launch_dim<256, 4>(a, rows, pdl, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace ocl

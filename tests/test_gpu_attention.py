@@ -1,0 +1,288 @@
+"""GPU: attention of new tokens over the paged cache vs the formula in 64 bits."""
+import pytest
+import torch
+
+from ocelotl_b200.errors import KernelError, UnsupportedError
+from tests.decode_cases import attention_reference, paged
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_device_errors(backend):
+    backend.take_device_errors()
+    yield
+    assert backend.take_device_errors() == (0, 0)
+
+
+def positions_of(lengths):
+    return torch.tensor([n - 1 for n in lengths], dtype=torch.int32, device="cuda")
+
+
+def check(backend, lengths, kv_heads, group, dim, page, dtype, seed=1, layout="hnd", scale=None, fill=None, sharp=1.0):
+    k, v, table = paged(lengths, page, kv_heads, dim, dtype, seed, layout, fill=fill)
+    g = torch.Generator("cuda").manual_seed(seed + 1)
+    q = torch.randn(len(lengths), kv_heads * group, dim, device="cuda", generator=g) * sharp
+    pos = positions_of(lengths)
+    out = torch.full_like(q, float("nan"))
+    got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, scale=scale, out=out)
+    backend.synchronize()
+    assert got is out
+    want, bound = attention_reference(q, k, v, pos, table, dim ** -0.5 if scale is None else scale)
+    off = (got.double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert (off <= bound).all(), ((off / bound.clamp(min=1e-300)).max().item(), lengths)
+    # and as a whole: f32 quality, far below one rounding of anything to 16 bits (2^-9)
+    if want.norm() > 0:
+        assert (off.norm() / want.norm()).item() < 2.0 ** -17
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_one_row(backend, dim, dtype):
+    for n in (1, 2, 15, 16, 17, 63, 64, 65, 200):
+        check(backend, [n], 2, 4, dim, 16, dtype, seed=n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_ragged_batch_with_empty_rows(backend, dim, dtype):
+    check(backend, [0, 1, 700, 64, 0, 129, 31, 5000, 0], 4, 7, dim, 16, dtype, seed=dim)
+
+
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (8, 1), (1, 8), (3, 5), (2, 9), (1, 20), (2, 16)])
+def test_head_groups(backend, kv_heads, group):
+    check(backend, [77, 300, 1], kv_heads, group, 128, 32, torch.bfloat16, seed=group)
+
+
+@pytest.mark.parametrize("page", [1, 3, 7, 16, 24, 100, 256, 1000])
+def test_page_sizes(backend, page):
+    check(backend, [333, 47, 1025], 2, 4, 128, page, torch.bfloat16, seed=page)
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_layouts(backend, layout, dtype):
+    check(backend, [500, 33], 4, 4, 128, 16, dtype, layout=layout)
+
+
+@pytest.mark.parametrize("n,kv_heads", [(9000, 8), (60001, 1), (30000, 2)])
+def test_one_row_over_many_ctas(backend, n, kv_heads):
+    check(backend, [n], kv_heads, 4, 128, 16, torch.bfloat16)
+    check(backend, [n], kv_heads, 3, 64, 16, torch.float16)
+    check(backend, [n], kv_heads, 8, 256, 64, torch.bfloat16)
+
+
+def test_many_short_rows(backend):
+    check(backend, [(i * 37) % 150 for i in range(400)], 2, 7, 64, 16, torch.float16)
+
+
+@pytest.mark.parametrize("scale,sharp", [(1e-6, 1.0), (1.0, 1.0), (0.0884, 8.0)])
+def test_flat_and_peaked_weights(backend, scale, sharp):
+    for dtype in (torch.bfloat16, torch.float16):
+        check(backend, [400, 2000], 2, 4, 128, 16, dtype, scale=scale, sharp=sharp)
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), -float("inf"), 3e4])
+def test_slots_behind_a_sequence_do_not_count(backend, fill):
+    for dtype in (torch.bfloat16, torch.float16):
+        check(backend, [70, 1, 0, 333, 16], 2, 4, 128, 48, dtype, fill=fill)
+
+
+def test_large_and_tiny_queries(backend):
+    # f16 pieces are scaled per head: magnitudes far outside f16's range keep their precision
+    k, v, table = paged([100, 100, 100], 16, 1, 128, torch.float16, 5)
+    q = torch.randn(3, 2, 128, device="cuda") * torch.tensor([1e6, 1.0, 1e-9], device="cuda")[:, None, None]
+    pos = positions_of([100] * 3)
+    for scale in (1e-6, 1.0):
+        got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, scale=scale)
+        backend.synchronize()
+        want, bound = attention_reference(q, k, v, pos, table, scale)
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_nan_in_a_seen_token_reaches_only_its_heads(backend):
+    k, v, table = paged([90, 90], 16, 2, 128, torch.bfloat16, 5)
+    k[table[0, 2].long(), 1, 3, 7] = float("nan")  # token 35 of sequence 0, k/v head 1
+    q = torch.randn(2, 8, 128, device="cuda")
+    got = backend.paged_attention(q, backend.kv_cache_view(k, v), positions_of([90, 90]), table)
+    backend.synchronize()
+    assert torch.isnan(got[0, 4:]).all()
+    assert torch.isfinite(got[0, :4]).all() and torch.isfinite(got[1]).all()
+
+
+def test_several_rows_of_one_sequence_are_causal(backend):
+    k, v, table = paged([40, 700, 9], 16, 2, 128, torch.bfloat16, 6)
+    seqs = torch.tensor([1, 1, 1, 0, 2, 1, 0, 2], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([699, 698, 0, 39, 8, 64, -1, 3], dtype=torch.int32, device="cuda")
+    q = torch.randn(8, 8, 128, device="cuda")
+    got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, seqs=seqs)
+    backend.synchronize()
+    want, bound = attention_reference(q, k, v, pos, table, 128 ** -0.5, seqs)
+    assert ((got.double() - want).abs() <= bound).all()
+    assert (got[6] == 0).all()
+
+
+def test_strided_queries_tables_and_neighbours(backend):
+    k, v, table = paged([90, 200], 16, 2, 64, torch.bfloat16, 7)
+    wide = torch.full((2, 40), 12345, dtype=torch.int32, device="cuda")
+    wide[:, 5:5 + table.shape[1]] = table
+    qkv = torch.randn(2, (8 + 4) * 64, device="cuda")
+    q = qkv[:, :8 * 64].view(2, 8, 64)
+    pos = positions_of([90, 200])
+    out = torch.full((4, 8, 64), 7.0, device="cuda")
+    backend.paged_attention(q, backend.kv_cache_view(k, v), pos, wide[:, 5:5 + table.shape[1]], out=out[1:3])
+    backend.synchronize()
+    want, bound = attention_reference(q, k, v, pos, table, 64 ** -0.5)
+    assert ((out[1:3].double() - want).abs() <= bound).all()
+    assert (out[0] == 7).all() and (out[3] == 7).all()
+
+
+def test_same_bits_again(backend):
+    lengths = [5000, 3, 0, 1200, 64]
+    a = check(backend, lengths, 4, 4, 128, 16, torch.bfloat16)
+    b = check(backend, lengths, 4, 4, 128, 16, torch.bfloat16)
+    assert torch.equal(a, b)
+
+
+def test_cache_offsets_past_32_bits(backend):
+    pages, kv, page, dim = 36000, 8, 64, 128  # 2.36e9 elements
+    k = torch.empty(pages, kv, page, dim, dtype=torch.bfloat16, device="cuda")
+    v = torch.empty_like(k)
+    table = torch.tensor([[pages - 1, 2, pages - 2]], dtype=torch.int32, device="cuda")
+    for p in table[0].tolist():
+        k[p].normal_()
+        v[p].normal_()
+    q = torch.randn(1, 32, dim, device="cuda")
+    pos = positions_of([3 * 64 - 5])
+    got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table)
+    backend.synchronize()
+    want, bound = attention_reference(q, k, v, pos, table, dim ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_captured_launch_follows_the_positions(backend):
+    k, v, table = paged([1500, 1500], 16, 2, 128, torch.bfloat16, 8)
+    cache = backend.kv_cache_view(k, v)
+    q = torch.randn(2, 8, 128, device="cuda")
+    pos = positions_of([3, 1])
+    out = torch.empty_like(q)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            backend.use_current_stream()
+            backend.paged_attention(q, cache, pos, table, out=out)
+    finally:
+        backend.set_stream(None)
+    for lengths in ([3, 1], [1500, 0], [700, 1499], [64, 65]):
+        pos.copy_(positions_of(lengths))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, bound = attention_reference(q, k, v, pos, table, 128 ** -0.5)
+        assert ((out.double() - want).abs() <= bound).all(), lengths
+        # an eager call between replays shares the workspace
+        eager = backend.paged_attention(q, cache, pos, table)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, out)
+
+
+def test_on_a_side_stream(backend):
+    k, v, table = paged([900], 16, 2, 128, torch.bfloat16, 9)
+    stream = torch.cuda.Stream()
+    q0 = torch.randn(1, 8, 128, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(stream):
+            backend.use_current_stream()
+            torch.cuda._sleep(20_000_000)
+            q = q0 * 2
+            got = backend.paged_attention(q, backend.kv_cache_view(k, v), positions_of([900]), table)
+        stream.synchronize()
+        # outputs of a call made under another current stream live on the backend's stream
+        other = backend.paged_attention(q, backend.kv_cache_view(k, v), positions_of([900]), table)
+        stream.synchronize()
+    finally:
+        backend.set_stream(None)
+    assert torch.equal(got, other)
+    want, bound = attention_reference(q, k, v, positions_of([900]), table, 128 ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_no_rows(backend):
+    k, v, table = paged([10], 16, 2, 128, torch.bfloat16, 9)
+    got = backend.paged_attention(torch.empty(0, 8, 128, device="cuda"), backend.kv_cache_view(k, v),
+                                  torch.empty(0, dtype=torch.int32, device="cuda"), table)
+    assert tuple(got.shape) == (0, 8, 128)
+
+
+def test_places_out_of_range_are_counted_and_left_out(backend):
+    k, v, table = paged([100, 100, 100, 100], 16, 2, 128, torch.bfloat16, 10)
+    cache = backend.kv_cache_view(k, v)
+    pos = positions_of([100, 100, 100, 100])
+    q = torch.randn(4, 8, 128, device="cuda")
+    bad = table.clone()
+    bad[1, 2] = -7          # 16 tokens of row 1 have no page
+    bad[2, :] = 1 << 30     # none of row 2's 100 has
+    seqs = torch.tensor([0, 1, 2, 9], dtype=torch.int32, device="cuda")  # row 3 has no sequence
+    got = backend.paged_attention(q, cache, pos, bad, seqs=seqs)
+    backend.synchronize()
+    assert backend.take_device_errors() == (16 + 100 + 1, 0)
+    want, bound = attention_reference(q, k, v, pos, table, 128 ** -0.5)
+    assert ((got[0].double() - want[0]).abs() <= bound[0]).all()
+    assert (got[2] == 0).all() and (got[3] == 0).all()
+    keep = [t for t in range(100) if not 32 <= t < 48]
+    t = torch.tensor(keep, device="cuda")
+    kk = k[table[1].long()[t // 16], :, t % 16].double().transpose(0, 1).repeat_interleave(4, 0)
+    vv = v[table[1].long()[t // 16], :, t % 16].double().transpose(0, 1).repeat_interleave(4, 0)
+    w = torch.softmax(torch.einsum("hd,htd->ht", q[1].double(), kk) * 128 ** -0.5, -1)
+    assert (got[1].double() - torch.einsum("ht,htd->hd", w, vv)).abs().max() < 1e-5
+    # a position past the block table: the tokens that it holds are used, and it is counted
+    far = pos.clone()
+    far[0] = 5000
+    got = backend.paged_attention(q[:1], cache, far[:1], table)
+    backend.synchronize()
+    assert backend.take_device_errors() == (1, 0)
+    full = torch.tensor([table.shape[1] * 16 - 1], dtype=torch.int32, device="cuda")
+    same = backend.paged_attention(q[:1], cache, full, table)
+    backend.synchronize()
+    assert torch.equal(got, same)
+
+
+def test_refusals(backend):
+    k, v, table = paged([100, 100], 16, 2, 128, torch.bfloat16, 11)
+    cache = backend.kv_cache_view(k, v)
+    pos = positions_of([100, 100])
+    q = torch.randn(2, 8, 128, device="cuda")
+    f = backend.paged_attention
+    with pytest.raises(KernelError):
+        f(q.double(), cache, pos, table)
+    with pytest.raises(KernelError):
+        f(q.cpu(), cache, pos, table)
+    with pytest.raises(KernelError):
+        f(q[:, :, :64].contiguous(), cache, pos, table)
+    with pytest.raises(KernelError, match="multiple of n_kv_heads"):
+        f(q[:, :7].contiguous(), cache, pos, table)
+    with pytest.raises(KernelError):
+        f(q, cache, pos.long(), table)
+    with pytest.raises(KernelError, match="positions"):
+        f(q, cache, pos[:1], table)
+    with pytest.raises(KernelError, match="exceed"):
+        f(q, cache, pos, table[:1])
+    with pytest.raises(KernelError, match="scale"):
+        f(q, cache, pos, table, scale=0.0)
+    with pytest.raises(KernelError, match="scale"):
+        f(q, cache, pos, table, scale=float("nan"))
+    with pytest.raises(KernelError, match="overlaps"):
+        f(q, cache, pos, table, out=q)
+    with pytest.raises(KernelError, match="16-byte"):
+        f(torch.randn(2 * 8 * 128 + 1, device="cuda")[1:].view(2, 8, 128), cache, pos, table)
+    with pytest.raises(UnsupportedError):
+        backend.kv_cache_view(k.float(), v.float())
+    with pytest.raises(UnsupportedError):
+        backend.kv_cache(4, 16, 2, 80)
+    with pytest.raises(KernelError):
+        backend.kv_cache_view(k, v[:, :, :8])

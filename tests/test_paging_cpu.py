@@ -1,0 +1,79 @@
+"""CPU: the index arithmetic of the paged cache and of the attention's work split
+(ocelotl_b200/csrc/paging.cuh, the same source the kernels are built from)."""
+import ctypes as C
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+HERE = Path(__file__).resolve().parent
+TILE = 64
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    so = tmp_path_factory.mktemp("paging") / "paging.so"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", str(HERE / "paging_host.cpp"), "-o", str(so)], check=True)
+    lib = C.CDLL(str(so))
+    lib.walk.restype = C.c_longlong
+    lib.walk.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong]
+    lib.place.argtypes = [C.c_void_p] + [C.c_longlong] * 4 + [C.c_int, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p]
+    return lib
+
+
+def walk(lib, positions, cap, items, ctas, seqs=None, n_seqs=None):
+    pos = np.asarray(positions, np.int32)
+    sq = None if seqs is None else np.asarray(seqs, np.int32)
+    room = int(sum(-(-(min(p + 1, cap)) // TILE) for p in pos.astype(int) if p >= 0)) * items + 1
+    out = np.full((room, 4), -1, np.int32)
+    n = lib.walk(pos.ctypes.data, None if sq is None else sq.ctypes.data, len(pos) if n_seqs is None else n_seqs, len(pos),
+                 cap, items, ctas, out.ctypes.data, room)
+    assert n >= 0, n
+    return out[:n]
+
+
+@pytest.mark.parametrize("positions,items,ctas", [
+    ([0], 1, 296), ([554], 8, 296), ([130999], 8, 296), ([130999], 1, 444), ([-1, -1], 8, 296), ([63, 64, 65, -1, 127], 3, 7),
+    ([5] * 230, 2, 444), (list(range(0, 4000, 37)), 16, 296), ([-1, 700, -1, -1, 3, -1], 1, 5), ([2147483647], 2, 148),
+    ([100000, 0, 0, 0, 0], 8, 148),
+])
+def test_every_tile_once_and_shares_agree(lib, positions, items, ctas):
+    cap = 140000
+    got = walk(lib, positions, cap, items, ctas)
+    want = [(r, i, t) for r, p in enumerate(positions) if p >= 0
+            for i in range(items) for t in range(-(-min(p + 1, cap) // TILE))]
+    assert [tuple(x[:3]) for x in got.tolist()] == want
+    if len(want):
+        per = np.bincount(got[:, 3])
+        assert per.min() >= 1 and per.max() - per.min() <= 1  # equal runs
+
+
+def test_random_batches(lib):
+    rng = np.random.default_rng(3)
+    for _ in range(200):
+        rows = int(rng.integers(1, 40))
+        pos = np.where(rng.random(rows) < 0.2, -1, rng.integers(0, int(rng.choice([2, 70, 900, 9000])), rows))
+        walk(lib, pos, int(rng.integers(1, 9000)), int(rng.integers(1, 17)), int(rng.integers(1, 300)))
+
+
+def test_rows_of_unknown_sequences_have_no_tiles(lib):
+    got = walk(lib, [100, 100, 100, 100], 1000, 2, 10, seqs=[0, -1, 2, 1], n_seqs=2)
+    assert sorted(set(got[:, 0].tolist())) == [0, 3]
+
+
+def test_place_of(lib):
+    table = np.array([[3, 7, -1, 99], [5, 9, 0, 1]], np.int32)
+    page, slot = C.c_int(-5), C.c_int(-5)
+
+    def place(seq, tok, n_pages=10, max_pages=4, size=24):
+        ok = lib.place(table.ctypes.data, 2, max_pages, 4, n_pages, size, seq, tok, C.byref(page), C.byref(slot))
+        return (page.value, slot.value) if ok else None
+
+    assert place(0, 0) == (3, 0) and place(0, 23) == (3, 23) and place(0, 24) == (7, 0) and place(1, 95) == (1, 23)
+    assert place(0, 48) is None      # page -1
+    assert place(0, 72) is None      # page past the cache
+    assert place(1, 96) is None      # past the table
+    assert place(1, 48, max_pages=2) is None
+    assert place(1, 2147483647) is None
+    assert place(1, 2, size=1) == (0, 0)
