@@ -74,6 +74,7 @@ struct AttnArgs {
     int rows, n_heads, n_kv, group, head_groups;
     KvCache kv;
     KvRows at;
+    Divisor page_size;
     int cap;      // tokens a row of the block table can hold
     float scale;  // in units of log2
     float* out;
@@ -92,24 +93,24 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 // c = a . b, and c += a . b
 #define OCL_MMA(NAME, TYPE)                                                                                            \
     __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,             \
                                          uint32_t b0, uint32_t b1, TYPE) {                                              \
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." NAME "." NAME                                             \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." NAME "." NAME                                             \
                      ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"                                   \
                      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                   \
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));                                 \
     }                                                                                                                   \
     __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, \
                                         uint32_t b1, TYPE) {                                                            \
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." NAME "." NAME                                             \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." NAME "." NAME                                             \
                      ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                                       \
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                   \
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));                                           \
@@ -150,6 +151,12 @@ template <> constexpr int kPieces<__half> = 2;
 template <class T> constexpr float kShift = 0.f;  // p is scaled by 2^kShift
 template <> constexpr float kShift<__half> = 14.f;
 
+__device__ __forceinline__ float ex2(float x) {  // 2 units, 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Two floats as N packed pairs of 16-bit pieces, leading piece first.
 template <int N, class T>
 __device__ __forceinline__ void cut(uint32_t (&w)[N], float a, float b) {
@@ -171,14 +178,16 @@ __device__ __forceinline__ int chunk_at(int c, int r) {
     return c / CP * part_bytes(D) + r * CP * 16 + ((c % CP) ^ x) * 16;
 }
 
-// TILED: 16 tokens lie in one page, which the tensor maps describe as (part element,
+// PACK (bf16, at most 4 heads): rows 0-3 leading pieces, 4-7 third, 8-11 second, so that
+// one MMA does what takes two with 8 heads; lanes 16-31 then hold the third pieces' part
+// of o.  TILED: 16 tokens lie in one page, which the tensor maps describe as (part element,
 // slot, part, k/v head, page).
-template <int D, class T, bool TILED>
+template <int D, class T, bool TILED, bool PACK>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     attention_kernel(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int S = stages(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
     constexpr int kHalf = half_bytes(D), kStage = 2 * kHalf, kPart = part_bytes(D), CP2 = part_elems(D) / 16;
-    constexpr int MC = merge_cols(D);
+    constexpr int MC = merge_cols(D), kRows = PACK ? 4 : kHeads;
     extern __shared__ __align__(1024) unsigned char smem[];
     float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D));
     uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem + ring_bytes(D) + merge_bytes(D));
@@ -258,21 +267,31 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     // Page of this lane's token (TILED: of the warp's 16 tokens; else lanes 0-15 have one
     // each) of the tile at `ld`, looked up one tile ahead of its loads.  -1: past the
     // row's tokens, or no such page.
+    const int32_t* pages = p.at.table + sequence_of(p.at, ld.row) * p.at.table_stride;
     int page = -1, in_page = 0;
+    bool looked = false;
     uint32_t filled = 0;  // TILED: byte s is the number of tokens on their way to stage s
     bool failed = false;  // a bounded wait gave up: nothing more is loaded or computed
-    auto look_up = [&]() {
+    auto look_up = [&]() {  // only starts the table's load: what it names is checked when it is used
         page = -1;
+        looked = false;
         if (to_load <= 0) return;
         const int tok = ld.tile * kTileTok + warp * kWarpTok + (TILED ? 0 : lane & 15);
-        if (tok < ld.tokens && !place_of(p.at, p.kv.n_pages, (int)p.kv.page_size, sequence_of(p.at, ld.row), tok, page, in_page)) {
-            page = -1;
-            if (ld.item == 0 && lane < (TILED ? 1 : 16)) atomicAdd(p.err, TILED ? (unsigned)min(kWarpTok, ld.tokens - tok) : 1u);
+        if (tok < ld.tokens) {
+            looked = true;
+            const uint32_t nth = quotient((uint32_t)tok, p.page_size);
+            in_page = (int)((uint32_t)tok - nth * p.page_size.d);
+            page = pages[nth];
         }
     };
     auto load = [&](int stage) {
         if (to_load > 0) {
-            const int head = ld.item / p.head_groups;
+            const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
+            if (looked && (page < 0 || page >= p.kv.n_pages)) {
+                page = -1;
+                if (ld.item == 0 && lane < (TILED ? 1 : 16))
+                    atomicAdd(p.err, TILED ? (unsigned)min(kWarpTok, ld.tokens - (ld.tile * kTileTok + warp * kWarpTok)) : 1u);
+            }
             if constexpr (TILED) {
                 if (page >= 0) {
                     filled |= (uint32_t)min(kWarpTok, ld.tokens - (ld.tile * kTileTok + warp * kWarpTok)) << (8 * stage);
@@ -304,7 +323,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                 }
             }
             --to_load;
-            if (++ld.tile == ld.tiles && to_load > 0) next_item(p.at, p.rows, p.cap, items, ld);
+            if (++ld.tile == ld.tiles && to_load > 0) {
+                next_item(p.at, p.rows, p.cap, items, ld);
+                pages = p.at.table + sequence_of(p.at, ld.row) * p.at.table_stride;
+            }
             look_up();
         }
         if constexpr (!TILED) cp_commit();
@@ -321,7 +343,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
 #pragma unroll
     for (int s = 0; s < (TILED ? S : S - 1); ++s) load(s);
 
-    uint32_t qa[q_in_smem(D) ? 1 : KS][N * 2];  // A fragments: pieces of (k = 2c, 2c+1) and (k = 2c+8, 2c+9)
+    // A fragments of q: [k][0..3] = rows g, g + 8 at (k = 2c, 2c+1), then at (2c+8, 2c+9).  The
+    // third pieces of two k steps share one fragment, in rows 0-7 and 8-15: each step's MMA
+    // reads its own half of the result.
+    constexpr bool THIRD = N == 3 && !PACK;
+    constexpr int QW = THIRD ? 6 : 4;  // words per k
+    uint32_t qa[q_in_smem(D) ? 1 : KS / 2][2 * QW];
     int stage = 0;
     uint32_t phase = 0;  // bit s: parity of stage s's next completed copy
     long long done = 0;  // tiles of the run behind cc
@@ -332,14 +359,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
         const int h0 = kvh * p.group + hg * kHeads, nh = min(kHeads, p.group - hg * kHeads);
         float scale = p.scale;
         {
-            const float* qr = p.q + (int64_t)cc.row * p.q_stride + (int64_t)(h0 + (g < nh ? g : 0)) * D + c4 * 2;
+            const int hq = PACK ? g & 3 : g;
+            const float* qr = p.q + (int64_t)cc.row * p.q_stride + (int64_t)(h0 + (hq < nh ? hq : 0)) * D + c4 * 2;
             float2 x[KS][2];
             float top = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    x[k][j] = g < nh ? *reinterpret_cast<const float2*>(qr + k * 16 + j * 8) : make_float2(0.f, 0.f);
+                    x[k][j] = hq < nh ? *reinterpret_cast<const float2*>(qr + k * 16 + j * 8) : make_float2(0.f, 0.f);
                     top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
                 }
             if constexpr (N == 2) {
@@ -355,20 +383,24 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     for (int j = 0; j < 2; ++j) x[k][j].x *= up, x[k][j].y *= up;
             }
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t w[2][N];
-                cut<N, T>(w[0], x[k][0].x, x[k][0].y);
-                cut<N, T>(w[1], x[k][1].x, x[k][1].y);
-                if constexpr (q_in_smem(D)) {
-                    if (k % kWarps == warp) {
+            for (int k = 0; k < KS; k += 2) {
+                uint32_t f[2 * QW];
 #pragma unroll
-                        for (int i = 0; i < N; ++i)
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t w[2][N];
+                    cut<N, T>(w[0], x[k + i][0].x, x[k + i][0].y);
+                    cut<N, T>(w[1], x[k + i][1].x, x[k + i][1].y);
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) q_frag[((k * N + i) * 2 + j) * 32 + lane] = w[j][i];
+                    for (int j = 0; j < 2; ++j) {
+                        f[4 * i + 2 * j] = PACK && g >= 4 ? w[j][N - 1] : w[j][0];
+                        f[4 * i + 2 * j + 1] = PACK && g >= 4 ? 0u : w[j][1];
+                        if constexpr (THIRD) f[8 + 2 * j + i] = w[j][2];
                     }
-                } else {
+                }
 #pragma unroll
-                    for (int i = 0; i < N; ++i) qa[k][2 * i] = w[0][i], qa[k][2 * i + 1] = w[1][i];
+                for (int i = 0; i < 2 * QW; ++i) {
+                    if constexpr (!q_in_smem(D)) qa[k / 2][i] = f[i];
+                    else if (k / 2 % kWarps == warp) q_frag[(k / 2 * 2 * QW + i) * 32 + lane] = f[i];
                 }
             }
         }
@@ -416,25 +448,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
             }
 
             // ---- s = q . k for 16 tokens: two 8-token MMA columns
-            float acc[2][2][4], low[2][4] = {};
+            float acc[2][2][4], low[2][2][4];
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t b[4], a[N * 2];
-                ldmatrix4(b, base + k / CP2 * kPart + k_at[k % CP2]);
+            for (int k = 0; k < KS; k += 2) {
+                uint32_t a[2 * QW];
                 if constexpr (q_in_smem(D)) {
 #pragma unroll
-                    for (int i = 0; i < N * 2; ++i) a[i] = q_frag[(k * N * 2 + i) * 32 + lane];
+                    for (int i = 0; i < 2 * QW; ++i) a[i] = q_frag[(k * QW + i) * 32 + lane];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < N * 2; ++i) a[i] = qa[k][i];
+                    for (int i = 0; i < 2 * QW; ++i) a[i] = qa[k / 2][i];
                 }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (k < 2) mma0(acc[j][k], a[0], a[2], a[1], a[3], b[2 * j], b[2 * j + 1], T());
-                    else mma(acc[j][k & 1], a[0], a[2], a[1], a[3], b[2 * j], b[2 * j + 1], T());
-                    if constexpr (N == 3) {
-                        if (k == 0) mma0(low[j], a[4], 0u, a[5], 0u, b[2 * j], b[2 * j + 1], T());
-                        else mma(low[j], a[4], 0u, a[5], 0u, b[2 * j], b[2 * j + 1], T());
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t b[4];
+                    ldmatrix4(b, base + (k + i) / CP2 * kPart + k_at[(k + i) % CP2]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if (k == 0) mma0(acc[j][i], a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3], b[2 * j], b[2 * j + 1], T());
+                        else mma(acc[j][i], a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3], b[2 * j], b[2 * j + 1], T());
+                        if constexpr (THIRD) {
+                            if (k == 0) mma0(low[j][i], a[8], a[9], a[10], a[11], b[2 * j], b[2 * j + 1], T());
+                            else mma(low[j][i], a[8], a[9], a[10], a[11], b[2 * j], b[2 * j + 1], T());
+                        }
                     }
                 }
             }
@@ -442,25 +478,39 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = i >> 1, e = i & 1;
-                s[i] = (acc[j][0][e] + acc[j][1][e]) + ((acc[j][0][e + 2] + acc[j][1][e + 2]) + low[j][e]);
-                if (!((have >> (8 * j + 2 * c4 + e)) & 1)) s[i] = -INFINITY;
+                s[i] = acc[j][0][e + 2] + acc[j][1][e + 2];
+                if constexpr (THIRD) s[i] += low[j][0][e] + low[j][1][e + 2];
+                s[i] += acc[j][0][e] + acc[j][1][e];
+                if constexpr (PACK) s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
+            }
+            if (have != 0xffffu) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!((have >> (8 * (i >> 1) + 2 * c4 + (i & 1))) & 1)) s[i] = -INFINITY;
             }
             float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float m_new = fmaxf(m, top * scale - kShift<T>);
             const float ref = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = exp2f(m - ref);
+            const float alpha = ex2(m - ref);
             m = m_new;
             float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = exp2f(fmaf(s[i], scale, -ref));
+            for (int i = 0; i < 4; ++i) w[i] = ex2(fmaf(s[i], scale, -ref));
             l = l * alpha + ((w[0] + w[1]) + (w[2] + w[3]));
 
             // ---- o = o * alpha + p . v
             uint32_t pa[2][N];
             cut<N, T>(pa[0], w[0], w[1]);
             cut<N, T>(pa[1], w[2], w[3]);
+            if constexpr (PACK) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    pa[j][0] = g >= 4 ? pa[j][2] : pa[j][0];
+                    pa[j][1] = g >= 4 ? 0u : pa[j][1];
+                }
+            }
 #pragma unroll
             for (int c = 0; c < NT; c += 2) {
                 uint32_t b[4];
@@ -468,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float d[4];
-                    if constexpr (N == 3) {
+                    if constexpr (THIRD) {
                         mma0(d, pa[0][2], 0u, pa[1][2], 0u, b[2 * j], b[2 * j + 1], T());
                         mma(d, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b[2 * j], b[2 * j + 1], T());
                     } else {
@@ -501,9 +551,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     make_float2(o[col0 / 8 + t][0], o[col0 / 8 + t][1]);
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < (kHeads * MC / 4 + kThreads - 1) / kThreads; ++i) {
+            for (int i = 0; i < (kRows * MC / 4 + kThreads - 1) / kThreads; ++i) {
                 const int idx = i * kThreads + tid, h = idx / (MC / 4), col = idx % (MC / 4) * 4;
-                if (idx >= kHeads * MC / 4) break;
+                if (idx >= kRows * MC / 4) break;
                 float top = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][h]);
@@ -512,8 +562,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    const float f = exp2f(sh.m[w][h] - ref);
-                    const float4 x = *reinterpret_cast<const float4*>(merge_o + (w * kHeads + h) * MC + (col ^ ((h & 3) << 3)));
+                    const float f = ex2(sh.m[w][h] - ref);
+                    float4 x = *reinterpret_cast<const float4*>(merge_o + (w * kHeads + h) * MC + (col ^ ((h & 3) << 3)));
+                    if constexpr (PACK) {  // h + 4 has the same swizzle
+                        const float4 z = *reinterpret_cast<const float4*>(merge_o + (w * kHeads + h + 4) * MC + (col ^ ((h & 3) << 3)));
+                        x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
+                    }
                     sum += sh.l[w][h] * f;
                     a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
                 }
@@ -554,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     const float ref = top == -INFINITY ? 0.f : top;
                     float sum = 0.f;
                     for (int i = lane; i < parts; i += 32)
-                        sum += __ldcg(part_of(i) + kHeads * D + kHeads + h) * exp2f(__ldcg(part_of(i) + kHeads * D + h) - ref);
+                        sum += __ldcg(part_of(i) + kHeads * D + kHeads + h) * ex2(__ldcg(part_of(i) + kHeads * D + h) - ref);
 #pragma unroll
                     for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
                     if (lane == 0) sh.m[0][h] = ref, sh.l[0][h] = sum == 0.f ? 0.f : 1.0f / sum;
@@ -566,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
                     for (int i = 0; i < parts; ++i) {
-                        const float f = exp2f(__ldcg(part_of(i) + kHeads * D + h) - ref);
+                        const float f = ex2(__ldcg(part_of(i) + kHeads * D + h) - ref);
                         const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(i) + h * D + col));
                         a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
                     }
@@ -617,21 +671,28 @@ bool encode(CUtensorMap* map, void* base, const KvCache& kv) {
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, class T, bool TILED>
+template <int D, class T, bool TILED, bool PACK>
 cudaError_t launch_typed(const AttnArgs& a, const CUtensorMap (&maps)[2], int sms, bool pdl, cudaStream_t s) {
     static bool configured[kMaxDevices] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices || !configured[dev]) {
-        e = cudaFuncSetAttribute(attention_kernel<D, T, TILED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
+        e = cudaFuncSetAttribute(attention_kernel<D, T, TILED, PACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) configured[dev] = true;
     }
     const int64_t tiles = (int64_t)a.rows * a.n_kv * a.head_groups * ((a.cap + kTileTok - 1) / kTileTok);
     const int64_t ctas = (int64_t)sms * ctas_per_sm(D);
-    return launch_kernel(attention_kernel<D, T, TILED>, dim3((unsigned)(tiles < ctas ? tiles : ctas)), kThreads,
+    return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)(tiles < ctas ? tiles : ctas)), kThreads,
                          smem_bytes(D), pdl, s, a, maps[0], maps[1]);
+}
+
+template <int D, bool TILED>
+cudaError_t launch_tiled(const AttnArgs& a, const CUtensorMap (&maps)[2], int sms, bool pdl, cudaStream_t s) {
+    if (a.kv.type != kKvBf16) return launch_typed<D, __half, TILED, false>(a, maps, sms, pdl, s);
+    return a.group <= 4 ? launch_typed<D, __nv_bfloat16, TILED, true>(a, maps, sms, pdl, s)
+                        : launch_typed<D, __nv_bfloat16, TILED, false>(a, maps, sms, pdl, s);
 }
 
 template <int D>
@@ -640,10 +701,8 @@ cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
     // strides of 2^40 bytes and more do not fit a tensor map
     const bool fits = a.kv.token_stride < (1ll << 39) && a.kv.head_stride < (1ll << 39) && a.kv.page_stride < (1ll << 39);
     if (a.kv.page_size % kWarpTok == 0 && fits && encode_fn() && encode<D>(&maps[0], a.kv.k, a.kv) && encode<D>(&maps[1], a.kv.v, a.kv))
-        return a.kv.type == kKvBf16 ? launch_typed<D, __nv_bfloat16, true>(a, maps, sms, pdl, s)
-                                    : launch_typed<D, __half, true>(a, maps, sms, pdl, s);
-    return a.kv.type == kKvBf16 ? launch_typed<D, __nv_bfloat16, false>(a, maps, sms, pdl, s)
-                                : launch_typed<D, __half, false>(a, maps, sms, pdl, s);
+        return launch_tiled<D, true>(a, maps, sms, pdl, s);
+    return launch_tiled<D, false>(a, maps, sms, pdl, s);
 }
 
 }  // namespace
@@ -671,6 +730,7 @@ cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t row
     a.head_groups = (a.group + kHeads - 1) / kHeads;
     a.kv = kv;
     a.at = at;
+    a.page_size = divisor_of((uint32_t)kv.page_size);
     const int64_t cap = at.max_pages * kv.page_size;
     a.cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
     a.scale = scale * 1.4426950408889634f;

@@ -24,13 +24,28 @@ OCL_HD int64_t sequence_of(const KvRows& at, int64_t row) {
     return seq >= 0 && seq < at.n_seqs ? seq : -1;
 }
 
-// Page and slot of token `tok` (>= 0) of a sequence that the table has.  False:
-// the table has no such token, or names a page that the cache has not.
-OCL_HD bool place_of(const KvRows& at, int64_t n_pages, int page_size, int64_t seq, int tok, int& page, int& in_page) {
-    const unsigned nth = (unsigned)tok / (unsigned)page_size;
-    if ((int64_t)nth >= at.max_pages) return false;
-    in_page = (int)((unsigned)tok - nth * (unsigned)page_size);
-    page = at.table[seq * at.table_stride + nth];
+// n / d for 0 <= n < 2^31 as a product and a shift (Granlund and Montgomery, Division
+// by invariant integers using multiplication): with l = ceil(log2 d) and
+// m = floor(2^(31 + l) / d) + 1, m * d exceeds 2^(31 + l) by at most 2^l.
+struct Divisor {
+    uint32_t d, m;
+    int shift;
+};
+inline Divisor divisor_of(uint32_t d) {
+    int l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, (uint32_t)(((unsigned long long)1 << (31 + l)) / d + 1), 31 + l};
+}
+OCL_HD uint32_t quotient(uint32_t n, const Divisor& by) { return (uint32_t)(((unsigned long long)n * by.m) >> by.shift); }
+
+// Page and slot of token `tok` (>= 0) of the sequence with page list `pages`.  False:
+// the list has no such token, or names a page that the cache has not.
+OCL_HD bool place_of(const int32_t* pages, int64_t max_pages, int64_t n_pages, const Divisor& page_size, int tok, int& page,
+                     int& in_page) {
+    const uint32_t nth = quotient((uint32_t)tok, page_size);
+    if ((int64_t)nth >= max_pages) return false;
+    in_page = (int)((uint32_t)tok - nth * page_size.d);
+    page = pages[nth];
     return page >= 0 && (int64_t)page < n_pages;
 }
 

@@ -30,6 +30,7 @@ struct RopeArgs {
     int n_heads, n_kv, groups;  // groups: CTAs per row
     KvCache kv;
     KvRows at;
+    Divisor page_size;
     const float *q_norm, *k_norm;
     float eps;
     RopeTable rope;
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p
     if (pos >= 0) {
         const int64_t seq = sequence_of(p.at, row);
         int page = -1, in_page = 0;
-        const bool ok = seq >= 0 && place_of(p.at, p.kv.n_pages, (int)p.kv.page_size, seq, pos, page, in_page);
+        const bool ok = seq >= 0 && place_of(p.at.table + seq * p.at.table_stride, p.at.max_pages, p.kv.n_pages, p.page_size, pos, page, in_page);
         slot = page * p.kv.page_stride + in_page * p.kv.token_stride;
         if (!ok) {
             slot = -1;
@@ -172,7 +173,7 @@ cudaError_t launch_qk_norm_rope(const float* qkv, int64_t qkv_stride, int64_t ro
                                 const KvRows& at, const float* q_norm, const float* k_norm, float eps,
                                 const RopeTable& rope, float* q_out, unsigned int* err, int sms, bool pdl,
                                 cudaStream_t s) {
-    RopeArgs a{qkv, qkv_stride, (int)n_heads, (int)kv.n_kv, 1, kv, at, q_norm, k_norm, eps, rope, q_out, err};
+    RopeArgs a{qkv, qkv_stride, (int)n_heads, (int)kv.n_kv, 1, kv, at, divisor_of((uint32_t)kv.page_size), q_norm, k_norm, eps, rope, q_out, err};
     const int64_t most = (n_heads + 2 * kv.n_kv + kWarps - 1) / kWarps;  // CTAs a row can use
     const int64_t want = (sms + rows - 1) / rows;
     a.groups = (int)(want < most ? want : most);

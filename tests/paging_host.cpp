@@ -54,8 +54,15 @@ extern "C" long long walk(const int32_t* positions, const int32_t* seqs, long lo
     return seen == total ? seen : -7;
 }
 
-extern "C" int place(const int32_t* table, long long n_seqs, long long max_pages, long long stride, long long n_pages,
-                     int page_size, long long seq, int tok, int* page, int* in_page) {
-    const KvRows at{nullptr, nullptr, table, n_seqs, max_pages, stride};
-    return place_of(at, n_pages, page_size, seq, tok, *page, *in_page) ? 1 : 0;
+extern "C" int place(const int32_t* table, long long max_pages, long long stride, long long n_pages, unsigned page_size,
+                     long long seq, int tok, int* page, int* in_page) {
+    return place_of(table + seq * stride, max_pages, n_pages, divisor_of(page_size), tok, *page, *in_page) ? 1 : 0;
+}
+
+// First n of [from, to) in steps whose quotient by d is wrong, or -1.
+extern "C" long long wrong_quotient(unsigned d, long long from, long long to, long long step) {
+    const Divisor by = divisor_of(d);
+    for (long long n = from; n < to; n += step)
+        if (quotient((uint32_t)n, by) != (uint32_t)n / d) return n;
+    return -1;
 }

@@ -18,7 +18,9 @@ def lib(tmp_path_factory):
     lib = C.CDLL(str(so))
     lib.walk.restype = C.c_longlong
     lib.walk.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong]
-    lib.place.argtypes = [C.c_void_p] + [C.c_longlong] * 4 + [C.c_int, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p]
+    lib.place.argtypes = [C.c_void_p] + [C.c_longlong] * 3 + [C.c_uint, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p]
+    lib.wrong_quotient.restype = C.c_longlong
+    lib.wrong_quotient.argtypes = [C.c_uint] + [C.c_longlong] * 3
     return lib
 
 
@@ -67,7 +69,7 @@ def test_place_of(lib):
     page, slot = C.c_int(-5), C.c_int(-5)
 
     def place(seq, tok, n_pages=10, max_pages=4, size=24):
-        ok = lib.place(table.ctypes.data, 2, max_pages, 4, n_pages, size, seq, tok, C.byref(page), C.byref(slot))
+        ok = lib.place(table.ctypes.data, max_pages, 4, n_pages, size, seq, tok, C.byref(page), C.byref(slot))
         return (page.value, slot.value) if ok else None
 
     assert place(0, 0) == (3, 0) and place(0, 23) == (3, 23) and place(0, 24) == (7, 0) and place(1, 95) == (1, 23)
@@ -77,3 +79,15 @@ def test_place_of(lib):
     assert place(1, 48, max_pages=2) is None
     assert place(1, 2147483647) is None
     assert place(1, 2, size=1) == (0, 0)
+
+
+def test_quotients(lib):
+    top = 2**31
+    divisors = list(range(1, 200)) + [255, 256, 257, 1000, 4095, 4096, 4097, 65535, 65536, 10**6, 2**30 - 1, 2**30, 2**30 + 1,
+                                      2**31 - 1]
+    for d in divisors:
+        assert lib.wrong_quotient(d, 0, 70000, 1) == -1
+        assert lib.wrong_quotient(d, top - 70000, top, 1) == -1
+        assert lib.wrong_quotient(d, 0, top, 10007) == -1
+        first = (top // d) * d  # around the last multiple
+        assert lib.wrong_quotient(d, max(0, first - 5), min(top, first + 5), 1) == -1
