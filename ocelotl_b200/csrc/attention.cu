@@ -30,6 +30,7 @@
 // several CTAs is joined by the last of them to arrive, in CTA order: the result
 // does not depend on which one it is.  Nothing waits on another CTA.
 #include <cuda.h>
+#include <cstdlib>
 
 #include "device.cuh"
 #include "internal.cuh"
@@ -38,18 +39,25 @@ namespace ocl {
 
 namespace {
 
-constexpr int kWarps = kTileWarps, kThreads = 32 * kWarps;
-constexpr int kHeads = 8;  // query heads of one k/v head worked on together
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kHeads = 8;   // query heads of one k/v head worked on together
+constexpr int kBoxTok = 16; // tokens of one tensor-map copy, and of one p.v MMA
 
-constexpr int stages(int d) { return d <= 96 ? 4 : 3; }
-constexpr int ctas_per_sm(int d) { return d == 64 ? 3 : d == 256 ? 1 : 2; }
-constexpr int max_ctas_per_sm = 3;
+// Tokens a warp takes at a time, and the ring's stages of as many.  32 tokens halve the
+// work a token costs besides its MMAs (maximum, rescaling, waits, look-ups) and give a
+// warp twice the independent MMAs; at head_dim 256 three stages of 32 do not fit.
+constexpr int warp_tok(int d) { return d == 256 ? 16 : 32; }
+constexpr int tile_tok(int d) { return kWarps * warp_tok(d); }
+constexpr int stages(int d) { return d == 96 ? 4 : 3; }
+constexpr int ctas_per_sm(int d) { return d == 64 ? 2 : 1; }
+constexpr int max_ctas_per_sm = 2;
 // 16 tokens of k or v are kept as parts of 64 elements (32 for head_dim 96): a part is
 // 16 rows of 128 (64) bytes, its 16-byte chunks exclusive-or'ed with the row as the
 // copy engine's 128-byte (64-byte) swizzle does.
 constexpr int part_elems(int d) { return d % 64 == 0 ? 64 : 32; }
-constexpr int part_bytes(int d) { return kWarpTok * part_elems(d) * 2; }
-constexpr int half_bytes(int d) { return kWarpTok * d * 2; }  // k (or v) of a stage
+constexpr int part_bytes(int d) { return kBoxTok * part_elems(d) * 2; }
+constexpr int box_bytes(int d) { return kBoxTok * d * 2; }
+constexpr int half_bytes(int d) { return warp_tok(d) * d * 2; }  // k (or v) of a stage
 constexpr int merge_cols(int d) { return d < 128 ? d : 128; }
 constexpr bool q_in_smem(int d) { return d > 128; }
 constexpr int q_bytes(int d) { return q_in_smem(d) ? d / 16 * 32 * 24 : 0; }
@@ -57,16 +65,18 @@ constexpr int slot_floats(int d) { return kHeads * d + 2 * kHeads; }
 
 struct Shared {  // behind the ring, the merge buffer and the q fragments
     uint64_t full[kWarps][4];
-    long long scan[kWarps], first_at;
-    int first_row, last_in;
-    uint32_t valid[kWarps][4];
+    uint32_t scan[kWarps], longest[kWarps];
+    Cursor first;
+    uint32_t edge[2];
+    int last_in;
+    uint32_t valid[kWarps][4];  // a bit per token of a stage
     float m[kWarps][kHeads], l[kWarps][kHeads];
 };
 constexpr int ring_bytes(int d) { return kWarps * stages(d) * 2 * half_bytes(d); }
 constexpr int merge_bytes(int d) { return kWarps * kHeads * merge_cols(d) * 4; }
 constexpr int smem_bytes(int d) { return ring_bytes(d) + merge_bytes(d) + q_bytes(d) + (int)sizeof(Shared); }
-static_assert(smem_bytes(256) <= 227 * 1024 && 2 * (smem_bytes(128) + 1024) <= 228 * 1024 &&
-              2 * (smem_bytes(96) + 1024) <= 228 * 1024 && 3 * (smem_bytes(64) + 1024) <= 228 * 1024, "CTAs per SM");
+static_assert(smem_bytes(256) <= 227 * 1024 && smem_bytes(128) <= 227 * 1024 && smem_bytes(96) <= 227 * 1024 &&
+              2 * (smem_bytes(64) + 1024) <= 228 * 1024, "CTAs per SM");
 
 struct AttnArgs {
     const float* q;
@@ -77,6 +87,7 @@ struct AttnArgs {
     Divisor page_size;
     int cap;      // tokens a row of the block table can hold
     float scale;  // in units of log2
+    int min_share, snap;  // tiles: the least that a run gets, and how far a cut moves to an item's edge
     float* out;
     float* part;
     unsigned int* counters;
@@ -146,6 +157,19 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+template <int V>
+__device__ __forceinline__ void load_cg(float (&x)[V], const float* p) {
+    if constexpr (V == 4) {
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(p));
+        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+    } else if constexpr (V == 2) {
+        const float2 t = __ldcg(reinterpret_cast<const float2*>(p));
+        x[0] = t.x; x[1] = t.y;
+    } else {
+        x[0] = __ldcg(p);
+    }
+}
+
 template <class T> constexpr int kPieces = 3;
 template <> constexpr int kPieces<__half> = 2;
 template <class T> constexpr float kShift = 0.f;  // p is scaled by 2^kShift
@@ -186,7 +210,10 @@ template <int D, class T, bool TILED, bool PACK>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     attention_kernel(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int S = stages(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
-    constexpr int kHalf = half_bytes(D), kStage = 2 * kHalf, kPart = part_bytes(D), CP2 = part_elems(D) / 16;
+    constexpr int WT = warp_tok(D), TT = tile_tok(D), H = WT / kBoxTok;  // H boxes of 16 tokens a stage
+    constexpr uint32_t kAll = 0xffffffffu >> (32 - WT);
+    constexpr int kBox = box_bytes(D), kHalf = half_bytes(D), kStage = 2 * kHalf, kPart = part_bytes(D);
+    constexpr int CP2 = part_elems(D) / 16;
     constexpr int MC = merge_cols(D), kRows = PACK ? 4 : kHeads;
     extern __shared__ __align__(1024) unsigned char smem[];
     float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D));
@@ -195,6 +222,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int items = p.n_kv * p.head_groups;
+    if (TILED && tid == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+    }
     if (TILED && lane < S) {
         mbar_init(&sh.full[warp][lane]);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -202,81 +233,86 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     }
     grid_wait();
 
-    // ---- this CTA's run of tiles
+    // ---- this CTA's run: rows' units summed over the threads, then the two cuts located
     const int per = (p.rows + kThreads - 1) / kThreads;
     const int r0 = min(tid * per, p.rows), r1 = min(r0 + per, p.rows);
-    long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += tiles_of(row_tokens(p.at, p.cap, r));
-    long long upto = mine;
+    uint32_t mine = 0, longest = 0;
+    for (int r = r0; r < r1; ++r) {
+        const int tiles = tiles_of(row_tokens(p.at, p.cap, r), TT);
+        if (tiles) mine += item_units(tiles);
+        longest = max(longest, (uint32_t)tiles);
+    }
+    mine *= items;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
-    if (lane == 31) sh.scan[warp] = upto;
+    if (lane == 31) sh.scan[warp] = upto, sh.longest[warp] = longest;
     __syncthreads();
-    long long total = 0;
+    uint32_t total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w < warp) upto += sh.scan[w];
         total += sh.scan[w];
+        longest = max(longest, sh.longest[w]);
     }
-    total *= items;
-    const long long P = total < (long long)gridDim.x ? total : (long long)gridDim.x;
-    const long long cta = blockIdx.x;
-    const long long begin = cta < P ? run_begin(total, P, cta) : total, end = cta < P ? run_begin(total, P, cta + 1) : total;
-    {
-        const long long b = (upto - mine) * items, e = upto * items;
-        if (begin < end && begin >= b && begin < e) {
-            long long at = b;
-            int r = r0;
-            for (;; ++r) {
-                const long long n = (long long)tiles_of(row_tokens(p.at, p.cap, r)) * items;
-                if (begin < at + n) break;
-                at += n;
+    // Pieces of an item cost their join: about a tenth of a tile's time each, so the
+    // longest item is cut into no more than sqrt(10 * tiles) of them.
+    const Runs runs = runs_of(total, gridDim.x, max((uint32_t)p.min_share, (uint32_t)(sqrtf(0.1f * (float)longest) + 0.999f)), p.snap);
+    const uint32_t cta = blockIdx.x;
+    const bool active = total > 0 && cta < runs.P;
+    if (active) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t cut = run_cut(runs, cta + i);
+            uint32_t at = upto - mine;
+            if (cut < at || cut >= upto) continue;
+            for (int r = r0;; ++r) {
+                const int tokens = row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
+                const uint32_t all = tiles ? item_units(tiles) : 0, off = cut - at;
+                if (off < all * items) {
+                    const uint32_t item = off / all, u = off - item * all, moved = moved_cut(runs, u, tiles);
+                    sh.edge[i] = cut - u + moved;
+                    if (i == 0) sh.first = {r, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
+                    break;
+                }
+                at += all * items;
             }
-            sh.first_row = r;
-            sh.first_at = begin - at;
         }
     }
     __syncthreads();
-
-    // rows without tokens are zeros; rows whose place is out of range are counted
-    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const int tokens = row_tokens(p.at, p.cap, r), pos = p.at.positions[r];
-        if (tid == 0 && pos >= 0 && pos >= tokens) atomicAdd(p.err, 1u);
-        if (tokens == 0)
-            for (int i = tid; i < p.n_heads * D; i += kThreads) p.out[(int64_t)r * p.n_heads * D + i] = 0.f;
+    uint32_t end = 0;
+    Cursor ld = {};  // the tile to load next
+    if (active) {
+        end = cta + 1 == runs.P ? total : sh.edge[1];
+        if (sh.edge[0] < end) {
+            ld = sh.first;
+            if (ld.tile == ld.tiles) next_item(p.at, p.rows, p.cap, items, TT, end, ld);
+            else set_stop(ld, end);
+        }
     }
-    if (begin >= end) return;
-
-    Cursor ld, cc;  // the tile to load next, the tile to compute next
-    ld.row = sh.first_row;
-    ld.tokens = row_tokens(p.at, p.cap, ld.row);
-    ld.tiles = tiles_of(ld.tokens);
-    ld.item = (int)(sh.first_at / ld.tiles);
-    ld.tile = (int)(sh.first_at % ld.tiles);
-    cc = ld;
-    const int count = (int)(end - begin);
-    int to_load = count;
+    Cursor cc = ld;  // the item to compute next
 
     unsigned char* ring = smem + warp * S * kStage;
     const T* kbase = static_cast<const T*>(p.kv.k);
     const T* vbase = static_cast<const T*>(p.kv.v);
 
-    // Page of this lane's token (TILED: of the warp's 16 tokens; else lanes 0-15 have one
-    // each) of the tile at `ld`, looked up one tile ahead of its loads.  -1: past the
-    // row's tokens, or no such page.
-    const int32_t* pages = p.at.table + sequence_of(p.at, ld.row) * p.at.table_stride;
+    // Page of this lane's token of the tile at `ld` (TILED: lane i < H has that of the
+    // i-th box; else lane i < WT that of token i), looked up one tile ahead of its loads.
+    const int32_t* pages = p.at.table + (ld.tile < ld.stop ? sequence_of(p.at, ld.row) * p.at.table_stride : 0);
     int page = -1, in_page = 0;
     bool looked = false;
-    uint32_t filled = 0;  // TILED: byte s is the number of tokens on their way to stage s
-    bool failed = false;  // a bounded wait gave up: nothing more is loaded or computed
+    uint32_t pending = 0;  // TILED: bit s: a copy to stage s is on its way
+    bool failed = false;   // a bounded wait gave up: nothing more is loaded or computed
+    const int my_tok = warp * WT + (TILED ? (lane % H) * kBoxTok : lane % WT);
     auto look_up = [&]() {  // only starts the table's load: what it names is checked when it is used
         page = -1;
         looked = false;
-        if (to_load <= 0) return;
-        const int tok = ld.tile * kTileTok + warp * kWarpTok + (TILED ? 0 : lane & 15);
+        if (ld.tile >= ld.stop) return;
+        const int tok = ld.tile * TT + my_tok;
         if (tok < ld.tokens) {
             looked = true;
             const uint32_t nth = quotient((uint32_t)tok, p.page_size);
@@ -285,48 +321,50 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
         }
     };
     auto load = [&](int stage) {
-        if (to_load > 0) {
+        if (ld.tile < ld.stop) {
             const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
+            const int left = ld.tokens - (ld.tile * TT + my_tok);  // tokens from this lane's on
             if (looked && (page < 0 || page >= p.kv.n_pages)) {
                 page = -1;
-                if (ld.item == 0 && lane < (TILED ? 1 : 16))
-                    atomicAdd(p.err, TILED ? (unsigned)min(kWarpTok, ld.tokens - (ld.tile * kTileTok + warp * kWarpTok)) : 1u);
+                if (ld.item == 0 && lane < (TILED ? H : WT)) atomicAdd(p.err, TILED ? (unsigned)min(kBoxTok, left) : 1u);
             }
+            uint32_t have;
             if constexpr (TILED) {
-                if (page >= 0) {
-                    filled |= (uint32_t)min(kWarpTok, ld.tokens - (ld.tile * kTileTok + warp * kWarpTok)) << (8 * stage);
-                    if (lane == 0) {
-                        const uint32_t dst = smem_u32(ring + stage * kStage);
-                        uint64_t* bar = &sh.full[warp][stage];
-                        mbar_expect(bar, kStage);
-                        tma_load(dst, &kmap, in_page, head, page, bar);
-                        tma_load(dst + kHalf, &vmap, in_page, head, page, bar);
+                const uint32_t mine = page < 0 ? 0u : left >= kBoxTok ? 0xffffu : (1u << left) - 1;
+                have = __shfl_sync(0xffffffffu, mine, 0);
+                if constexpr (H == 2) have |= __shfl_sync(0xffffffffu, mine, 1) << 16;
+                if (have) {
+                    pending |= 1u << stage;
+                    uint64_t* bar = &sh.full[warp][stage];
+                    const uint32_t dst = smem_u32(ring + stage * kStage);
+                    if (lane == 0) mbar_expect(bar, 2 * kBox * ((have & 0xffffu ? 1 : 0) + (have >> 16 ? 1 : 0)));
+                    __syncwarp();
+                    if (lane < H && page >= 0) {
+                        tma_load(dst + lane * kBox, &kmap, in_page, head, page, bar);
+                        tma_load(dst + kHalf + lane * kBox, &vmap, in_page, head, page, bar);
                     }
                 }
             } else {
                 const int64_t off = page < 0 ? -1
                                              : (int64_t)page * p.kv.page_stride + (int64_t)in_page * p.kv.token_stride +
                                                    (int64_t)head * p.kv.head_stride;
-                const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-                if (lane == 0) sh.valid[warp][stage] = have;
+                have = __ballot_sync(0xffffffffu, page >= 0) & kAll;
                 if (have) {
                     const uint32_t dst = smem_u32(ring + stage * kStage);
-#pragma unroll
-                    for (int i = 0; i < kWarpTok * C / 32; ++i) {
+#pragma unroll 4
+                    for (int i = 0; i < WT * C / 32; ++i) {
                         const int idx = i * 32 + lane, r = idx / C, ch = idx % C;
                         const int64_t ro = __shfl_sync(0xffffffffu, off, r);
-                        const uint32_t at = (uint32_t)chunk_at<D>(ch, r);
+                        const uint32_t at = (uint32_t)(r / kBoxTok * kBox + chunk_at<D>(ch, r % kBoxTok));
                         const int64_t el = ro < 0 ? 0 : ro + ch * 8;
                         cp_async16(dst + at, kbase + el, ro < 0 ? 0 : 16);
                         cp_async16(dst + kHalf + at, vbase + el, ro < 0 ? 0 : 16);
                     }
                 }
             }
-            --to_load;
-            if (++ld.tile == ld.tiles && to_load > 0) {
-                next_item(p.at, p.rows, p.cap, items, ld);
+            if (lane == 0) sh.valid[warp][stage] = have;
+            if (++ld.tile == ld.stop && next_item(p.at, p.rows, p.cap, items, TT, end, ld))
                 pages = p.at.table + sequence_of(p.at, ld.row) * p.at.table_stride;
-            }
             look_up();
         }
         if constexpr (!TILED) cp_commit();
@@ -339,9 +377,32 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
         v_at[k] = chunk_at<D>(2 * k + (lane >> 4), lane & 15) + kHalf;
     }
 
+    // q of the query heads of the item at `cc`, f32: loaded ahead of its use
+    float2 x[KS][2];
+    auto load_q = [&]() {
+        const int kvh = p.head_groups == 1 ? cc.item : cc.item / p.head_groups, hg = cc.item - kvh * p.head_groups;
+        const int nh = min(kHeads, p.group - hg * kHeads), hq = PACK ? g & 3 : g;
+        const float* qr = p.q + (int64_t)cc.row * p.q_stride + (int64_t)(kvh * p.group + hg * kHeads + hq) * D + c4 * 2;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                x[k][j] = hq < nh ? *reinterpret_cast<const float2*>(qr + k * 16 + j * 8) : make_float2(0.f, 0.f);
+    };
+
     look_up();
+    if (cc.tile < cc.stop) load_q();
 #pragma unroll
     for (int s = 0; s < (TILED ? S : S - 1); ++s) load(s);
+
+    // rows without tokens are zeros; rows whose place is out of range are counted
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const int tokens = row_tokens(p.at, p.cap, r), pos = p.at.positions[r];
+        if (tid == 0 && pos >= 0 && pos >= tokens) atomicAdd(p.err, 1u);
+        if (tokens == 0)
+            for (int i = tid; i < p.n_heads * D; i += kThreads) p.out[(int64_t)r * p.n_heads * D + i] = 0.f;
+    }
+    if (cc.tile >= cc.stop) return;
 
     // A fragments of q: [k][0..3] = rows g, g + 8 at (k = 2c, 2c+1), then at (2c+8, 2c+9).  The
     // third pieces of two k steps share one fragment, in rows 0-7 and 8-15: each step's MMA
@@ -351,27 +412,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     uint32_t qa[q_in_smem(D) ? 1 : KS / 2][2 * QW];
     int stage = 0;
     uint32_t phase = 0;  // bit s: parity of stage s's next completed copy
-    long long done = 0;  // tiles of the run behind cc
-    while (done < count) {
-        // ---- one item: query heads h0..h0+nh of a row, tiles [cc.tile, cc.tile + n)
-        const int n = (int)min((long long)(cc.tiles - cc.tile), (long long)count - done);
-        const int kvh = cc.item / p.head_groups, hg = cc.item % p.head_groups;
+    for (;;) {
+        // ---- one item, or this run's piece of it: query heads h0..h0+nh of a row
+        const int row = cc.row, tiles = cc.stop - cc.tile;
+        const bool whole = tiles == cc.tiles;
+        const int kvh = p.head_groups == 1 ? cc.item : cc.item / p.head_groups, hg = cc.item - kvh * p.head_groups;
         const int h0 = kvh * p.group + hg * kHeads, nh = min(kHeads, p.group - hg * kHeads);
         float scale = p.scale;
         {
-            const int hq = PACK ? g & 3 : g;
-            const float* qr = p.q + (int64_t)cc.row * p.q_stride + (int64_t)(h0 + (hq < nh ? hq : 0)) * D + c4 * 2;
-            float2 x[KS][2];
-            float top = 0.f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    x[k][j] = hq < nh ? *reinterpret_cast<const float2*>(qr + k * 16 + j * 8) : make_float2(0.f, 0.f);
-                    top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
-                }
             if constexpr (N == 2) {
                 // f16 pieces: bring the head's largest |q| into [2^7, 2^8)
+                float top = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int e = max(-100, min(100, 134 - (int)((__float_as_uint(top) >> 23) & 255)));
@@ -411,14 +466,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
         for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = 0.f;
         float m = -INFINITY, l = 0.f;  // running maximum (scaled, less kShift) and this lane's part of the sum
 
-        for (int t = 0; t < n; ++t) {
+        for (int t = 0; t < tiles; ++t) {
             const int cur = stage;
             stage = stage + 1 == S ? 0 : stage + 1;
             const uint32_t base = smem_u32(ring + cur * kStage);
             uint32_t have;  // bit per token
             if constexpr (TILED) {
                 if (failed) continue;
-                have = (1u << ((filled >> (8 * cur)) & 255)) - 1;
+                have = sh.valid[warp][cur];
                 if (have) {
                     if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[warp][cur], (phase >> cur) & 1))) {
                         if (lane == 0) atomicAdd(p.err + 1, 1u);
@@ -426,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                         continue;
                     }
                     phase ^= 1u << cur;
-                    filled &= ~(255u << (8 * cur));
+                    pending &= ~(1u << cur);
                 }
             } else {
                 cp_wait<S - 2>();
@@ -435,20 +490,28 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                 have = sh.valid[warp][cur];
             }
             if (have == 0) {
-                if constexpr (TILED) load(cur);
+                if constexpr (TILED) {
+                    __syncwarp();  // every lane has read `valid`
+                    load(cur);
+                }
                 continue;
             }
-            if (TILED && have != 0xffffu) {
-                // slots behind the last token may hold anything, also NaN: their values are zeroed
-                for (int i = lane; i < kWarpTok * C; i += 32)
-                    if (!((have >> (i / C)) & 1))
-                        *reinterpret_cast<uint4*>(ring + cur * kStage + kHalf + chunk_at<D>(i % C, i / C)) = make_uint4(0, 0, 0, 0);
+            if (TILED && have != kAll) {
+                // slots behind the last token may hold anything, also NaN, and boxes without a page
+                // what was there before: their values are zeroed (their scores are replaced below)
+#pragma unroll
+                for (int n = 0; n < WT * C / 32; ++n) {
+                    const int i = n * 32 + lane, r = i / C;
+                    if (!((have >> r) & 1))
+                        *reinterpret_cast<uint4*>(ring + cur * kStage + kHalf + r / kBoxTok * kBox + chunk_at<D>(i % C, r % kBoxTok)) =
+                            make_uint4(0, 0, 0, 0);
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
 
-            // ---- s = q . k for 16 tokens: two 8-token MMA columns
-            float acc[2][2][4], low[2][2][4];
+            // ---- s = q . k: two 8-token MMA columns a box
+            float acc[H][2][2][4], low[H][2][2][4];
 #pragma unroll
             for (int k = 0; k < KS; k += 2) {
                 uint32_t a[2 * QW];
@@ -460,72 +523,91 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     for (int i = 0; i < 2 * QW; ++i) a[i] = qa[k / 2][i];
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t b[4];
-                    ldmatrix4(b, base + (k + i) / CP2 * kPart + k_at[(k + i) % CP2]);
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if (k == 0) mma0(acc[j][i], a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3], b[2 * j], b[2 * j + 1], T());
-                        else mma(acc[j][i], a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3], b[2 * j], b[2 * j + 1], T());
-                        if constexpr (THIRD) {
-                            if (k == 0) mma0(low[j][i], a[8], a[9], a[10], a[11], b[2 * j], b[2 * j + 1], T());
-                            else mma(low[j][i], a[8], a[9], a[10], a[11], b[2 * j], b[2 * j + 1], T());
+                    for (int h = 0; h < H; ++h) {
+                        uint32_t b[4];
+                        ldmatrix4(b, base + h * kBox + (k + i) / CP2 * kPart + k_at[(k + i) % CP2]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if (k == 0) mma0(acc[h][j][i], a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3], b[2 * j], b[2 * j + 1], T());
+                            else mma(acc[h][j][i], a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3], b[2 * j], b[2 * j + 1], T());
+                            if constexpr (THIRD) {
+                                if (k == 0) mma0(low[h][j][i], a[8], a[9], a[10], a[11], b[2 * j], b[2 * j + 1], T());
+                                else mma(low[h][j][i], a[8], a[9], a[10], a[11], b[2 * j], b[2 * j + 1], T());
+                            }
                         }
                     }
+            }
+            float s[H][4];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = i >> 1, e = i & 1;
+                    s[h][i] = acc[h][j][0][e + 2] + acc[h][j][1][e + 2];
+                    if constexpr (THIRD) s[h][i] += low[h][j][0][e] + low[h][j][1][e + 2];
+                    s[h][i] += acc[h][j][0][e] + acc[h][j][1][e];
+                    if constexpr (PACK) s[h][i] += __shfl_xor_sync(0xffffffffu, s[h][i], 16);
                 }
-            }
-            float s[4];
+            if (have != kAll) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = i >> 1, e = i & 1;
-                s[i] = acc[j][0][e + 2] + acc[j][1][e + 2];
-                if constexpr (THIRD) s[i] += low[j][0][e] + low[j][1][e + 2];
-                s[i] += acc[j][0][e] + acc[j][1][e];
-                if constexpr (PACK) s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
-            }
-            if (have != 0xffffu) {
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!((have >> (8 * (i >> 1) + 2 * c4 + (i & 1))) & 1)) s[i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i)
+                        if (!((have >> (16 * h + 8 * (i >> 1) + 2 * c4 + (i & 1))) & 1)) s[h][i] = -INFINITY;
             }
-            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            float top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < H; ++h) top = fmaxf(top, fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3])));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float m_new = fmaxf(m, top * scale - kShift<T>);
             const float ref = m_new == -INFINITY ? 0.f : m_new;
             const float alpha = ex2(m - ref);
             m = m_new;
-            float w[4];
+            // ---- p, in pieces
+            uint32_t pa[H][2][N];
+            float more = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = ex2(fmaf(s[i], scale, -ref));
-            l = l * alpha + ((w[0] + w[1]) + (w[2] + w[3]));
-
-            // ---- o = o * alpha + p . v
-            uint32_t pa[2][N];
-            cut<N, T>(pa[0], w[0], w[1]);
-            cut<N, T>(pa[1], w[2], w[3]);
-            if constexpr (PACK) {
+            for (int h = 0; h < H; ++h) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = ex2(fmaf(s[h][i], scale, -ref));
+                more += (w[0] + w[1]) + (w[2] + w[3]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    pa[j][0] = g >= 4 ? pa[j][2] : pa[j][0];
-                    pa[j][1] = g >= 4 ? 0u : pa[j][1];
+                    cut<N, T>(pa[h][j], w[2 * j], w[2 * j + 1]);
+                    if constexpr (PACK) {
+                        pa[h][j][0] = g >= 4 ? pa[h][j][2] : pa[h][j][0];
+                        pa[h][j][1] = g >= 4 ? 0u : pa[h][j][1];
+                    }
                 }
             }
+            l = fmaf(l, alpha, more);
+
+            // ---- o = o * alpha + p . v
 #pragma unroll
             for (int c = 0; c < NT; c += 2) {
-                uint32_t b[4];
-                ldmatrix4_t(b, base + c / 2 / CP2 * kPart + v_at[c / 2 % CP2]);
+                float d[2][4];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    uint32_t b[4];
+                    ldmatrix4_t(b, base + h * kBox + c / 2 / CP2 * kPart + v_at[c / 2 % CP2]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if constexpr (THIRD) {
+                            if (h == 0) mma0(d[j], pa[h][0][2], 0u, pa[h][1][2], 0u, b[2 * j], b[2 * j + 1], T());
+                            else mma(d[j], pa[h][0][2], 0u, pa[h][1][2], 0u, b[2 * j], b[2 * j + 1], T());
+                        }
+                        if (h == 0 && !THIRD) mma0(d[j], pa[h][0][0], pa[h][0][1], pa[h][1][0], pa[h][1][1], b[2 * j], b[2 * j + 1], T());
+                        else mma(d[j], pa[h][0][0], pa[h][0][1], pa[h][1][0], pa[h][1][1], b[2 * j], b[2 * j + 1], T());
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float d[4];
-                    if constexpr (THIRD) {
-                        mma0(d, pa[0][2], 0u, pa[1][2], 0u, b[2 * j], b[2 * j + 1], T());
-                        mma(d, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b[2 * j], b[2 * j + 1], T());
-                    } else {
-                        mma0(d, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b[2 * j], b[2 * j + 1], T());
-                    }
-                    o[c + j][0] = fmaf(o[c + j][0], alpha, d[0] + d[2]);
-                    o[c + j][1] = fmaf(o[c + j][1], alpha, d[1] + d[3]);
+                    o[c + j][0] = fmaf(o[c + j][0], alpha, d[j][0] + d[j][2]);
+                    o[c + j][1] = fmaf(o[c + j][1], alpha, d[j][1] + d[j][3]);
                 }
             }
             if constexpr (TILED) {
@@ -534,14 +616,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
             }
         }
 
+        uint32_t c0 = cta, c1 = cta;
+        if (!whole) item_runs(runs, cc.begin, cc.tiles, c0, c1);
+        next_item(p.at, p.rows, p.cap, items, TT, end, cc);
+        const bool more = cc.tile < cc.stop;
+        if (more) load_q();
+
         // ---- join the four warps
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (c4 == 0) sh.m[warp][g] = m, sh.l[warp][g] = l;
-        const long long item_begin = begin + done - cc.tile, item_end = item_begin + cc.tiles;
-        const long long c0 = run_of(total, P, item_begin), c1 = run_of(total, P, item_end - 1);
-        const bool whole = c0 == c1;
-        float* slot = p.part + (2 * cta + (cta == c0 ? 1 : 0)) * slot_floats(D);
+        float* slot = p.part + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * slot_floats(D);
 #pragma unroll
         for (int col0 = 0; col0 < D; col0 += MC) {
             if (col0) __syncthreads();  // the previous columns are read
@@ -574,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                 if (h >= nh) continue;
                 if (whole) {
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    *reinterpret_cast<float4*>(p.out + ((int64_t)cc.row * p.n_heads + h0 + h) * D + col0 + col) =
+                    *reinterpret_cast<float4*>(p.out + ((int64_t)row * p.n_heads + h0 + h) * D + col0 + col) =
                         make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
                 } else {
                     __stcg(reinterpret_cast<float4*>(slot + h * D + col0 + col), a);
@@ -586,9 +671,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
             }
         }
         if (!whole) {
-            __threadfence();
             __syncthreads();
             if (tid == 0) {
+                __threadfence();
                 sh.last_in = atomicAdd(p.counters + c0, 1u) == (unsigned)(c1 - c0);
                 if (sh.last_in) p.counters[c0] = 0;
                 __threadfence();
@@ -596,46 +681,74 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
             __syncthreads();
             if (sh.last_in) {
                 // ---- this CTA is the last one of the item: join all, in CTA order
+                // A warp takes a head: lane i holds the maximum and the sum of the i-th CTA, then
+                // every lane adds its columns, 16 CTAs' loads in flight.
                 const int parts = (int)(c1 - c0) + 1;
-                const float* first = p.part + (2 * c0 + 1) * slot_floats(D);
-                const float* rest = p.part + 2 * c0 * slot_floats(D);
-                auto part_of = [&](int i) { return i == 0 ? first : rest + (int64_t)2 * i * slot_floats(D); };
+                const float* first = p.part + (size_t)(2 * c0 + 1) * slot_floats(D);
+                const float* rest = p.part + (size_t)(2 * c0) * slot_floats(D);
+                auto part_of = [&](int i) { return i == 0 ? first : rest + (size_t)(2 * i) * slot_floats(D); };
+                constexpr int V = D % 128 == 0 ? 4 : D == 64 ? 2 : 1, L = D / (32 * V);  // floats a load, loads a lane
+                constexpr int B = 16 / L;
                 for (int h = warp; h < nh; h += kWarps) {
-                    float top = -INFINITY;
-                    for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(part_of(i) + kHeads * D + h));
+                    float top = -INFINITY, sum = 0.f, acc[L][V] = {};
+                    for (int i0 = 0; i0 < parts; i0 += 32) {
+                        float m_i = -INFINITY, l_i = 0.f;
+                        if (i0 + lane < parts) {
+                            m_i = __ldcg(part_of(i0 + lane) + kHeads * D + h);
+                            l_i = __ldcg(part_of(i0 + lane) + kHeads * D + kHeads + h);
+                        }
+                        const int n32 = min(32, parts - i0);
+                        float weight = 0.f;
+                        for (int b = 0; b < n32; b += B) {
+                            float part[B][L][V];
 #pragma unroll
-                    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                    const float ref = top == -INFINITY ? 0.f : top;
-                    float sum = 0.f;
-                    for (int i = lane; i < parts; i += 32)
-                        sum += __ldcg(part_of(i) + kHeads * D + kHeads + h) * ex2(__ldcg(part_of(i) + kHeads * D + h) - ref);
+                            for (int i = 0; i < B; ++i) {
+                                const float* from = part_of(i0 + min(b + i, n32 - 1)) + h * D + lane * V;
+#pragma unroll
+                                for (int j = 0; j < L; ++j) load_cg<V>(part[i][j], from + j * 32 * V);
+                            }
+                            if (b == 0) {  // the maximum over these CTAs, behind the loads
+                                float t = m_i;
+#pragma unroll
+                                for (int s = 16; s; s >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, s));
+                                t = fmaxf(t, top);
+                                const float ref = t == -INFINITY ? 0.f : t, alpha = ex2(top - ref);
+                                top = t;
+                                weight = ex2(m_i - ref);
+                                sum = fmaf(sum, alpha, l_i * weight);
+#pragma unroll
+                                for (int j = 0; j < L; ++j)
+#pragma unroll
+                                    for (int e = 0; e < V; ++e) acc[j][e] *= alpha;
+                            }
+#pragma unroll
+                            for (int i = 0; i < B; ++i) {
+                                const float f = __shfl_sync(0xffffffffu, weight, (b + i) & 31);
+                                const bool in = b + i < n32;
+#pragma unroll
+                                for (int j = 0; j < L; ++j)
+#pragma unroll
+                                    for (int e = 0; e < V; ++e) acc[j][e] = fmaf(in ? part[i][j][e] : 0.f, in ? f : 0.f, acc[j][e]);
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-                    if (lane == 0) sh.m[0][h] = ref, sh.l[0][h] = sum == 0.f ? 0.f : 1.0f / sum;
-                }
-                __syncthreads();
-                for (int idx = tid; idx < nh * (D / 4); idx += kThreads) {
-                    const int h = idx / (D / 4), col = idx % (D / 4) * 4;
-                    const float ref = sh.m[0][h], inv = sh.l[0][h];
-                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int i = 0; i < parts; ++i) {
-                        const float f = ex2(__ldcg(part_of(i) + kHeads * D + h) - ref);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(i) + h * D + col));
-                        a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
-                    }
-                    *reinterpret_cast<float4*>(p.out + ((int64_t)cc.row * p.n_heads + h0 + h) * D + col) =
-                        make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                    float* to = p.out + ((int64_t)row * p.n_heads + h0 + h) * D + lane * V;
+#pragma unroll
+                    for (int j = 0; j < L; ++j)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) to[j * 32 * V + e] = acc[j][e] * inv;
                 }
             }
         }
-        done += n;
-        if (done < count) next_item(p.at, p.rows, p.cap, items, cc);
+        if (!more) break;
     }
     if constexpr (TILED) {
         if (failed)  // copies in flight must not land after the CTA has gone
             for (int i = 0; i < S; ++i)
-                if ((filled >> (8 * i)) & 255) mbar_wait(&sh.full[warp][i], (phase >> i) & 1);
+                if ((pending >> i) & 1) mbar_wait(&sh.full[warp][i], (phase >> i) & 1);
     } else {
         cp_wait<0>();
     }
@@ -665,7 +778,7 @@ bool encode(CUtensorMap* map, void* base, const KvCache& kv) {
     const cuuint64_t dims[5] = {PE, (cuuint64_t)kv.page_size, D / PE, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_pages};
     const cuuint64_t strides[4] = {(cuuint64_t)kv.token_stride * 2, PE * 2, bytes(kv.n_kv, kv.head_stride),
                                    bytes(kv.n_pages, kv.page_stride)};
-    const cuuint32_t box[5] = {PE, kWarpTok, D / PE, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const cuuint32_t box[5] = {PE, kBoxTok, D / PE, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
     return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        PE == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -682,7 +795,7 @@ cudaError_t launch_typed(const AttnArgs& a, const CUtensorMap (&maps)[2], int sm
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) configured[dev] = true;
     }
-    const int64_t tiles = (int64_t)a.rows * a.n_kv * a.head_groups * ((a.cap + kTileTok - 1) / kTileTok);
+    const int64_t tiles = (int64_t)a.rows * a.n_kv * a.head_groups * tiles_of(a.cap, tile_tok(D));
     const int64_t ctas = (int64_t)sms * ctas_per_sm(D);
     return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)(tiles < ctas ? tiles : ctas)), kThreads,
                          smem_bytes(D), pdl, s, a, maps[0], maps[1]);
@@ -700,7 +813,7 @@ cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
     CUtensorMap maps[2] = {};
     // strides of 2^40 bytes and more do not fit a tensor map
     const bool fits = a.kv.token_stride < (1ll << 39) && a.kv.head_stride < (1ll << 39) && a.kv.page_stride < (1ll << 39);
-    if (a.kv.page_size % kWarpTok == 0 && fits && encode_fn() && encode<D>(&maps[0], a.kv.k, a.kv) && encode<D>(&maps[1], a.kv.v, a.kv))
+    if (a.kv.page_size % kBoxTok == 0 && fits && encode_fn() && encode<D>(&maps[0], a.kv.k, a.kv) && encode<D>(&maps[1], a.kv.v, a.kv))
         return launch_tiled<D, true>(a, maps, sms, pdl, s);
     return launch_tiled<D, false>(a, maps, sms, pdl, s);
 }
@@ -734,6 +847,8 @@ cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t row
     const int64_t cap = at.max_pages * kv.page_size;
     a.cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
     a.scale = scale * 1.4426950408889634f;
+    a.min_share = getenv("MS") ? atoi(getenv("MS")) : 1;
+    a.snap = getenv("SN") ? atoi(getenv("SN")) : 2;
     a.out = out;
     a.part = part;
     a.counters = counters;

@@ -57,27 +57,75 @@ OCL_HD int row_tokens(const KvRows& at, int cap, int64_t row) {
     return pos >= cap ? cap : pos + 1;
 }
 
-constexpr int kWarpTok = 16, kTileWarps = 4, kTileTok = kWarpTok * kTileWarps;  // attention: tokens of a tile
-OCL_HD int tiles_of(int tokens) { return (tokens + kTileTok - 1) / kTileTok; }
+OCL_HD int tiles_of(int tokens, int tile_tok) { return (tokens + tile_tok - 1) / tile_tok; }
 
-// `total` tiles in P <= total runs: run c is [run_begin(c), run_begin(c + 1)), never
-// empty; run_of(t) is the run that tile t lies in.
-OCL_HD long long run_begin(long long total, long long P, long long c) { return total * c / P; }
-OCL_HD long long run_of(long long total, long long P, long long t) { return ((t + 1) * P - 1) / total; }
-
-// A place in the order of all tiles: by row, item (k/v head and head group), tile.
-struct Cursor {
-    int row, item, tile, tokens, tiles;
+// The work of all items (an item: a row and group of heads; its tiles, after kItemCost
+// units for what an item costs by itself) in order, cut into P runs, one per CTA.
+// Cut c lies on unit c * total / P, up to a unit; one within `snap` tiles of an item's
+// edge moves to that edge, so that an item is not shared for a sliver of it, and items
+// of up to 2 * snap tiles are never shared.  All in 32 bits: total < 2^31.
+constexpr int kItemCost = 1;
+struct Runs {
+    uint32_t total, P, share, rest;  // total = P * share + rest
+    int snap;
 };
-OCL_HD void next_item(const KvRows& at, int rows, int cap, int items, Cursor& c) {
-    c.tile = 0;
-    if (++c.item < items) return;
-    c.item = 0;
-    c.tokens = 0;
-    do {
-        ++c.row;
-    } while (c.row < rows && (c.tokens = row_tokens(at, cap, c.row)) == 0);
-    c.tiles = tiles_of(c.tokens);
+OCL_HD uint32_t item_units(int tiles) { return (uint32_t)(tiles + kItemCost); }
+OCL_HD Runs runs_of(uint32_t total, uint32_t ctas, uint32_t min_share, int snap) {
+    Runs r;
+    r.total = total;
+    r.P = total / min_share;
+    r.P = r.P < 1 ? 1 : r.P < ctas ? r.P : ctas;
+    r.share = total / r.P;
+    r.rest = total - r.share * r.P;
+    r.snap = snap;
+    return r;
+}
+OCL_HD uint32_t run_cut(const Runs& r, uint32_t c) { return c * r.share + (c < r.rest ? c : r.rest); }
+// Largest c whose unmoved cut lies on unit u or before (u < total).
+OCL_HD uint32_t run_before(const Runs& r, uint32_t u) {
+    const uint32_t wide = r.rest * (r.share + 1);
+    return u < wide ? u / (r.share + 1) : r.rest + (u - wide) / r.share;
+}
+// Where a cut on unit u of an item moves: 0 (its start), item_units (the next one's), or u itself.
+OCL_HD uint32_t moved_cut(const Runs& r, uint32_t u, int tiles) {
+    const uint32_t low = (uint32_t)(kItemCost + (r.snap < tiles / 2 ? r.snap : tiles / 2)), all = item_units(tiles);
+    return u <= low ? 0 : all - u <= (uint32_t)r.snap ? all : u;
+}
+// First and last run that have a piece of the item that begins on unit `begin`.
+OCL_HD void item_runs(const Runs& r, uint32_t begin, int tiles, uint32_t& c0, uint32_t& c1) {
+    const int low = kItemCost + (r.snap < tiles / 2 ? r.snap : tiles / 2), high = kItemCost + tiles - r.snap - 1;
+    c0 = run_before(r, begin + (uint32_t)low);
+    c1 = high <= low ? c0 : run_before(r, begin + (uint32_t)high);
+}
+
+// A place in the order of all tiles.
+struct Cursor {
+    int row, item;   // item of the row: k/v head and group of query heads
+    int tokens, tiles;
+    int tile, stop;  // next tile, and where this run's piece of the item ends
+    uint32_t begin;  // the item's first unit
+};
+// `stop` of the item for a run that ends on (moved) unit `end`.
+OCL_HD void set_stop(Cursor& c, uint32_t end) {
+    const uint32_t behind = end - c.begin;  // > kItemCost
+    c.stop = behind >= item_units(c.tiles) ? c.tiles : (int)behind - kItemCost;
+}
+// On to the next item of the run; without one, tile == stop.  True: on another row.
+OCL_HD bool next_item(const KvRows& at, int rows, int cap, int items, int tile_tok, uint32_t end, Cursor& c) {
+    c.tile = c.stop = 0;
+    c.begin += item_units(c.tiles);
+    if (c.begin >= end) return false;
+    const bool other = ++c.item == items;
+    if (other) {
+        c.item = 0;
+        c.tokens = 0;
+        do {
+            ++c.row;
+        } while (c.row < rows && (c.tokens = row_tokens(at, cap, c.row)) == 0);
+        c.tiles = tiles_of(c.tokens, tile_tok);
+    }
+    set_stop(c, end);
+    return other;
 }
 
 }  // namespace ocl

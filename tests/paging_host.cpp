@@ -2,56 +2,83 @@
 #include "../ocelotl_b200/csrc/paging.cuh"
 
 using namespace ocl;
+constexpr int kTile = 64;
 
-// Walk every run of `ctas` CTAs as the attention kernel does.  For each visited
-// tile writes (row, item, tile, cta) to out; returns the number of tiles, or a
-// negative code where two runs disagree about an item that they share.
+static uint32_t units_of(const KvRows& at, int cap, int items, int r) {
+    const int tokens = row_tokens(at, cap, r);
+    return tokens ? item_units(tiles_of(tokens, kTile)) * (uint32_t)items : 0;
+}
+
+// Walk every run of the CTAs as the attention kernel does.  For each visited tile
+// writes (row, item, tile, cta) to out; returns the number of tiles, or a negative
+// code where two runs disagree about an item that they share.
 extern "C" long long walk(const int32_t* positions, const int32_t* seqs, long long n_seqs, int rows, int cap, int items,
-                          long long ctas, int32_t* out, long long room) {
+                          unsigned ctas, unsigned min_share, int snap, int32_t* out, long long room) {
     const KvRows at{positions, seqs, nullptr, n_seqs, 0, 0};
-    long long total = 0;
-    for (int r = 0; r < rows; ++r) total += tiles_of(row_tokens(at, cap, r));
-    total *= items;
-    const long long P = total < ctas ? total : ctas;
+    uint32_t total = 0;
+    long long tiles = 0;
+    for (int r = 0; r < rows; ++r) {
+        total += units_of(at, cap, items, r);
+        tiles += (long long)tiles_of(row_tokens(at, cap, r), kTile) * items;
+    }
+    if (!total) return 0;
+    const Runs runs = runs_of(total, ctas, min_share, snap);
+    if (run_cut(runs, 0) != 0 || run_cut(runs, runs.P) != total) return -9;
     long long seen = 0;
-    for (long long c = 0; c < P; ++c) {
-        const long long begin = run_begin(total, P, c), end = run_begin(total, P, c + 1);
-        if (begin >= end) return -1;
-        long long at_row = 0;
-        int r = 0;
-        for (;; ++r) {
-            const long long n = (long long)tiles_of(row_tokens(at, cap, r)) * items;
-            if (begin < at_row + n) break;
-            at_row += n;
+    uint32_t last_end = 0;
+    for (uint32_t c = 0; c < runs.P; ++c) {
+        uint32_t edge[2];
+        Cursor cc{};
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t cut = run_cut(runs, c + i);
+            edge[i] = total;
+            uint32_t before = 0;
+            for (int r = 0; r < rows; ++r) {
+                const uint32_t n = units_of(at, cap, items, r);
+                if (cut < before + n) {
+                    Cursor e{};
+                    e.row = r;
+                    e.tokens = row_tokens(at, cap, r);
+                    e.tiles = tiles_of(e.tokens, kTile);
+                    const uint32_t all = item_units(e.tiles), off = cut - before, u = off % all;
+                    e.item = (int)(off / all);
+                    e.begin = cut - u;
+                    const uint32_t moved = moved_cut(runs, u, e.tiles);
+                    edge[i] = e.begin + moved;
+                    e.tile = moved == 0 ? 0 : (int)moved - kItemCost;  // == tiles: at its end
+                    if (i == 0) cc = e;
+                    break;
+                }
+                before += n;
+            }
         }
-        Cursor cc{r, 0, 0, row_tokens(at, cap, r), 0};
-        cc.tiles = tiles_of(cc.tokens);
-        cc.item = (int)((begin - at_row) / cc.tiles);
-        cc.tile = (int)((begin - at_row) % cc.tiles);
-        const long long count = end - begin;
+        if (edge[0] != last_end) return -1;
+        last_end = edge[1];
+        if (edge[0] >= edge[1]) continue;
+        if (cc.tile == cc.tiles) next_item(at, rows, cap, items, kTile, edge[1], cc);
+        else set_stop(cc, edge[1]);
         int starts = 0, goes_on = 0;  // shared items that this run starts, and that it continues
-        for (long long done = 0; done < count;) {
-            const long long left = count - done, n = cc.tiles - cc.tile < left ? cc.tiles - cc.tile : left;
-            const long long b = begin + done - cc.tile, e = b + cc.tiles;
-            const long long c0 = run_of(total, P, b), c1 = run_of(total, P, e - 1);
+        while (cc.tile < cc.stop) {
+            uint32_t c0, c1;
+            item_runs(runs, cc.begin, cc.tiles, c0, c1);
             if (c < c0 || c > c1) return -2;
-            if (run_begin(total, P, c0) > b || (c0 + 1 <= P && run_begin(total, P, c0 + 1) <= b)) return -3;
+            if ((c == c0) != (cc.tile == 0)) return -3;          // the first piece starts the item
+            if ((c == c1) != (cc.stop == cc.tiles)) return -8;   // the last one ends it
             if (c0 != c1) {
                 if (c == c0) ++starts;
                 else ++goes_on;
             }
-            if ((c0 == c1) != (n == cc.tiles)) return -4;
-            for (long long t = 0; t < n; ++t, ++seen) {
+            if ((c0 == c1) != (cc.tile == 0 && cc.stop == cc.tiles)) return -4;
+            for (int t = cc.tile; t < cc.stop; ++t, ++seen) {
                 if (seen >= room) return -5;
                 int32_t* o = out + 4 * seen;
-                o[0] = cc.row, o[1] = cc.item, o[2] = cc.tile + (int)t, o[3] = (int32_t)c;
+                o[0] = cc.row, o[1] = cc.item, o[2] = t, o[3] = (int32_t)c;
             }
-            done += n;
-            if (done < count) next_item(at, rows, cap, items, cc);
+            next_item(at, rows, cap, items, kTile, edge[1], cc);
         }
         if (starts > 1 || goes_on > 1) return -6;  // one workspace slot each
     }
-    return seen == total ? seen : -7;
+    return seen == tiles && last_end == total ? seen : -7;
 }
 
 extern "C" int place(const int32_t* table, long long max_pages, long long stride, long long n_pages, unsigned page_size,

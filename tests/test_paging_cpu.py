@@ -17,20 +17,20 @@ def lib(tmp_path_factory):
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", str(HERE / "paging_host.cpp"), "-o", str(so)], check=True)
     lib = C.CDLL(str(so))
     lib.walk.restype = C.c_longlong
-    lib.walk.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong]
+    lib.walk.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_uint, C.c_uint, C.c_int, C.c_void_p, C.c_longlong]
     lib.place.argtypes = [C.c_void_p] + [C.c_longlong] * 3 + [C.c_uint, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p]
     lib.wrong_quotient.restype = C.c_longlong
     lib.wrong_quotient.argtypes = [C.c_uint] + [C.c_longlong] * 3
     return lib
 
 
-def walk(lib, positions, cap, items, ctas, seqs=None, n_seqs=None):
+def walk(lib, positions, cap, items, ctas, snap=0, min_share=1, seqs=None, n_seqs=None):
     pos = np.asarray(positions, np.int32)
     sq = None if seqs is None else np.asarray(seqs, np.int32)
     room = int(sum(-(-(min(p + 1, cap)) // TILE) for p in pos.astype(int) if p >= 0)) * items + 1
     out = np.full((room, 4), -1, np.int32)
     n = lib.walk(pos.ctypes.data, None if sq is None else sq.ctypes.data, len(pos) if n_seqs is None else n_seqs, len(pos),
-                 cap, items, ctas, out.ctypes.data, room)
+                 cap, items, ctas, min_share, snap, out.ctypes.data, room)
     assert n >= 0, n
     return out[:n]
 
@@ -42,13 +42,19 @@ def walk(lib, positions, cap, items, ctas, seqs=None, n_seqs=None):
 ])
 def test_every_tile_once_and_shares_agree(lib, positions, items, ctas):
     cap = 140000
+    for snap in (1, 2, 5, 64):
+        moved = walk(lib, positions, cap, items, ctas, snap, min_share=1 + snap % 4)
     got = walk(lib, positions, cap, items, ctas)
+    assert np.array_equal(moved[:, :3], got[:, :3])
     want = [(r, i, t) for r, p in enumerate(positions) if p >= 0
             for i in range(items) for t in range(-(-min(p + 1, cap) // TILE))]
     assert [tuple(x[:3]) for x in got.tolist()] == want
     if len(want):
-        per = np.bincount(got[:, 3])
-        assert per.min() >= 1 and per.max() - per.min() <= 1  # equal runs
+        # without moved cuts every run has an equal share of units (a tile, or an item's start), but for one
+        # unit of rounding and the one that a cut within an item's start moves at either end
+        total = len(want) + sum(1 for p in positions if p >= 0) * items
+        cost = np.bincount(got[:, 3]) + np.bincount(got[got[:, 2] == 0][:, 3], minlength=got[:, 3].max() + 1)
+        assert cost.max() <= -(-total // min(ctas, total)) + 2
 
 
 def test_random_batches(lib):
@@ -56,7 +62,16 @@ def test_random_batches(lib):
     for _ in range(200):
         rows = int(rng.integers(1, 40))
         pos = np.where(rng.random(rows) < 0.2, -1, rng.integers(0, int(rng.choice([2, 70, 900, 9000])), rows))
-        walk(lib, pos, int(rng.integers(1, 9000)), int(rng.integers(1, 17)), int(rng.integers(1, 300)))
+        walk(lib, pos, int(rng.integers(1, 9000)), int(rng.integers(1, 17)), int(rng.integers(1, 300)),
+             snap=int(rng.integers(0, 9)), min_share=int(rng.integers(1, 12)))
+
+
+def test_short_items_are_not_shared(lib):
+    got = walk(lib, [255] * 16, 4096, 8, 296, snap=2)  # 128 items of 4 tiles
+    owners = {}
+    for r, i, _, c in got.tolist():
+        owners.setdefault((r, i), set()).add(c)
+    assert all(len(v) == 1 for v in owners.values())
 
 
 def test_rows_of_unknown_sequences_have_no_tiles(lib):
