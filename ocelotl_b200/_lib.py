@@ -7,6 +7,7 @@ path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libocelotl_cuda.so"
@@ -28,10 +29,9 @@ class KvCacheDesc(C.Structure):
         "n_pages", "page_size", "n_kv_heads", "head_dim", "page_stride", "head_stride", "token_stride")]
 
 
-class KvRowsDesc(C.Structure):
-    """ocl_kv_rows"""
-    _fields_ = [("positions_dev", _vp), ("seqs_dev", _vp), ("block_table_dev", _vp), ("n_seqs", _sz),
-                ("max_pages", _sz), ("table_stride", _sz)]
+# ocl_kv_rows as bytes (packing them costs a quarter of a Structure): positions, seqs, block table, n_seqs,
+# max_pages, table_stride
+KV_ROWS = struct.Struct("PPPNNN")
 
 
 class LogitRulesDesc(C.Structure):
@@ -78,9 +78,9 @@ SIGNATURES = {
     "ocl_q_embed_rows": (C.c_int, [_vp, _vp, _vp, _sz, _vp]),
     "ocl_rope_create": (C.c_int, [_vp, _sz, C.c_double, _vp, C.c_int, C.POINTER(_vp)]),
     "ocl_rope_free": (C.c_int, [_vp]),
-    "ocl_qk_norm_rope": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(KvCacheDesc), C.POINTER(KvRowsDesc), _vp, _vp,
+    "ocl_qk_norm_rope": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(KvCacheDesc), C.c_char_p, _vp, _vp,
                                    C.c_float, _vp, _vp]),
-    "ocl_paged_attention": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(KvCacheDesc), C.POINTER(KvRowsDesc), C.c_float,
+    "ocl_paged_attention": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(KvCacheDesc), C.c_char_p, C.c_float,
                                       _vp]),
     "ocl_logits_process": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(LogitRulesDesc), _vp, _sz, _vp]),
     "ocl_take_device_errors": (C.c_int, [_vp, C.POINTER(C.c_uint), C.POINTER(C.c_uint)]),

@@ -30,6 +30,11 @@ from .ggml import GgmlType, byte_len, geometry
 BACKEND_ID = "cuda-sm100a"
 
 
+# torch's current stream of a device as a cudaStream_t, without building a Stream object (2 us) where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _kernel_err(message: str) -> KernelError:
     return KernelError(BACKEND_ID, message)
 
@@ -471,40 +476,41 @@ class CudaKernelBackend:
         """The rules of a batch of requests (see LogitRules), as process_logits and greedy_sample take them."""
         return LogitRules(self.torch_device, **parts)
 
-    def _empty(self, shape, dtype=torch.float32) -> torch.Tensor:
+    def _alloc(self, like: torch.Tensor, *shape: int, dtype: torch.dtype | None = None) -> torch.Tensor:
         """Device memory for an output, allocated on the stream that the kernels run on."""
         s = self._stream
-        if torch.cuda.current_stream(self.torch_device).cuda_stream == s:
+        if _raw_stream(self.device_index) == s:
+            if dtype is None:
+                return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(*shape)
             return torch.empty(shape, dtype=dtype, device=self.torch_device)
         stream = torch.cuda.default_stream(self.torch_device) if s == 0 else \
             torch.cuda.ExternalStream(s, device=self.torch_device)
         with torch.cuda.stream(stream):
-            return torch.empty(shape, dtype=dtype, device=self.torch_device)
+            return torch.empty(shape, dtype=dtype or like.dtype, device=self.torch_device)
 
-    def _out(self, out, shape: tuple, op: str) -> torch.Tensor:
+    def _out(self, out, like: torch.Tensor, op: str, *shape: int) -> torch.Tensor:
         if out is None:
-            return self._empty(shape)
-        if out.dtype != torch.float32 or out.device != self.torch_device or tuple(out.shape) != shape \
-                or not out.is_contiguous():
+            return self._alloc(like, *shape)
+        if not isinstance(out, torch.Tensor) or out.dtype is not torch.float32 or out.device != self.torch_device \
+                or out.shape != shape or not out.is_contiguous():
             raise _kernel_err(f"{op} out must be a contiguous f32 {list(shape)} tensor on {self.torch_device}")
         return out
 
-    def _rows(self, op: str, rows: int, cache: PagedKvCache, positions, block_table, seqs) -> _lib.KvRowsDesc:
+    def _rows(self, op: str, rows: int, cache: PagedKvCache, positions, block_table, seqs) -> bytes:
         dev = self.torch_device
-        if not isinstance(cache, PagedKvCache) or cache.k.device != dev:
+        if not isinstance(cache, PagedKvCache) or cache.device != dev:
             raise _kernel_err(f"{op} cache must be a PagedKvCache on {dev}")
-        check_tensor(positions, f"{op} positions", torch.int32, dev, 1)
-        check_tensor(block_table, f"{op} block_table", torch.int32, dev, 2)
-        if positions.shape[0] != rows:
-            raise _kernel_err(f"{op} positions.len()={positions.shape[0]} does not match rows={rows}")
+        check_tensor(positions, op, "positions", torch.int32, dev, 1)
+        check_tensor(block_table, op, "block_table", torch.int32, dev, 2)
+        if len(positions) != rows:
+            raise _kernel_err(f"{op} positions.len()={len(positions)} does not match rows={rows}")
         n_seqs, max_pages = block_table.shape
-        stride = block_table.stride(0) if n_seqs > 1 else max_pages
         if seqs is not None:
-            check_tensor(seqs, f"{op} seqs", torch.int32, dev, 1)
-            if seqs.shape[0] != rows:
-                raise _kernel_err(f"{op} seqs.len()={seqs.shape[0]} does not match rows={rows}")
-            return _lib.KvRowsDesc(positions.data_ptr(), seqs.data_ptr(), block_table.data_ptr(), n_seqs, max_pages, stride)
-        return _lib.KvRowsDesc(positions.data_ptr(), None, block_table.data_ptr(), n_seqs, max_pages, stride)
+            check_tensor(seqs, op, "seqs", torch.int32, dev, 1)
+            if len(seqs) != rows:
+                raise _kernel_err(f"{op} seqs.len()={len(seqs)} does not match rows={rows}")
+        return _lib.KV_ROWS.pack(positions.data_ptr(), 0 if seqs is None else seqs.data_ptr(), block_table.data_ptr(), n_seqs,
+                                 max_pages, block_table.stride(0) if n_seqs > 1 else max_pages)
 
     def qk_norm_rope(self, qkv: torch.Tensor, cache: PagedKvCache, positions: torch.Tensor, block_table: torch.Tensor,
                      rope: RopeTable | None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
@@ -518,7 +524,7 @@ class CudaKernelBackend:
         (zeros, nothing cached).  Places out of range cache nothing and count as bad
         ids (take_device_errors).  Rows of one call must stand at different places.
         """
-        check_tensor(qkv, "qk_norm_rope qkv", torch.float32, self.torch_device, 2)
+        check_tensor(qkv, "qk_norm_rope", "qkv", torch.float32, self.torch_device, 2)
         rows, width = qkv.shape
         at = self._rows("qk_norm_rope", rows, cache, positions, block_table, seqs)
         dim = cache.head_dim
@@ -527,12 +533,12 @@ class CudaKernelBackend:
             raise _kernel_err(f"qk_norm_rope qkv width {width} is not (n_heads + 2*{cache.n_kv_heads})*{dim}")
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
             if w is not None:
-                check_tensor(w, "qk_norm_rope " + name, torch.float32, self.torch_device, 1)
-                if w.shape[0] != dim:
-                    raise _kernel_err(f"qk_norm_rope {name}.len()={w.shape[0]} does not match head_dim={dim}")
-        out = self._out(out, (rows, heads, dim), "qk_norm_rope")
+                check_tensor(w, "qk_norm_rope", name, torch.float32, self.torch_device, 1)
+                if len(w) != dim:
+                    raise _kernel_err(f"qk_norm_rope {name}.len()={len(w)} does not match head_dim={dim}")
+        out = self._out(out, qkv, "qk_norm_rope", rows, heads, dim)
         rc = self._lib.ocl_qk_norm_rope(
-            self._ctx, qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, cache.ref, C.byref(at),
+            self._ctx, qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, cache.ref, at,
             None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
             None if rope is None else rope.handle, out.data_ptr())
         if rc:
@@ -548,21 +554,21 @@ class CudaKernelBackend:
         head_dim^-0.5; positions, block_table and seqs as for qk_norm_rope.  A
         negative position gives zeros.
         """
-        check_tensor(q, "paged_attention q", torch.float32, self.torch_device, 3)
+        check_tensor(q, "paged_attention", "q", torch.float32, self.torch_device, 3)
         rows, heads, dim = q.shape
         at = self._rows("paged_attention", rows, cache, positions, block_table, seqs)
         if dim != cache.head_dim or (heads > 1 and q.stride(1) != dim):
             raise _kernel_err(f"paged_attention q must hold heads of head_dim={cache.head_dim} side by side")
-        out = self._out(out, (rows, heads, dim), "paged_attention")
+        out = self._out(out, q, "paged_attention", rows, heads, dim)
         rc = self._lib.ocl_paged_attention(
-            self._ctx, q.data_ptr(), q.stride(0) if rows > 1 else heads * dim, rows, heads, cache.ref, C.byref(at),
+            self._ctx, q.data_ptr(), q.stride(0) if rows > 1 else heads * dim, rows, heads, cache.ref, at,
             dim ** -0.5 if scale is None else scale, out.data_ptr())
         if rc:
             self._check(rc)
         return out
 
     def _logits_call(self, op: str, logits: torch.Tensor, rules: LogitRules, out, ids) -> None:
-        check_tensor(logits, f"{op} logits", torch.float32, self.torch_device, 2)
+        check_tensor(logits, op, "logits", torch.float32, self.torch_device, 2)
         if not isinstance(rules, LogitRules) or rules.device != self.torch_device:
             raise _kernel_err(f"{op} rules must be LogitRules on {self.torch_device}")
         rows, vocab = logits.shape
@@ -571,13 +577,13 @@ class CudaKernelBackend:
         if rules.words is not None and rules.words * 32 < vocab:
             raise _kernel_err(f"{op} allowed mask has {rules.words} words a row, {vocab} tokens need {(vocab + 31) // 32}")
         if out is not None:
-            check_tensor(out, f"{op} out", torch.float32, self.torch_device, 2)
+            check_tensor(out, op, "out", torch.float32, self.torch_device, 2)
             if out.shape != logits.shape:
                 raise _kernel_err(f"{op} out {list(out.shape)} does not match logits {list(logits.shape)}")
         if ids is not None:
-            check_tensor(ids, f"{op} ids", torch.int32, self.torch_device, 1)
-            if ids.shape[0] != rows:
-                raise _kernel_err(f"{op} ids.len()={ids.shape[0]} does not match rows={rows}")
+            check_tensor(ids, op, "ids", torch.int32, self.torch_device, 1)
+            if len(ids) != rows:
+                raise _kernel_err(f"{op} ids.len()={len(ids)} does not match rows={rows}")
         rc = self._lib.ocl_logits_process(
             self._ctx, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, rules.ref,
             None if out is None else out.data_ptr(),
@@ -593,8 +599,8 @@ class CudaKernelBackend:
         result is written there in the same launch.
         """
         if out is None:
-            check_tensor(logits, "process_logits logits", torch.float32, self.torch_device, 2)
-            out = self._empty(tuple(logits.shape))
+            check_tensor(logits, "process_logits", "logits", torch.float32, self.torch_device, 2)
+            out = self._alloc(logits, *logits.shape)
         self._logits_call("process_logits", logits, rules, out, ids)
         return out
 
@@ -611,12 +617,12 @@ class CudaKernelBackend:
         returning the id as an int (copied in and out).
         """
         if rules is not None:
-            check_tensor(logits, "greedy_sample logits", torch.float32, self.torch_device,
+            check_tensor(logits, "greedy_sample", "logits", torch.float32, self.torch_device,
                          logits.dim() if isinstance(logits, torch.Tensor) and logits.dim() == 1 else 2)
             if logits.dim() == 1:
                 logits = logits.unsqueeze(0)
             if out is None:
-                out = self._empty((logits.shape[0],), torch.int32)
+                out = self._alloc(logits, logits.shape[0], dtype=torch.int32)
             self._logits_call("greedy_sample", logits, rules, None, out)
             return out
         if not isinstance(logits, torch.Tensor):

@@ -1049,6 +1049,13 @@ int ocl_paged_attention(ocl_ctx* ctx, const float* q, size_t q_stride, size_t ro
     if (rows == 0) return OCL_OK;
     if (!q || !out) return fail(ctx, OCL_ERR_INVALID, "paged_attention q/out pointer is null");
     if (misaligned(q) || misaligned(out)) return fail(ctx, OCL_ERR_INVALID, "paged_attention q and out must be 16-byte aligned");
+    // the work split counts 64-token tiles of every row, k/v head and group of 8 query heads in 31 bits
+    const double tiles = (double)rows * cache->n_kv_heads * ((n_heads / cache->n_kv_heads + 7) / 8) *
+                         ((double)at->max_pages * cache->page_size / 64 + 2);
+    if (tiles > 2147483647.0)
+        return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `paged_attention size` (requested `%zu rows, %zu k/v heads, "
+                    "block table of %zu tokens`): supported = [rows * heads * tokens / 64 < 2^31]", rows, cache->n_kv_heads,
+                    at->max_pages * cache->page_size);
     const size_t width = n_heads * cache->head_dim;
     if (overlap(q, q_stride, out, width, rows, width, width))
         return fail(ctx, OCL_ERR_INVALID, "paged_attention out overlaps q");
@@ -1082,9 +1089,9 @@ int ocl_logits_process(ocl_ctx* ctx, const float* logits, size_t in_stride, size
     if (r->allowed_dev && r->allowed_stride < (vocab + 31) / 32)
         return fail(ctx, OCL_ERR_INVALID, "process_logits allowed mask has %zu words a row, %zu tokens need %zu",
                     r->allowed_stride, vocab, (vocab + 31) / 32);
-    if (r->history_max > 0x7FFFFFFFu || r->bias_count > 0x7FFFFFFFu)
+    if (r->history_max > 0x3FFFFFFFu || r->bias_count > 0x3FFFFFFFu)
         return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `process_logits history` (requested `%zu` tokens, `%zu` "
-                    "biases): supported = [< 2^31]", r->history_max, r->bias_count);
+                    "biases): supported = [< 2^30]", r->history_max, r->bias_count);
     if ((r->history_dev && r->history_stride < r->history_max) || (r->bias_ids_dev && r->bias_stride < r->bias_count))
         return fail(ctx, OCL_ERR_INVALID, "process_logits history / bias row stride is below the row's length");
     if (rows == 0) return OCL_OK;

@@ -17,20 +17,19 @@
 //     bf16: 3 pieces of 8 bits = 24 bits;   f16: 2 pieces of 11 bits = 22 bits
 // (q scaled by a power of two per head, p by 2^14, so that f16's range is enough).
 // The tensor core truncates when it adds; chains are kept short (two chains over
-// head_dim, one 16-token step for p.v) and joined with rounding f32 adds.
+// head_dim, 32 tokens of p.v) and joined with rounding f32 adds.
 //
-// Work split: the tiles (64 tokens of one row and k/v head) of all rows, in order,
-// are cut into equal runs, one per resident CTA, from the positions in device
-// memory -- so one captured launch stays balanced while the lengths grow.  Each of
-// the 4 warps streams its own 16 tokens of a tile through a private ring of stages
-// and needs no barrier inside a run.  Where 16 tokens always lie in one page (page
-// sizes that are multiples of 16), one tensor-map copy (cp.async.bulk.tensor, its
-// swizzle doing the bank spreading) brings the keys and one the values; other page
-// sizes gather rows with cp.async.  A row whose tiles lie in
-// several CTAs is joined by the last of them to arrive, in CTA order: the result
-// does not depend on which one it is.  Nothing waits on another CTA.
+// Work split: the tiles (4 warps of 32 tokens of one row and k/v head) of all rows, in
+// order, are cut into equal runs, one per resident CTA, from the positions in device
+// memory -- so one captured launch stays balanced while the lengths grow (paging.cuh has
+// the arithmetic).  Each warp streams its own tokens through a private ring of stages and
+// needs no barrier inside an item.  Where 16 tokens always lie in one page (page sizes
+// that are multiples of 16), tensor-map copies (cp.async.bulk.tensor, its swizzle doing
+// the bank spreading) bring 16 keys or values each; other page sizes gather rows with
+// cp.async.  A row whose tiles lie in several CTAs is joined by the last of them to
+// arrive, in CTA order: the result does not depend on which one it is.  Nothing waits on
+// another CTA.
 #include <cuda.h>
-#include <cstdlib>
 
 #include "device.cuh"
 #include "internal.cuh"
@@ -87,7 +86,7 @@ struct AttnArgs {
     Divisor page_size;
     int cap;      // tokens a row of the block table can hold
     float scale;  // in units of log2
-    int min_share, snap;  // tiles: the least that a run gets, and how far a cut moves to an item's edge
+    int snap;     // tiles that a cut moves at most to reach an item's edge
     float* out;
     float* part;
     unsigned int* counters;
@@ -261,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     }
     // Pieces of an item cost their join: about a tenth of a tile's time each, so the
     // longest item is cut into no more than sqrt(10 * tiles) of them.
-    const Runs runs = runs_of(total, gridDim.x, max((uint32_t)p.min_share, (uint32_t)(sqrtf(0.1f * (float)longest) + 0.999f)), p.snap);
+    const Runs runs = runs_of(total, gridDim.x, max(1u, (uint32_t)(sqrtf(0.1f * (float)longest) + 0.999f)), p.snap);
     const uint32_t cta = blockIdx.x;
     const bool active = total > 0 && cta < runs.P;
     if (active) {
@@ -300,21 +299,25 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     const T* kbase = static_cast<const T*>(p.kv.k);
     const T* vbase = static_cast<const T*>(p.kv.v);
 
-    // Page of this lane's token of the tile at `ld` (TILED: lane i < H has that of the
-    // i-th box; else lane i < WT that of token i), looked up one tile ahead of its loads.
+    // Pages are looked up ahead of their loads.  TILED: for the next 32 / H tiles at once,
+    // lane i has the page of the (i % H)-th box of tile `window` + i / H.  Else for one
+    // tile, lane i < WT has that of token i.
     const int32_t* pages = p.at.table + (ld.tile < ld.stop ? sequence_of(p.at, ld.row) * p.at.table_stride : 0);
-    int page = -1, in_page = 0;
-    bool looked = false;
+    int page = -1, in_page = 0, window = 0, window_row = -1;
     uint32_t pending = 0;  // TILED: bit s: a copy to stage s is on its way
     bool failed = false;   // a bounded wait gave up: nothing more is loaded or computed
-    const int my_tok = warp * WT + (TILED ? (lane % H) * kBoxTok : lane % WT);
-    auto look_up = [&]() {  // only starts the table's load: what it names is checked when it is used
-        page = -1;
-        looked = false;
+    auto look_up = [&]() {  // only starts the table's loads: what they name is checked when it is used
         if (ld.tile >= ld.stop) return;
-        const int tok = ld.tile * TT + my_tok;
+        int tok = ld.tile * TT + warp * WT;
+        if constexpr (TILED) {
+            if (ld.row == window_row && (unsigned)(ld.tile - window) < 32 / H) return;
+            window_row = ld.row;
+            window = ld.tile;
+            tok += lane / H * TT + lane % H * kBoxTok;
+        } else {
+            tok += lane % WT;
+        }
         if (tok < ld.tokens) {
-            looked = true;
             const uint32_t nth = quotient((uint32_t)tok, p.page_size);
             in_page = (int)((uint32_t)tok - nth * p.page_size.d);
             page = pages[nth];
@@ -323,14 +326,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     auto load = [&](int stage) {
         if (ld.tile < ld.stop) {
             const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
-            const int left = ld.tokens - (ld.tile * TT + my_tok);  // tokens from this lane's on
-            if (looked && (page < 0 || page >= p.kv.n_pages)) {
-                page = -1;
+            // tokens from this lane's on, the lane's page and its slot there
+            const int left = ld.tokens - (ld.tile * TT + warp * WT + (TILED ? lane % H * kBoxTok : lane % WT));
+            int pg = page, slot = in_page;
+            if constexpr (TILED) {
+                const int from = (ld.tile - window) * H + lane % H;
+                pg = __shfl_sync(0xffffffffu, page, from);
+                slot = __shfl_sync(0xffffffffu, in_page, from);
+            }
+            if (left <= 0) {
+                pg = -1;
+            } else if (pg < 0 || pg >= p.kv.n_pages) {
+                pg = -1;
                 if (ld.item == 0 && lane < (TILED ? H : WT)) atomicAdd(p.err, TILED ? (unsigned)min(kBoxTok, left) : 1u);
             }
             uint32_t have;
             if constexpr (TILED) {
-                const uint32_t mine = page < 0 ? 0u : left >= kBoxTok ? 0xffffu : (1u << left) - 1;
+                const uint32_t mine = pg < 0 ? 0u : left >= kBoxTok ? 0xffffu : (1u << left) - 1;
                 have = __shfl_sync(0xffffffffu, mine, 0);
                 if constexpr (H == 2) have |= __shfl_sync(0xffffffffu, mine, 1) << 16;
                 if (have) {
@@ -339,16 +351,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     const uint32_t dst = smem_u32(ring + stage * kStage);
                     if (lane == 0) mbar_expect(bar, 2 * kBox * ((have & 0xffffu ? 1 : 0) + (have >> 16 ? 1 : 0)));
                     __syncwarp();
-                    if (lane < H && page >= 0) {
-                        tma_load(dst + lane * kBox, &kmap, in_page, head, page, bar);
-                        tma_load(dst + kHalf + lane * kBox, &vmap, in_page, head, page, bar);
+                    if (lane < H && pg >= 0) {
+                        tma_load(dst + lane * kBox, &kmap, slot, head, pg, bar);
+                        tma_load(dst + kHalf + lane * kBox, &vmap, slot, head, pg, bar);
                     }
                 }
             } else {
-                const int64_t off = page < 0 ? -1
-                                             : (int64_t)page * p.kv.page_stride + (int64_t)in_page * p.kv.token_stride +
-                                                   (int64_t)head * p.kv.head_stride;
-                have = __ballot_sync(0xffffffffu, page >= 0) & kAll;
+                const int64_t off = pg < 0 ? -1
+                                           : (int64_t)pg * p.kv.page_stride + (int64_t)slot * p.kv.token_stride +
+                                                 (int64_t)head * p.kv.head_stride;
+                have = __ballot_sync(0xffffffffu, pg >= 0) & kAll;
                 if (have) {
                     const uint32_t dst = smem_u32(ring + stage * kStage);
 #pragma unroll 4
@@ -785,7 +797,7 @@ bool encode(CUtensorMap* map, void* base, const KvCache& kv) {
 }
 
 template <int D, class T, bool TILED, bool PACK>
-cudaError_t launch_typed(const AttnArgs& a, const CUtensorMap (&maps)[2], int sms, bool pdl, cudaStream_t s) {
+cudaError_t launch_typed(AttnArgs a, const CUtensorMap (&maps)[2], int sms, bool pdl, cudaStream_t s) {
     static bool configured[kMaxDevices] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -795,10 +807,16 @@ cudaError_t launch_typed(const AttnArgs& a, const CUtensorMap (&maps)[2], int sm
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) configured[dev] = true;
     }
-    const int64_t tiles = (int64_t)a.rows * a.n_kv * a.head_groups * tiles_of(a.cap, tile_tok(D));
-    const int64_t ctas = (int64_t)sms * ctas_per_sm(D);
-    return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)(tiles < ctas ? tiles : ctas)), kThreads,
-                         smem_bytes(D), pdl, s, a, maps[0], maps[1]);
+    const int64_t items = (int64_t)a.rows * a.n_kv * a.head_groups, tiles = items * tiles_of(a.cap, tile_tok(D));
+    if (tiles + items > 0x7fffffff) return cudaErrorInvalidValue;  // the runs' arithmetic; checked by the caller
+    const int64_t ctas = tiles < (int64_t)sms * ctas_per_sm(D) ? tiles : (int64_t)sms * ctas_per_sm(D);
+    // With about as many items as CTAs, a short item is better left whole than shared (its
+    // join takes longer than its tiles: 16 rows of 555 tokens and 8 k/v heads 15.2 -> 11.1
+    // us, 230 rows of 5 to 180 tokens 15.3 -> 12.5); with fewer items every cut is wanted (one
+    // row of 1000 tokens and 8 k/v heads 9.3 us, with moved cuts 11.7).
+    a.snap = 2 * items >= ctas ? 2 : 0;
+    return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)ctas), kThreads, smem_bytes(D), pdl, s, a, maps[0],
+                         maps[1]);
 }
 
 template <int D, bool TILED>
@@ -847,8 +865,6 @@ cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t row
     const int64_t cap = at.max_pages * kv.page_size;
     a.cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
     a.scale = scale * 1.4426950408889634f;
-    a.min_share = getenv("MS") ? atoi(getenv("MS")) : 1;
-    a.snap = getenv("SN") ? atoi(getenv("SN")) : 2;
     a.out = out;
     a.part = part;
     a.counters = counters;

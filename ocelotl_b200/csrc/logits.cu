@@ -9,15 +9,16 @@
 // each step rounded to f32 on its own (no contraction), so the result is the
 // formula's to the bit.
 //
-// A CTA owns a run of a row's logits: it starts its logit loads, counts the row's
-// history into a shared-memory table of its own run (integer atomics: the order does
-// not show), adds up the biases that fall into the run, then applies everything to
-// the registers and stores.  Nothing of the size of the vocabulary is kept between
-// calls.  Bound: one read and one write of the logits; the history is read again by
-// every run of its row, from L2.
+// A CTA owns a run of a row's logits: it starts its logit and history loads, marks
+// the history's tokens that fall into the run in a shared-memory table (integer
+// atomics: their order does not show), adds up the biases that do, then applies
+// everything to the registers and stores.  Nothing of the size of the vocabulary is
+// kept between calls.  Bound: one read and one write of the logits; the history is
+// read again by every run of its row, from L2, with eight loads of a thread in flight.
 //
 // The greedy pick is argmax.cu's: one 64-bit key per run, the last run of a row
 // writes the id.
+#include <cstdlib>
 #include "device.cuh"
 #include "internal.cuh"
 
@@ -25,12 +26,14 @@ namespace ocl {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr uint32_t kPrompt = 0x80000000u;  // table word: seen in the prompt | times generated
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+// a table word: seen in the prompt | has a bias | times generated
+constexpr uint32_t kPrompt = 0x80000000u, kBiased = 0x40000000u, kTimes = 0x3fffffffu;
 
 struct RuleArgs {
     const float* logits;
-    int64_t in_stride, vocab;
+    int64_t in_stride;
+    int vocab;
     LogitRules r;
     float* out;
     int64_t out_stride;
@@ -44,17 +47,27 @@ struct RuleArgs {
 // whatever the row's own alignment: the run of CTA b starts at b * chunk - shift.
 template <int PER>
 __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p) {
-    constexpr int kChunk = kThreads * PER, G = PER / 4;
+    constexpr int kChunk = kThreads * PER, G = PER / 4, H = 8;
     __shared__ __align__(16) uint32_t table[kChunk];
-    __shared__ __align__(16) float bias[kChunk];
-    __shared__ unsigned long long warp_best[kThreads / 32];
+    __shared__ float bias[kChunk];  // only where the table says kBiased
+    __shared__ unsigned long long warp_best[kWarps];
     grid_wait();
     const int64_t row = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const float* x = p.logits + row * p.in_stride;
     const int shift = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-    const int64_t c0 = (int64_t)blockIdx.x * kChunk - shift;
+    const int64_t c0 = (int64_t)blockIdx.x * kChunk - shift;  // below 2^31 + a chunk
 
+    const bool counted = p.r.history != nullptr, biased = p.r.bias_ids != nullptr;
+    const int32_t* h = counted ? p.r.history + row * p.r.history_stride : nullptr;
+    int n = 0, prompt = 0;
+    int32_t seen[H];
+    if (counted) {
+        n = min(p.r.history_lens[row], (int)p.r.history_max);
+        prompt = p.r.prompt_lens ? p.r.prompt_lens[row] : 0;
+#pragma unroll
+        for (int j = 0; j < H; ++j) seen[j] = j * kThreads + tid < n ? __ldg(h + j * kThreads + tid) : -1;
+    }
     float v[G][4];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
@@ -68,54 +81,51 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
         }
     }
 
-    const bool counted = p.r.history != nullptr, biased = p.r.bias_ids != nullptr;
     if (counted || biased) {
-        for (int i = tid; i < kChunk / 4; i += kThreads) {
-            if (counted) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
-            // NaN with this payload: no bias on the token (a bias of 0 is one)
-            if (biased) reinterpret_cast<uint4*>(bias)[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+#pragma unroll
+        for (int j = 0; j < G; ++j) reinterpret_cast<uint4*>(table)[j * kThreads + tid] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        for (int b = 0; b < n; b += H * kThreads) {
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                const int i = b + j * kThreads + tid, t = seen[j];
+                const int64_t at = t - c0;
+                if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
+                if (t >= 0 && t < p.vocab && at >= 0 && at < kChunk) {
+                    if (i < prompt) atomicOr(table + at, kPrompt);
+                    else atomicAdd(table + at, 1u);
+                }
+                const int next = i + H * kThreads;
+                seen[j] = next < n ? __ldg(h + next) : -1;
+            }
+        }
+        if (biased && warp == kWarps - 1) {  // one warp, so that biases of one token add up in list order
+            const int32_t* ids = p.r.bias_ids + row * p.r.bias_stride;
+            const float* values = p.r.bias_values + row * p.r.bias_stride;
+            const int count = (int)p.r.bias_count;
+            int next = lane < count ? ids[lane] : -1;
+            for (int b = 0; b < count; b += 32) {
+                const int t = next;
+                next = b + 32 + lane < count ? ids[b + 32 + lane] : -1;
+                if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
+                const bool here = t >= 0 && t < p.vocab && t >= c0 && t < c0 + kChunk;
+                if (!__any_sync(0xffffffffu, here)) continue;
+                const float value = here ? values[b + lane] : 0.f;
+                const int at = here ? (int)(t - c0) : -1 - lane;
+                const uint32_t same = __match_any_sync(0xffffffffu, at);
+                if (here && (same & ((1u << lane) - 1)) == 0) {  // the first of its token in these 32
+                    const bool old = table[at] & kBiased;
+                    float sum = old ? __fadd_rn(bias[at], value) : value;
+                    for (uint32_t rest = same & ~(1u << lane); rest; rest &= rest - 1)
+                        sum = __fadd_rn(sum, values[b + __ffs(rest) - 1]);
+                    bias[at] = sum;
+                    if (!old) atomicOr(table + at, kBiased);
+                }
+                __syncwarp();
+            }
         }
         __syncthreads();
     }
-    if (counted) {
-        const int32_t* h = p.r.history + row * p.r.history_stride;
-        int64_t n = p.r.history_lens[row];
-        n = n < 0 ? 0 : n > p.r.history_max ? p.r.history_max : n;
-        const int64_t prompt = p.r.prompt_lens ? p.r.prompt_lens[row] : 0;
-        for (int64_t i = tid; i < n; i += kThreads) {
-            const int64_t t = h[i];
-            if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
-            const int64_t at = t - c0;
-            if (t >= 0 && t < p.vocab && at >= 0 && at < kChunk) {
-                if (i < prompt) atomicOr(table + at, kPrompt);
-                else atomicAdd(table + at, 1u);
-            }
-        }
-    }
-    if (biased && warp == kThreads / 32 - 1) {  // one warp, so that biases of one token add up in list order
-        const int32_t* ids = p.r.bias_ids + row * p.r.bias_stride;
-        const float* values = p.r.bias_values + row * p.r.bias_stride;
-        for (int64_t b = 0; b < p.r.bias_count; b += 32) {
-            const int64_t t = b + lane < p.r.bias_count ? ids[b + lane] : -1;
-            if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
-            const bool here = t >= 0 && t < p.vocab && t >= c0 && t < c0 + kChunk;
-            if (!__any_sync(0xffffffffu, here)) continue;
-            const float value = here ? values[b + lane] : 0.f;
-            const int at = here ? (int)(t - c0) : -1 - lane;
-            const uint32_t same = __match_any_sync(0xffffffffu, at);
-            const bool leads = here && __ffs(same) - 1 == lane;
-            float sum = 0.f;
-            bool any = false;
-            if (leads && __float_as_uint(bias[at]) != ~0u) sum = bias[at], any = true;
-            for (int k = 0; k < 32; ++k) {
-                const float f = __shfl_sync(0xffffffffu, value, k);
-                if ((same >> k) & 1) sum = any ? __fadd_rn(sum, f) : f, any = true;
-            }
-            if (leads) bias[at] = isnan(sum) ? __uint_as_float(0x7fc00000u) : sum;
-            __syncwarp();
-        }
-    }
-    if (counted || biased) __syncthreads();
 
     const float rep = counted && p.r.repetition ? p.r.repetition[row] : 1.f;
     const float freq = counted && p.r.frequency ? p.r.frequency[row] : 0.f;
@@ -124,35 +134,44 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
     const uint32_t* allowed = p.r.allowed ? p.r.allowed + row * p.r.allowed_stride : nullptr;
     float* y = p.out ? p.out + row * p.out_stride : nullptr;
     const bool vec_out = y && ((reinterpret_cast<uintptr_t>(y) >> 2) & 3) == (uintptr_t)shift;
-    unsigned long long best = 0;  // below every key of a number
+    float top = -INFINITY;  // this thread's pick: the first of its largest numbers
+    int top_at = -1;
+    bool nan_first = false;
 #pragma unroll
     for (int j = 0; j < G; ++j) {
         const int at = (j * kThreads + tid) * 4;
         const int64_t i = c0 + at;
         if (i + 4 <= 0 || i >= p.vocab) continue;
-        uint32_t seen[4] = {};
-        float add[4];
-        if (counted) *reinterpret_cast<uint4*>(seen) = *reinterpret_cast<const uint4*>(table + at);
-        if (biased) *reinterpret_cast<float4*>(add) = *reinterpret_cast<const float4*>(bias + at);
+        if (counted || biased) {
+            uint32_t w[4];
+            *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(table + at);
+            if (w[0] | w[1] | w[2] | w[3]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (i + e < 0 || i + e >= p.vocab) continue;
-            float l = v[j][e];
-            if (seen[e]) {
-                if (use_rep) l = l > 0.f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
-                const uint32_t c = seen[e] & ~kPrompt;
-                if (c && use_made) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)c)), pres);
-            }
-            if (biased && __float_as_uint(add[e]) != ~0u) l = __fadd_rn(l, add[e]);
-            if (allowed && !((allowed[(i + e) >> 5] >> ((i + e) & 31)) & 1)) l = -INFINITY;
-            v[j][e] = l;
-            if (p.ids) {
-                if (!isnan(l)) {
-                    const unsigned long long k = greedy_key(l, (uint32_t)(i + e));
-                    best = k > best ? k : best;
-                } else if (i + e == 0) {
-                    best = ~0ull;  // a NaN at token 0 is the pick, and the largest key says so
+                for (int e = 0; e < 4; ++e) {
+                    float l = v[j][e];
+                    if ((w[e] & ~kBiased) && use_rep) l = l > 0.f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
+                    const uint32_t c = w[e] & kTimes;
+                    if (c && use_made) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)c)), pres);
+                    if (w[e] & kBiased) l = __fadd_rn(l, bias[at + e]);
+                    v[j][e] = l;
                 }
+            }
+        }
+        if (allowed) {  // the 4 bits from token i on, which may lie in two words
+            const int64_t f = i < 0 ? 0 : i, g = i + 3 < p.vocab ? i + 3 : p.vocab - 1;
+            const uint32_t lo = allowed[f >> 5], hi = allowed[g >> 5];
+            const uint32_t bits = i < 0 ? lo << (int)-i : __funnelshift_r(lo, hi, (uint32_t)i & 31);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!((bits >> e) & 1)) v[j][e] = -INFINITY;
+        }
+        if (p.ids) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i + e < 0 || i + e >= p.vocab) continue;
+                const float l = v[j][e];
+                if (l > top || (top_at < 0 && l == top)) top = l, top_at = (int)(i + e);
+                if (i + e == 0) nan_first = isnan(l);
             }
         }
         if (vec_out && i >= 0 && i + 4 <= p.vocab) {
@@ -164,6 +183,8 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
         }
     }
     if (!p.ids) return;
+    // 0: no number here; a NaN at token 0 is the pick, and the largest key says so
+    unsigned long long best = nan_first ? ~0ull : top_at < 0 ? 0ull : greedy_key(top, (uint32_t)top_at);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
@@ -172,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
     if (lane == 0) warp_best[warp] = best;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kThreads / 32; ++w) best = warp_best[w] > best ? warp_best[w] : best;
+        for (int w = 1; w < kWarps; ++w) best = warp_best[w] > best ? warp_best[w] : best;
         if (best) atomicMax(p.slots + row, best);
         __threadfence();
         if (atomicAdd(p.counters + row, 1u) == gridDim.x - 1) {
@@ -197,8 +218,12 @@ cudaError_t launch_logit_rules(const float* logits, int64_t in_stride, int64_t r
                                const LogitRules& rules, float* out, int64_t out_stride, int32_t* ids,
                                unsigned long long* slots, unsigned int* counters, unsigned int* err, int sms, bool pdl,
                                cudaStream_t s) {
-    const RuleArgs a{logits, in_stride, vocab, rules, out, out_stride, ids, slots, counters, err};
+    const RuleArgs a{logits, in_stride, (int)vocab, rules, out, out_stride, ids, slots, counters, err};
     (void)sms;
+    switch (getenv("PER") ? atoi(getenv("PER")) : 16) {
+        case 4: return launch_per<4>(a, rows, pdl, s);
+        case 8: return launch_per<8>(a, rows, pdl, s);
+    }
     return launch_per<16>(a, rows, pdl, s);
 }
 

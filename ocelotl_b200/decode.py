@@ -25,10 +25,10 @@ def _err(message: str) -> KernelError:
     return KernelError("cuda-sm100a", message)
 
 
-def check_tensor(t, name: str, dtype: torch.dtype, device: torch.device, dims: int) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.dim() != dims \
-            or (dims and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise _err(f"{name} must be a {dims}-D {str(dtype)[6:]} tensor on {device} with a dense last dimension")
+def check_tensor(t, op: str, name: str, dtype: torch.dtype, device: torch.device, dims: int) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.dim() != dims \
+            or not (t.is_contiguous() or t.shape[-1] <= 1 or t.stride(-1) == 1):
+        raise _err(f"{op} {name} must be a {dims}-D {str(dtype)[6:]} tensor on {device} with a dense last dimension")
 
 
 class PagedKvCache:
@@ -49,7 +49,7 @@ class PagedKvCache:
             raise UnsupportedError("head_dim", str(k.shape[3]), [str(d) for d in HEAD_DIMS])
         if k.numel() == 0 or k.stride(3) != 1:
             raise _err("kv cache must not be empty and must hold the elements of a head side by side")
-        self.k, self.v = k, v
+        self.k, self.v, self.device = k, v, k.device
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         # a dimension of size 1 has no stride of its own
         stride = [k.stride(i) if k.shape[i] > 1 else self.head_dim for i in range(3)]
@@ -104,7 +104,7 @@ class LogitRules:
                  "allowed": (allowed, torch.int32, 2)}
         given = {n: t for n, (t, _, _) in parts.items() if t is not None}
         for n, t in given.items():
-            check_tensor(t, f"logit_rules {n}", parts[n][1], device, parts[n][2])
+            check_tensor(t, "logit_rules", n, parts[n][1], device, parts[n][2])
         if (history is None) != (history_lens is None):
             raise _err("logit_rules history and history_lens go together")
         if history is None and any(t is not None for t in (prompt_lens, repetition, frequency, presence)):
