@@ -1074,9 +1074,9 @@ int ocl_logits_process(ocl_ctx* ctx, const float* logits, size_t in_stride, size
     std::lock_guard<std::mutex> lk(ctx->mu);
     if (vocab == 0) return fail(ctx, OCL_ERR_INVALID, "process_logits requires at least one logit");
     if (!r) return fail(ctx, OCL_ERR_INVALID, "process_logits rules are null");
-    if (rows > (size_t)ocl::kArgmaxRowsMax || vocab > 0x7FFFFFFFu)
+    if (rows > (size_t)ocl::kArgmaxRowsMax || vocab > 0x7FFF0000u)
         return fail(ctx, OCL_ERR_UNSUPPORTED,
-                    "unsupported feature `process_logits shape` (requested `%zu x %zu`): supported = [rows <= %d, vocab < 2^31]",
+                    "unsupported feature `process_logits shape` (requested `%zu x %zu`): supported = [rows <= %d, vocab <= 2^31 - 65536]",
                     rows, vocab, ocl::kArgmaxRowsMax);
     if (in_stride < vocab || (out && out_stride < vocab))
         return fail(ctx, OCL_ERR_INVALID, "process_logits row stride is below vocab=%zu", vocab);

@@ -18,7 +18,6 @@
 //
 // The greedy pick is argmax.cu's: one 64-bit key per run, the last run of a row
 // writes the id.
-#include <cstdlib>
 #include "device.cuh"
 #include "internal.cuh"
 
@@ -45,39 +44,61 @@ struct RuleArgs {
 
 // PER logits a thread, in groups of 4 that are 16-byte aligned in `logits`
 // whatever the row's own alignment: the run of CTA b starts at b * chunk - shift.
+// Logits of the run outside the row are NaN, which no rule changes and no pick takes.
 template <int PER>
-__global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p) {
-    constexpr int kChunk = kThreads * PER, G = PER / 4, H = 8;
-    __shared__ __align__(16) uint32_t table[kChunk];
-    __shared__ float bias[kChunk];  // only where the table says kBiased
-    __shared__ unsigned long long warp_best[kWarps];
+__global__ void __launch_bounds__(kThreads, 5) logit_rules_kernel(const RuleArgs p) {
+    constexpr int kChunk = kThreads * PER, G = PER / 4, H = 4;
+    extern __shared__ __align__(16) uint32_t table[];
+    float* bias = reinterpret_cast<float*>(table + kChunk);  // only where the table says kBiased
+    __shared__ float warp_top[kWarps];
+    __shared__ uint32_t top_at;
     grid_wait();
     const int64_t row = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const float* x = p.logits + row * p.in_stride;
     const int shift = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-    const int64_t c0 = (int64_t)blockIdx.x * kChunk - shift;  // below 2^31 + a chunk
+    const int c0 = (int)blockIdx.x * kChunk - shift;
+    const int lo = max(c0, 0), skip = lo - c0;                     // the run's first token of the row, and its place
+    const uint32_t len = (uint32_t)max(min(c0 + kChunk, p.vocab) - lo, 0);  // its tokens of the row: none in a last run behind it
 
     const bool counted = p.r.history != nullptr, biased = p.r.bias_ids != nullptr;
     const int32_t* h = counted ? p.r.history + row * p.r.history_stride : nullptr;
-    int n = 0, prompt = 0;
+    const int room = counted ? (int)p.r.history_max : 0, count = biased ? (int)p.r.bias_count : 0;
+    // What a length rules out is loaded all the same and dropped afterwards: a run waits
+    // for memory once.
     int32_t seen[H];
-    if (counted) {
-        n = min(p.r.history_lens[row], (int)p.r.history_max);
-        prompt = p.r.prompt_lens ? p.r.prompt_lens[row] : 0;
 #pragma unroll
-        for (int j = 0; j < H; ++j) seen[j] = j * kThreads + tid < n ? __ldg(h + j * kThreads + tid) : -1;
-    }
+    for (int j = 0; j < H; ++j) seen[j] = j * kThreads + tid < room ? __ldg(h + j * kThreads + tid) : -1;
+    const int n = counted ? min(p.r.history_lens[row], room) : 0;
+    const int prompt = counted && p.r.prompt_lens ? p.r.prompt_lens[row] : 0;
+    const bool use_rep = counted && p.r.repetition, use_made = counted && (p.r.frequency || p.r.presence);
+    const float rep = use_rep ? p.r.repetition[row] : 1.f;
+    const float freq = use_made && p.r.frequency ? p.r.frequency[row] : 0.f;
+    const float pres = use_made && p.r.presence ? p.r.presence[row] : 0.f;
+    const bool adds = biased && warp == kWarps - 1;  // one warp, so that biases of one token add up in list order
+    const int32_t* bias_ids = biased ? p.r.bias_ids + row * p.r.bias_stride : nullptr;
+    const float* bias_values = biased ? p.r.bias_values + row * p.r.bias_stride : nullptr;
+    int next_id = adds && lane < count ? bias_ids[lane] : -1;
+    float next_value = adds && lane < count ? bias_values[lane] : 0.f;
+    const uint32_t* allowed = p.r.allowed ? p.r.allowed + row * p.r.allowed_stride : nullptr;
+
+    const float nan = __uint_as_float(0x7fc00000u);
     float v[G][4];
+    uint32_t word[G], over[G];  // the mask word of a group's first token, and the next one where the group runs into it
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-        const int64_t i = c0 + (j * kThreads + tid) * 4;
+        const int i = c0 + (j * kThreads + tid) * 4;
+        word[j] = over[j] = 0xffffffffu;
         if (i >= 0 && i + 4 <= p.vocab) {
             const float4 q = __ldcs(reinterpret_cast<const float4*>(x + i));
             v[j][0] = q.x; v[j][1] = q.y; v[j][2] = q.z; v[j][3] = q.w;
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][e] = i + e >= 0 && i + e < p.vocab ? x[i + e] : 0.f;
+            for (int e = 0; e < 4; ++e) v[j][e] = i + e >= 0 && i + e < p.vocab ? x[i + e] : nan;
+        }
+        if (allowed && i < p.vocab) {
+            if (i >= 0) word[j] = __ldg(allowed + (i >> 5));
+            if ((i & 31) > 28 && (i | 31) + 1 < p.vocab) over[j] = __ldg(allowed + (i >> 5) + 1);
         }
     }
 
@@ -88,60 +109,47 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
         for (int b = 0; b < n; b += H * kThreads) {
 #pragma unroll
             for (int j = 0; j < H; ++j) {
-                const int i = b + j * kThreads + tid, t = seen[j];
-                const int64_t at = t - c0;
-                if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
-                if (t >= 0 && t < p.vocab && at >= 0 && at < kChunk) {
-                    if (i < prompt) atomicOr(table + at, kPrompt);
-                    else atomicAdd(table + at, 1u);
-                }
-                const int next = i + H * kThreads;
+                if (b + j * kThreads >= n) break;
+                const int i = b + j * kThreads + tid, t = seen[j], next = i + H * kThreads;
                 seen[j] = next < n ? __ldg(h + next) : -1;
+                const uint32_t at = (uint32_t)t - (uint32_t)lo;
+                if (at < len && i < n) {
+                    if (i < prompt) atomicOr(table + skip + at, kPrompt);
+                    else atomicAdd(table + skip + at, 1u);
+                }
+                if (blockIdx.x == 0 && t >= p.vocab && i < n) atomicAdd(p.err, 1u);
             }
         }
-        if (biased && warp == kWarps - 1) {  // one warp, so that biases of one token add up in list order
-            const int32_t* ids = p.r.bias_ids + row * p.r.bias_stride;
-            const float* values = p.r.bias_values + row * p.r.bias_stride;
-            const int count = (int)p.r.bias_count;
-            int next = lane < count ? ids[lane] : -1;
-            for (int b = 0; b < count; b += 32) {
-                const int t = next;
-                next = b + 32 + lane < count ? ids[b + 32 + lane] : -1;
-                if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
-                const bool here = t >= 0 && t < p.vocab && t >= c0 && t < c0 + kChunk;
-                if (!__any_sync(0xffffffffu, here)) continue;
-                const float value = here ? values[b + lane] : 0.f;
-                const int at = here ? (int)(t - c0) : -1 - lane;
-                const uint32_t same = __match_any_sync(0xffffffffu, at);
-                if (here && (same & ((1u << lane) - 1)) == 0) {  // the first of its token in these 32
-                    const bool old = table[at] & kBiased;
-                    float sum = old ? __fadd_rn(bias[at], value) : value;
-                    for (uint32_t rest = same & ~(1u << lane); rest; rest &= rest - 1)
-                        sum = __fadd_rn(sum, values[b + __ffs(rest) - 1]);
-                    bias[at] = sum;
-                    if (!old) atomicOr(table + at, kBiased);
-                }
-                __syncwarp();
+        for (int b = 0; adds && b < count; b += 32) {
+            const int t = next_id;
+            const float value = next_value;
+            next_id = b + 32 + lane < count ? bias_ids[b + 32 + lane] : -1;
+            next_value = b + 32 + lane < count ? bias_values[b + 32 + lane] : 0.f;
+            if (t >= p.vocab && blockIdx.x == 0) atomicAdd(p.err, 1u);
+            const bool here = (uint32_t)t - (uint32_t)lo < len;
+            if (!__any_sync(0xffffffffu, here)) continue;
+            const int at = here ? t - c0 : -1 - lane;
+            const uint32_t same = __match_any_sync(0xffffffffu, at);
+            if (here && (same & ((1u << lane) - 1)) == 0) {  // the first of its token in these 32
+                const bool old = table[at] & kBiased;
+                float sum = old ? __fadd_rn(bias[at], value) : value;
+                for (uint32_t rest = same & ~(1u << lane); rest; rest &= rest - 1)
+                    sum = __fadd_rn(sum, bias_values[b + __ffs(rest) - 1]);
+                bias[at] = sum;
+                if (!old) atomicOr(table + at, kBiased);
             }
+            __syncwarp();
         }
         __syncthreads();
     }
 
-    const float rep = counted && p.r.repetition ? p.r.repetition[row] : 1.f;
-    const float freq = counted && p.r.frequency ? p.r.frequency[row] : 0.f;
-    const float pres = counted && p.r.presence ? p.r.presence[row] : 0.f;
-    const bool use_rep = counted && p.r.repetition, use_made = counted && (p.r.frequency || p.r.presence);
-    const uint32_t* allowed = p.r.allowed ? p.r.allowed + row * p.r.allowed_stride : nullptr;
     float* y = p.out ? p.out + row * p.out_stride : nullptr;
     const bool vec_out = y && ((reinterpret_cast<uintptr_t>(y) >> 2) & 3) == (uintptr_t)shift;
-    float top = -INFINITY;  // this thread's pick: the first of its largest numbers
-    int top_at = -1;
-    bool nan_first = false;
+    float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-        const int at = (j * kThreads + tid) * 4;
-        const int64_t i = c0 + at;
-        if (i + 4 <= 0 || i >= p.vocab) continue;
+        const int at = (j * kThreads + tid) * 4, i = c0 + at;
+        const bool edge = i < 0 || i + 4 > p.vocab;
         if (counted || biased) {
             uint32_t w[4];
             *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(table + at);
@@ -157,24 +165,14 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
                 }
             }
         }
-        if (allowed) {  // the 4 bits from token i on, which may lie in two words
-            const int64_t f = i < 0 ? 0 : i, g = i + 3 < p.vocab ? i + 3 : p.vocab - 1;
-            const uint32_t lo = allowed[f >> 5], hi = allowed[g >> 5];
-            const uint32_t bits = i < 0 ? lo << (int)-i : __funnelshift_r(lo, hi, (uint32_t)i & 31);
+        if (allowed) {
+            const uint32_t bits = __funnelshift_r(word[j], over[j], i & 31);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (!((bits >> e) & 1)) v[j][e] = -INFINITY;
+                if (!(bits & (1u << e)) && !(edge && (i + e < 0 || i + e >= p.vocab))) v[j][e] = -INFINITY;
         }
-        if (p.ids) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (i + e < 0 || i + e >= p.vocab) continue;
-                const float l = v[j][e];
-                if (l > top || (top_at < 0 && l == top)) top = l, top_at = (int)(i + e);
-                if (i + e == 0) nan_first = isnan(l);
-            }
-        }
-        if (vec_out && i >= 0 && i + 4 <= p.vocab) {
+        top = fmaxf(top, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+        if (vec_out && !edge) {
             *reinterpret_cast<float4*>(y + i) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
         } else if (y) {
 #pragma unroll
@@ -183,17 +181,31 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
         }
     }
     if (!p.ids) return;
-    // 0: no number here; a NaN at token 0 is the pick, and the largest key says so
-    unsigned long long best = nan_first ? ~0ull : top_at < 0 ? 0ull : greedy_key(top, (uint32_t)top_at);
+    // ---- the run's largest number, then the first token that has it
+    const float mine = top;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
-        best = k > best ? k : best;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) warp_top[warp] = top;
+    if (tid == 0) top_at = 0xffffffffu;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_top[w]);
+    if (mine == top) {
+        uint32_t at = 0xffffffffu;  // stays where the thread has no number at all
+#pragma unroll
+        for (int j = G - 1; j >= 0; --j)
+#pragma unroll
+            for (int e = 3; e >= 0; --e)
+                if (v[j][e] == top) at = (uint32_t)((j * kThreads + tid) * 4 + e);
+        atomicMin(&top_at, at);
     }
-    if (lane == 0) warp_best[warp] = best;
+    // a NaN at token 0 is the pick of its row, and the largest key says so
+    const bool nan_first = blockIdx.x == 0 && tid == 0 && isnan(shift == 0 ? v[0][0] : shift == 1 ? v[0][1] : shift == 2 ? v[0][2] : v[0][3]);
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kWarps; ++w) best = warp_best[w] > best ? warp_best[w] : best;
+        const unsigned long long best = nan_first                 ? ~0ull
+                                        : top_at == 0xffffffffu ? 0ull  // no number here
+                                                                  : greedy_key(top, (uint32_t)(c0 + (int)top_at));
         if (best) atomicMax(p.slots + row, best);
         __threadfence();
         if (atomicAdd(p.counters + row, 1u) == gridDim.x - 1) {
@@ -208,8 +220,10 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const RuleArgs p)
 template <int PER>
 cudaError_t launch_per(const RuleArgs& a, int64_t rows, bool pdl, cudaStream_t s) {
     constexpr int64_t chunk = kThreads * PER;
+    static_assert(chunk * 8 <= 48 * 1024, "no opt-in for more shared memory");
     const dim3 grid((unsigned)((a.vocab + 3 + chunk - 1) / chunk), (unsigned)rows);
-    return launch_kernel(logit_rules_kernel<PER>, grid, kThreads, 0, pdl, s, a);
+    const size_t smem = (size_t)(chunk * 4) * (a.r.bias_ids ? 2 : a.r.history ? 1 : 0);  // the table, and the biases
+    return launch_kernel(logit_rules_kernel<PER>, grid, kThreads, smem, pdl, s, a);
 }
 
 }  // namespace
@@ -219,11 +233,13 @@ cudaError_t launch_logit_rules(const float* logits, int64_t in_stride, int64_t r
                                unsigned long long* slots, unsigned int* counters, unsigned int* err, int sms, bool pdl,
                                cudaStream_t s) {
     const RuleArgs a{logits, in_stride, (int)vocab, rules, out, out_stride, ids, slots, counters, err};
-    (void)sms;
-    switch (getenv("PER") ? atoi(getenv("PER")) : 16) {
-        case 4: return launch_per<4>(a, rows, pdl, s);
-        case 8: return launch_per<8>(a, rows, pdl, s);
-    }
+    // Few logits: short runs, so that every SM has some.  Many: long ones, whose fixed
+    // work (tables, history, pick) is shared by more logits.  Measured at 128256 logits and 600
+    // tokens of history, 4 / 8 / 16 a thread: 1 row 4.0 / 4.8 / 5.4 us, 4 rows 5.0 / 5.0 / 5.6,
+    // 8 rows 6.8 / 5.7 / 6.0, 32 rows 16.7 / 12.6 / 11.1.
+    auto ctas = [&](int per) { return rows * ((vocab + kThreads * per - 1) / (kThreads * per)); };
+    if (2 * ctas(4) <= 5 * sms) return launch_per<4>(a, rows, pdl, s);
+    if (2 * ctas(8) <= 7 * sms) return launch_per<8>(a, rows, pdl, s);
     return launch_per<16>(a, rows, pdl, s);
 }
 

@@ -12,13 +12,18 @@ quantized in HBM and run through the fused dequant-GEMV (`linear_d`), with
 * gate and up interleaved into one pair for the fused gated MLP
   (`mlp_gated_silu`: silu(gate) * up, then down);
 * the output head as a GEMV over the vocabulary followed by greedy argmax on
-  the device (`greedy_sample`), the embedding as a Q8_0 row gather.
+  the device (`greedy_sample`), with penalties, biases and a grammar mask where a
+  request has them, the embedding as a Q8_0 row gather;
+* between qkv and o, head norms, rotation and the paged cache write in one launch
+  (`qk_norm_rope`) and the attention over the cache in another (`paged_attention`),
+  set up from the file's metadata at their first use.
 
 Tensor names follow the GGUF convention for these models (token_embd.weight,
 blk.N.attn_{q,k,v}.{weight,bias}, blk.N.attn_output.weight,
 blk.N.ffn_{gate,up,down}.weight, output.weight; a missing head is tied to the
-embedding table).  Attention, norms and rotary embeddings are not part of this
-path; the caller runs them between the projections.
+embedding table; blk.N.attn_{q,k}_norm.weight and rope_freqs.weight where a model
+has them).  The norms of the residual stream are not part of this path; the caller
+runs them between the calls.
 """
 from __future__ import annotations
 
@@ -123,6 +128,85 @@ def plan(m: Manifest, n_layers: int | None = None) -> ModelPlan:
     return out
 
 
+@dataclass
+class AttentionPlan:
+    """What the metadata says about the attention of every layer."""
+    n_heads: int
+    n_kv_heads: int
+    head_dim: int
+    scale: float
+    rot_dim: int
+    rope_base: float
+    rope_scale: float            # every frequency is divided by it (linear position scaling)
+    rope_factors: str | None     # tensor of per-pair frequency divisors
+    interleaved: bool            # pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2)
+    eps: float
+    q_norm: list[str | None] = field(default_factory=list)
+    k_norm: list[str | None] = field(default_factory=list)
+
+
+# How an architecture's files pair the elements that a rotation turns together.
+ROPE_INTERLEAVED = {"llama": True, "qwen2": False, "qwen3": False}
+
+
+def attention_plan(m: Manifest, p: ModelPlan) -> AttentionPlan:
+    """Head layout, rotation and head norms of a planned decoder (host only, reads no payload)."""
+    def need(key):
+        if key not in m.metadata:
+            raise InvalidRequestError("metadata", f"GGUF file {m.path} has no `{key}`")
+        return m.metadata[key]
+
+    arch = need("general.architecture")
+    if arch not in ROPE_INTERLEAVED:
+        raise UnsupportedError("attention architecture", str(arch), sorted(ROPE_INTERLEAVED))
+    heads = need(f"{arch}.attention.head_count")
+    kv = m.metadata.get(f"{arch}.attention.head_count_kv", heads)
+    if not isinstance(heads, int) or not isinstance(kv, int):
+        raise UnsupportedError("heads per layer", f"{heads} / {kv}", ["one head count for all layers"])
+    if heads <= 0 or kv <= 0 or heads % kv:
+        raise InvalidRequestError("metadata", f"{heads} heads are not a multiple of {kv} key/value heads")
+    dim = m.metadata.get(f"{arch}.attention.key_length", p.hidden // heads)
+    if m.metadata.get(f"{arch}.attention.value_length", dim) != dim:
+        raise UnsupportedError("attention value_length", str(m.metadata[f"{arch}.attention.value_length"]), [f"key_length={dim}"])
+    for feature in ("attention.sliding_window", "attn_logit_softcapping"):
+        if m.metadata.get(f"{arch}.{feature}"):
+            raise UnsupportedError(feature, str(m.metadata[f"{arch}.{feature}"]), ["none"])
+    scaling = m.metadata.get(f"{arch}.rope.scaling.type", "none")
+    if scaling not in ("none", "linear"):
+        raise UnsupportedError("rope scaling", str(scaling), ["none", "linear"])
+    for lp in p.layers:
+        if lp.qkv_rows != [heads * dim, kv * dim, kv * dim]:
+            raise InvalidRequestError("tensor", f"layer {lp.index}: q/k/v rows {lp.qkv_rows} are not {heads} + 2 * {kv} heads of {dim}")
+    names = {t.name for t in m.tensors}
+
+    def norms(s):
+        out = []
+        for lp in p.layers:
+            name = f"blk.{lp.index}.attn_{s}_norm.weight"
+            out.append(name if name in names else None)
+            if name in names:
+                t = m.tensor(name)
+                if t.tensor_type != F32:
+                    raise UnsupportedError("norm type", f"{name}: {t.tensor_type}", ["F32(0)"])
+                if t.shape != [dim]:
+                    raise InvalidRequestError("tensor", f"`{name}` has shape {t.shape}, expected [{dim}]")
+        return out
+
+    rot = m.metadata.get(f"{arch}.rope.dimension_count", dim)
+    factors = "rope_freqs.weight" if "rope_freqs.weight" in names else None
+    if factors and (m.tensor(factors).tensor_type != F32 or m.tensor(factors).shape != [rot // 2]):
+        raise InvalidRequestError("tensor", f"`{factors}` is not {rot // 2} F32 values")
+    return AttentionPlan(
+        heads, kv, dim, float(m.metadata.get(f"{arch}.attention.scale", 0.0)) or dim ** -0.5, rot,
+        float(m.metadata.get(f"{arch}.rope.freq_base", 10000.0)),
+        float(m.metadata.get(f"{arch}.rope.scaling.factor", 1.0)) if scaling == "linear" else 1.0, factors,
+        ROPE_INTERLEAVED[arch], float(need(f"{arch}.attention.layer_norm_rms_epsilon")), norms("q"), norms("k"))
+
+
+def _f32(m: Manifest, name: str) -> np.ndarray:
+    return np.frombuffer(bytes(read_payload(m, name)), dtype=np.float32)
+
+
 def fused_qkv_payload(m: Manifest, lp: LayerPlan) -> tuple[int, np.ndarray, int]:
     """(type, concatenated GGUF rows of q, k, v, total rows)."""
     ts = [m.tensor(n) for n in lp.qkv]
@@ -133,10 +217,11 @@ def fused_qkv_payload(m: Manifest, lp: LayerPlan) -> tuple[int, np.ndarray, int]
 class QuantizedDecoderLinears:
     """Every linear layer of the decoder resident in HBM, quantized.
 
-    Per layer: `qkv(x, rows, out)` -> [rows, q+k+v] (bias added), `o(...)`,
-    `mlp(x, rows, act, out)` (silu(gate)*up then down); plus `embed(ids, out)`
-    and `head_argmax(h, rows)` -> next token ids on the device.  x / out are
-    contiguous f32 torch tensors on the backend's device.
+    Per layer: `qkv(x, rows, out)` -> [rows, q+k+v] (bias added),
+    `attention(i, qkv, cache, ...)` -> [rows, q], `o(...)`, `mlp(x, rows, act, out)`
+    (silu(gate)*up then down); plus `kv_caches(...)`, `embed(ids, out)` and
+    `head_argmax(h, rows)` -> next token ids on the device.  x / out are contiguous
+    f32 torch tensors on the backend's device.
     """
 
     def __init__(self, backend, manifest: Manifest, n_layers: int | None = None):
@@ -145,6 +230,8 @@ class QuantizedDecoderLinears:
         from .gguf import upload_quant_tensor
         self.backend = backend
         self.plan = plan(manifest, n_layers)
+        self._manifest = manifest
+        self._attention = None
         dev = backend.torch_device
         self.layers = []
         for lp in self.plan.layers:
@@ -174,6 +261,41 @@ class QuantizedDecoderLinears:
         L = self.layers[i]
         self.backend.linear_dev(L["qkv"], x, rows, out, bias=L["qkv_bias"])
 
+    def _attention_parts(self):
+        """(plan, rotation table, q norms, k norms), from the file at the first use."""
+        if self._attention is None:
+            import torch
+            m, a = self._manifest, attention_plan(self._manifest, self.plan)
+            factors = None
+            if a.rope_factors or a.rope_scale != 1.0:
+                factors = (_f32(m, a.rope_factors) if a.rope_factors else np.ones(a.rot_dim // 2, np.float32)) * a.rope_scale
+            rope = self.backend.rope_table(a.rot_dim, a.rope_base, factors=factors, interleaved=a.interleaved)
+            dev = self.backend.torch_device
+            qn, kn = ([None if n is None else torch.from_numpy(_f32(m, n).copy()).to(dev) for n in names]
+                      for names in (a.q_norm, a.k_norm))
+            self._attention = (a, rope, qn, kn)
+        return self._attention
+
+    def kv_caches(self, n_pages: int, page_size: int = 16, dtype=None) -> list:
+        """A paged key/value cache for every layer (bf16 unless told otherwise)."""
+        import torch
+        a = self._attention_parts()[0]
+        return [self.backend.kv_cache(n_pages, page_size, a.n_kv_heads, a.head_dim, dtype or torch.bfloat16)
+                for _ in self.layers]
+
+    def attention(self, i: int, qkv, cache, positions, block_table, seqs=None, q=None, out=None):
+        """Layer i between `qkv` and `o`: norms, rotation, cache write, attention -> f32 [rows, n_heads * head_dim].
+
+        Row r of qkv is token positions[r] of sequence seqs[r] (r when None), as for
+        qk_norm_rope; several rows of one sequence (a prompt) see each other causally.
+        q, out: optional [rows, n_heads, head_dim] buffers.
+        """
+        a, rope, qn, kn = self._attention_parts()
+        q = self.backend.qk_norm_rope(qkv, cache, positions, block_table, rope, q_norm=qn[i], k_norm=kn[i], eps=a.eps,
+                                      seqs=seqs, out=q)
+        o = self.backend.paged_attention(q, cache, positions, block_table, scale=a.scale, seqs=seqs, out=out)
+        return o.view(o.shape[0], -1)
+
     def o(self, i: int, x, rows: int, out) -> None:
         self.backend.linear_dev(self.layers[i]["o"], x, rows, out)
 
@@ -186,9 +308,10 @@ class QuantizedDecoderLinears:
     def embed(self, ids, out=None):
         return self.backend.embed_rows(self.embed_table, ids, out)
 
-    def head_argmax(self, h, rows: int, logits=None, ids=None):
+    def head_argmax(self, h, rows: int, logits=None, ids=None, rules=None):
+        """Greedy pick of the head's logits (under `rules`, see LogitRules, when given): (ids, the head's logits)."""
         import torch
         if logits is None:
             logits = torch.empty(rows, self.plan.vocab, device=self.backend.torch_device)
         self.backend.linear_dev(self.head_w, h, rows, logits)
-        return self.backend.greedy_sample(logits, out=ids), logits
+        return self.backend.greedy_sample(logits, out=ids, rules=rules), logits

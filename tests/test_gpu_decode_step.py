@@ -1,0 +1,150 @@
+"""GPU: a decoder's steps through QuantizedDecoderLinears: prompt rows, then one token at a
+time, eagerly and as a captured graph, with the logit rules at the end."""
+import numpy as np
+import pytest
+import torch
+
+from tests.decode_cases import attention_reference, rope_reference
+from tests.test_attention_plan_cpu import META
+
+pytestmark = pytest.mark.gpu
+
+HEADS, KV_HEADS, DIM, PAGE = 4, 1, 64, 16
+PROMPTS = [[5, 17, 900, 3, 3, 41, 7, 7, 7, 12, 99, 250, 251, 252, 253, 254, 255, 256, 1], [8, 1, 1]]
+
+
+def f32_tensor(name, values):
+    return name, [len(values)], 0, np.asarray(values, np.float32).tobytes()
+
+
+@pytest.fixture(scope="module", params=["qwen3", "llama"])
+def model(request, backend, tmp_path_factory):
+    from ocelotl_b200 import gguf
+    from ocelotl_b200.model import QuantizedDecoderLinears
+    from tests.gguf_writer import write_gguf
+    from tests.model_files import decoder_tensors
+    rng = np.random.default_rng(5)
+    t = decoder_tensors(n_layers=2)
+    if request.param == "qwen3":
+        t += [f32_tensor(f"blk.{i}.attn_{s}_norm.weight", 1 + 0.2 * rng.standard_normal(DIM)) for i in range(2) for s in "qk"]
+    else:
+        t += [f32_tensor("rope_freqs.weight", 1 + rng.random(DIM // 2))]
+    f = tmp_path_factory.mktemp("d") / "decoder.gguf"
+    write_gguf(f, t)
+    m = gguf.inspect(f)
+    m.metadata.update({k.replace("qwen3", request.param): v for k, v in META.items()})
+    m.metadata["general.architecture"] = request.param
+    return QuantizedDecoderLinears(backend, m)
+
+
+class Run:
+    """The caller's side: caches, tables, histories, residual norms, and buffers that stay in place."""
+
+    def __init__(self, model, dtype):
+        self.m, b = model, model.backend
+        self.caches = model.kv_caches(12, PAGE, dtype)
+        self.table = torch.tensor([[7, 2, 9], [4, 0, 11]], dtype=torch.int32, device="cuda")
+        self.history = torch.full((2, 64), -1, dtype=torch.int32, device="cuda")
+        self.lens = torch.tensor([len(p) for p in PROMPTS], dtype=torch.int32, device="cuda")
+        for r, p in enumerate(PROMPTS):
+            self.history[r, :len(p)] = torch.tensor(p, dtype=torch.int32)
+        mask = torch.full((2, (model.plan.vocab + 31) // 32), -1, dtype=torch.int32, device="cuda")
+        mask[1] &= 0x55555555  # only even tokens for the second
+        self.rules = b.logit_rules(
+            history=self.history, history_lens=self.lens, prompt_lens=self.lens.clone(),
+            repetition=torch.tensor([1.3, 1.0], device="cuda"), frequency=torch.tensor([0.2, 0.5], device="cuda"),
+            presence=torch.tensor([0.1, 0.0], device="cuda"), allowed=mask,
+            bias_ids=torch.tensor([[3, -1], [10, 12]], dtype=torch.int32, device="cuda"),
+            bias_values=torch.tensor([[2.0, 0.0], [-50.0, 1.0]], device="cuda"))
+        self.positions = self.lens - 1
+        self.ids = torch.tensor([p[-1] for p in PROMPTS], dtype=torch.int32, device="cuda")
+        self.last_logits = self.seen = None
+
+    def norm(self, h):
+        return (h * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-5)).contiguous()
+
+    def layers(self, h, rows, positions, seqs, watch=None):
+        m, p = self.m, self.m.plan
+        for i in range(len(p.layers)):
+            qkv = torch.empty(rows, (HEADS + 2 * KV_HEADS) * DIM, device="cuda")
+            m.qkv(i, self.norm(h), rows, qkv)
+            a = m.attention(i, qkv, self.caches[i], positions, self.table, seqs=seqs)
+            if watch:
+                watch(i, qkv, a)
+            o, act, mlp = (torch.empty(rows, n, device="cuda") for n in (p.hidden, p.intermediate, p.hidden))
+            m.o(i, a, rows, o)
+            h = h + o
+            m.mlp(i, self.norm(h), rows, act, mlp)
+            h = h + mlp
+        return h
+
+    def prefill(self, watch=None):
+        """Every prompt token but the last of each sequence, in one pass; two padding rows at the end."""
+        rows = [(t, s, i) for s, p in enumerate(PROMPTS) for i, t in enumerate(p[:-1])] + [(0, 0, -1)] * 2
+        ids, seqs, pos = (torch.tensor([r[k] for r in rows], dtype=torch.int32, device="cuda") for k in range(3))
+        self.layers(self.m.embed(ids), len(rows), pos, seqs, (lambda i, qkv, a: watch(i, qkv, a, pos, seqs)) if watch else None)
+
+    def step(self, watch=None):
+        pos = self.positions
+        h = self.layers(self.m.embed(self.ids), 2, pos, None, (lambda i, qkv, a: watch(i, qkv, a, pos, None)) if watch else None)
+        ids, self.last_logits = self.m.head_argmax(self.norm(h), 2, rules=self.rules)
+        self.seen = self.history.clone(), self.lens.clone()
+        self.ids.copy_(ids)
+        self.history.scatter_(1, self.lens.long()[:, None], ids[:, None])
+        self.lens.add_(1)
+        self.positions.add_(1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_and_steps(backend, oracle, model, dtype):
+    from tests.test_gpu_logits import reference
+    backend.take_device_errors()
+    run = Run(model, dtype)
+    plan, _, qn, kn = model._attention_parts()
+    factors = None if plan.rope_factors is None else np.frombuffer(
+        __import__("ocelotl_b200.gguf", fromlist=["x"]).read_payload(model._manifest, plan.rope_factors).tobytes(), np.float32)
+
+    def watch(i, qkv, a, pos, seqs):
+        torch.cuda.synchronize()
+        (q, _), _, _ = rope_reference(qkv, HEADS, KV_HEADS, DIM, pos.clamp(min=0), DIM, 1e6, plan.interleaved, qn[i], kn[i], plan.eps,
+                                      factors)
+        want, bound = attention_reference(q, run.caches[i].k, run.caches[i].v, pos, run.table, plan.scale, seqs)
+        # the kernel's own q is off by up to 16 units of 2^-24 of its pairs: as much again in each score
+        k_max = run.caches[i].k.double().abs().max().item()
+        more = 2 * 32 * 2.0 ** -24 * q.abs().sum(-1).amax().item() * k_max * plan.scale * run.caches[i].v.double().abs().max().item()
+        assert ((a.view(want.shape).double() - want).abs() <= bound + more).all()
+
+    run.prefill(watch)
+    picks = []
+    for _ in range(5):
+        run.step(watch)
+        torch.cuda.synchronize()
+        hist, lens = (t.cpu().numpy() for t in run.seen)
+        parts = {n: t.cpu().numpy() for n, t in run.rules.parts.items()}
+        ruled = reference(run.last_logits.cpu().numpy(), **{**parts, "history": hist, "history_lens": lens})
+        assert run.ids.tolist() == [oracle.greedy_sample_fast(r) for r in ruled]
+        assert run.ids[1] % 2 == 0
+        picks.append(run.ids.tolist())
+    assert backend.take_device_errors() == (0, 0)
+
+    # the same as a captured step, replayed: the same tokens
+    other = Run(model, dtype)
+    other.prefill()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            backend.use_current_stream()
+            other.step()
+    finally:
+        backend.set_stream(None)
+    got = []
+    for _ in range(5):
+        graph.replay()
+        torch.cuda.synchronize()
+        got.append(other.ids.tolist())
+    assert got == picks
+    for a, b in zip(run.caches, other.caches):
+        assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+    assert backend.take_device_errors() == (0, 0)
