@@ -71,45 +71,57 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p
     grid_wait();
     const int64_t row = blockIdx.x / p.groups;
     const int group = blockIdx.x % p.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int half = p.rope.rot / 2, i0 = lane * V;  // i0: the lane's first pair
+    const bool active = i0 < D / 2;                  // other lanes only take part in the reductions
+    const int qk = p.n_heads + p.n_kv, heads = qk + p.n_kv, step = p.groups * kWarps;
+    // first elements of the lane's two runs in a q or k head, and in a v head (as they lie)
+    const bool turned = i0 < half, halves = turned && !p.rope.interleaved;
+    const int a_qk = halves ? i0 : 2 * i0, b_qk = halves ? i0 + half : 2 * i0 + V;
+    const float* src = p.qkv + row * p.qkv_stride;
+    float x[V] = {}, y[V] = {};
+    auto load = [&](int h) {
+        if (!active || h >= heads) return;
+        load_vec<V>(x, src + (int64_t)h * D + (h < qk ? a_qk : 2 * i0));
+        load_vec<V>(y, src + (int64_t)h * D + (h < qk ? b_qk : 2 * i0 + V));
+    };
+    int h = group * kWarps + warp;
+    load(h);  // on its way while the row's place and angles are worked out
+
     const int pos = p.at.positions[row];
-    const int half = p.rope.rot / 2;
     if ((int)threadIdx.x < half) {
         const unsigned long long phase = (unsigned long long)(long long)pos * p.rope.steps[threadIdx.x];
         float s, c;
         sincospif((float)(long long)phase * 0x1p-63f, &s, &c);  // phase as a signed fraction of a revolution
         turn[threadIdx.x] = make_float2(c, s);
     }
-    // the row's page: -1 when nothing is to be cached
-    int64_t slot = -1;
+    int64_t slot = -1;  // the row's place in the cache: -1 when nothing is to be cached
     if (pos >= 0) {
         const int64_t seq = sequence_of(p.at, row);
         int page = -1, in_page = 0;
         const bool ok = seq >= 0 && place_of(p.at.table + seq * p.at.table_stride, p.at.max_pages, p.kv.n_pages, p.page_size, pos, page, in_page);
-        slot = page * p.kv.page_stride + in_page * p.kv.token_stride;
-        if (!ok) {
-            slot = -1;
-            if (threadIdx.x == 0 && group == 0) atomicAdd(p.err, 1u);
-        }
+        if (ok) slot = page * p.kv.page_stride + in_page * p.kv.token_stride;
+        else if (threadIdx.x == 0 && group == 0) atomicAdd(p.err, 1u);
     }
     __syncthreads();
-    const int i0 = lane * V;  // first pair
-    const int heads = p.n_heads + 2 * p.n_kv;
-    const bool active = i0 < D / 2;  // other lanes only take part in the reductions
-    for (int h = group * kWarps + warp; h < heads; h += p.groups * kWarps) {
-        const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.n_kv;
-        const bool turned = !is_v && i0 < half, halves = turned && !p.rope.interleaved;
-        const int a = halves ? i0 : 2 * i0, b = halves ? i0 + half : 2 * i0 + V;
-        float x[V] = {}, y[V] = {};
-        if (active && pos >= 0) {
-            const float* src = p.qkv + row * p.qkv_stride + (int64_t)h * D;
-            load_vec<V>(x, src + a);
-            load_vec<V>(y, src + b);
+    float2 t[V];  // the lane's turns, the same for every head
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[e] = turned ? turn[i0 + e] : make_float2(1.f, 0.f);
+
+    for (; h < heads; h += step) {
+        const bool is_q = h < p.n_heads, is_v = h >= qk;
+        const int a = is_v ? 2 * i0 : a_qk, b = is_v ? 2 * i0 + V : b_qk;
+        float u[V], v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            u[e] = pos >= 0 ? x[e] : 0.f;  // a padding row is zeros
+            v[e] = pos >= 0 ? y[e] : 0.f;
         }
+        load(h + step);
         const float* w = is_v || pos < 0 ? nullptr : is_q ? p.q_norm : p.k_norm;
         if (w) {
             float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum += x[e] * x[e] + y[e] * y[e];
+            for (int e = 0; e < V; ++e) sum += u[e] * u[e] + v[e] * v[e];
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
@@ -119,43 +131,42 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const RopeArgs p
                 load_vec<V>(wb, w + b);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    x[e] *= inv * wa[e];
-                    y[e] *= inv * wb[e];
+                    u[e] *= inv * wa[e];
+                    v[e] *= inv * wb[e];
                 }
             }
         }
-        if (turned && !p.rope.interleaved) {
+        if (turned && !is_v) {
+            if (halves) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 t = turn[i0 + e];
-                const float u = x[e], v = y[e];
-                x[e] = u * t.x - v * t.y;
-                y[e] = v * t.x + u * t.y;
+                for (int e = 0; e < V; ++e) {
+                    const float f = u[e], g = v[e];
+                    u[e] = f * t[e].x - g * t[e].y;
+                    v[e] = g * t[e].x + f * t[e].y;
+                }
+            } else {
+                float z[2 * V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[e] = u[e], z[V + e] = v[e];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float f = z[2 * e], g = z[2 * e + 1];
+                    z[2 * e] = f * t[e].x - g * t[e].y;
+                    z[2 * e + 1] = g * t[e].x + f * t[e].y;
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) u[e] = z[e], v[e] = z[V + e];
             }
-        } else if (turned) {
-            float z[2 * V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) z[e] = x[e], z[V + e] = y[e];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 t = turn[i0 + e];
-                const float u = z[2 * e], v = z[2 * e + 1];
-                z[2 * e] = u * t.x - v * t.y;
-                z[2 * e + 1] = v * t.x + u * t.y;
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = z[e], y[e] = z[V + e];
         }
         if (!active) continue;
         if (is_q) {
             float* dst = p.q_out + (row * p.n_heads + h) * D;
-            store_vec<V>(dst + a, x);
-            store_vec<V>(dst + b, y);
+            store_vec<V>(dst + a, u);
+            store_vec<V>(dst + b, v);
         } else if (slot >= 0) {
-            T* dst = static_cast<T*>(is_v ? p.kv.v : p.kv.k) + slot +
-                     (int64_t)(h - p.n_heads - (is_v ? p.n_kv : 0)) * p.kv.head_stride;
-            store_vec<V>(dst + a, x);
-            store_vec<V>(dst + b, y);
+            T* dst = static_cast<T*>(is_v ? p.kv.v : p.kv.k) + slot + (int64_t)(h - (is_v ? qk : p.n_heads)) * p.kv.head_stride;
+            store_vec<V>(dst + a, u);
+            store_vec<V>(dst + b, v);
         }
     }
 }

@@ -97,12 +97,13 @@ class Run:
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_prompt_and_steps(backend, oracle, model, dtype):
+    from ocelotl_b200.gguf import read_payload
     from tests.test_gpu_logits import reference
     backend.take_device_errors()
     run = Run(model, dtype)
     plan, _, qn, kn = model._attention_parts()
-    factors = None if plan.rope_factors is None else np.frombuffer(
-        __import__("ocelotl_b200.gguf", fromlist=["x"]).read_payload(model._manifest, plan.rope_factors).tobytes(), np.float32)
+    factors = None if plan.rope_factors is None else \
+        np.array(read_payload(model._manifest, plan.rope_factors)).view(np.float32).tolist()
 
     def watch(i, qkv, a, pos, seqs):
         torch.cuda.synchronize()
