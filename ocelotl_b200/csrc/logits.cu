@@ -42,6 +42,18 @@ struct RuleArgs {
     unsigned int* err;
 };
 
+// The key of one run joins its row's; the last run writes the id.
+__device__ __forceinline__ void pick_row(const RuleArgs& p, int64_t row, unsigned long long key) {
+    if (key) atomicMax(p.slots + row, key);
+    __threadfence();
+    if (atomicAdd(p.counters + row, 1u) == gridDim.x - 1) {
+        __threadfence();
+        const unsigned long long k = atomicExch(p.slots + row, 0ull);  // read and reset
+        p.ids[row] = k == 0 || k == ~0ull ? 0 : (int32_t)(0xFFFFFFFFu - (uint32_t)(k & 0xFFFFFFFFull));
+        p.counters[row] = 0;
+    }
+}
+
 // PER logits a thread, in groups of 4 that are 16-byte aligned in `logits`
 // whatever the row's own alignment: the run of CTA b starts at b * chunk - shift.
 // Logits of the run outside the row are NaN, which no rule changes and no pick takes.
@@ -50,8 +62,7 @@ __global__ void __launch_bounds__(kThreads, 5) logit_rules_kernel(const RuleArgs
     constexpr int kChunk = kThreads * PER, G = PER / 4, H = 4;
     extern __shared__ __align__(16) uint32_t table[];
     float* bias = reinterpret_cast<float*>(table + kChunk);  // only where the table says kBiased
-    __shared__ float warp_top[kWarps];
-    __shared__ uint32_t top_at;
+    __shared__ unsigned long long warp_best[kWarps];
     grid_wait();
     const int64_t row = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -169,7 +180,12 @@ __global__ void __launch_bounds__(kThreads, 5) logit_rules_kernel(const RuleArgs
             const uint32_t bits = __funnelshift_r(word[j], over[j], i & 31);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (!(bits & (1u << e)) && !(edge && (i + e < 0 || i + e >= p.vocab))) v[j][e] = -INFINITY;
+                if (!(bits & (1u << e))) v[j][e] = -INFINITY;
+        }
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < 0 || i + e >= p.vocab) v[j][e] = nan;
         }
         top = fmaxf(top, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
         if (vec_out && !edge) {
@@ -181,39 +197,27 @@ __global__ void __launch_bounds__(kThreads, 5) logit_rules_kernel(const RuleArgs
         }
     }
     if (!p.ids) return;
-    // ---- the run's largest number, then the first token that has it
-    const float mine = top;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) warp_top[warp] = top;
-    if (tid == 0) top_at = 0xffffffffu;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_top[w]);
-    if (mine == top) {
-        uint32_t at = 0xffffffffu;  // stays where the thread has no number at all
+    // ---- the warp's largest number and the first token that has it, then the run's
+    const uint32_t mine = (uint32_t)(greedy_key(top, 0) >> 32), most = __reduce_max_sync(0xffffffffu, mine);
+    uint32_t at = 0xffffffffu;  // stays where there is no number
+    if (mine == most) {
 #pragma unroll
         for (int j = G - 1; j >= 0; --j)
 #pragma unroll
             for (int e = 3; e >= 0; --e)
                 if (v[j][e] == top) at = (uint32_t)((j * kThreads + tid) * 4 + e);
-        atomicMin(&top_at, at);
     }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) warp_best[warp] = at == 0xffffffffu ? 0ull : (unsigned long long)most << 32 | (0xffffffffu - (uint32_t)(c0 + (int)at));
     // a NaN at token 0 is the pick of its row, and the largest key says so
-    const bool nan_first = blockIdx.x == 0 && tid == 0 && isnan(shift == 0 ? v[0][0] : shift == 1 ? v[0][1] : shift == 2 ? v[0][2] : v[0][3]);
+    const bool nan_first = blockIdx.x == 0 && tid == 0 &&
+                           isnan(shift == 0 ? v[0][0] : shift == 1 ? v[0][1] : shift == 2 ? v[0][2] : v[0][3]);
     __syncthreads();
     if (tid == 0) {
-        const unsigned long long best = nan_first                 ? ~0ull
-                                        : top_at == 0xffffffffu ? 0ull  // no number here
-                                                                  : greedy_key(top, (uint32_t)(c0 + (int)top_at));
-        if (best) atomicMax(p.slots + row, best);
-        __threadfence();
-        if (atomicAdd(p.counters + row, 1u) == gridDim.x - 1) {
-            __threadfence();
-            const unsigned long long k = atomicExch(p.slots + row, 0ull);  // read and reset
-            p.ids[row] = k == 0 || k == ~0ull ? 0 : (int32_t)(0xFFFFFFFFu - (uint32_t)(k & 0xFFFFFFFFull));
-            p.counters[row] = 0;
-        }
+        unsigned long long best = nan_first ? ~0ull : 0ull;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) best = warp_best[w] > best ? warp_best[w] : best;
+        pick_row(p, row, best);
     }
 }
 
