@@ -502,13 +502,13 @@ class CudaKernelBackend:
             raise _kernel_err(f"{op} cache must be a PagedKvCache on {dev}")
         check_tensor(positions, op, "positions", torch.int32, dev, 1)
         check_tensor(block_table, op, "block_table", torch.int32, dev, 2)
-        if len(positions) != rows:
-            raise _kernel_err(f"{op} positions.len()={len(positions)} does not match rows={rows}")
+        if positions.shape[0] != rows:
+            raise _kernel_err(f"{op} positions.len()={positions.shape[0]} does not match rows={rows}")
         n_seqs, max_pages = block_table.shape
         if seqs is not None:
             check_tensor(seqs, op, "seqs", torch.int32, dev, 1)
-            if len(seqs) != rows:
-                raise _kernel_err(f"{op} seqs.len()={len(seqs)} does not match rows={rows}")
+            if seqs.shape[0] != rows:
+                raise _kernel_err(f"{op} seqs.len()={seqs.shape[0]} does not match rows={rows}")
         return _lib.KV_ROWS.pack(positions.data_ptr(), 0 if seqs is None else seqs.data_ptr(), block_table.data_ptr(), n_seqs,
                                  max_pages, block_table.stride(0) if n_seqs > 1 else max_pages)
 
@@ -534,8 +534,8 @@ class CudaKernelBackend:
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
             if w is not None:
                 check_tensor(w, "qk_norm_rope", name, torch.float32, self.torch_device, 1)
-                if len(w) != dim:
-                    raise _kernel_err(f"qk_norm_rope {name}.len()={len(w)} does not match head_dim={dim}")
+                if w.shape[0] != dim:
+                    raise _kernel_err(f"qk_norm_rope {name}.len()={w.shape[0]} does not match head_dim={dim}")
         out = self._out(out, qkv, "qk_norm_rope", rows, heads, dim)
         rc = self._lib.ocl_qk_norm_rope(
             self._ctx, qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, cache.ref, at,
@@ -582,8 +582,8 @@ class CudaKernelBackend:
                 raise _kernel_err(f"{op} out {list(out.shape)} does not match logits {list(logits.shape)}")
         if ids is not None:
             check_tensor(ids, op, "ids", torch.int32, self.torch_device, 1)
-            if len(ids) != rows:
-                raise _kernel_err(f"{op} ids.len()={len(ids)} does not match rows={rows}")
+            if ids.shape[0] != rows:
+                raise _kernel_err(f"{op} ids.len()={ids.shape[0]} does not match rows={rows}")
         rc = self._lib.ocl_logits_process(
             self._ctx, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, rules.ref,
             None if out is None else out.data_ptr(),

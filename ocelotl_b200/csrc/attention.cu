@@ -38,41 +38,50 @@ namespace ocl {
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kHeads = 8;   // query heads of one k/v head worked on together
 constexpr int kBoxTok = 16; // tokens of one tensor-map copy, and of one p.v MMA
 
-// Tokens a warp takes at a time, and the ring's stages of as many.  32 tokens halve the
-// work a token costs besides its MMAs (maximum, rescaling, waits, look-ups) and give a
-// warp twice the independent MMAs; at head_dim 256 three stages of 32 do not fit.
+// Tokens a warp takes at a time.  32 halve the work a token costs besides its MMAs
+// (maximum, rescaling, waits, look-ups) and give a warp twice the independent MMAs; at
+// head_dim 256 they would not leave three slots to each of 8 warps.
 constexpr int warp_tok(int d) { return d == 256 ? 16 : 32; }
-constexpr int tile_tok(int d) { return kWarps * warp_tok(d); }
-constexpr int stages(int d) { return d == 96 ? 4 : 3; }
+// Warps and ring.  Up to head_dim 128 four warps, each with a ring of slots that hold the
+// keys and the values of its tokens: 1.5 us a tile, about what HBM takes to bring it.  At
+// head_dim 256 a tile takes a warp twice as long and eight are wanted; their rings have
+// separate slots for keys and values, so that three of 8 KB keep copies under way
+// (6 rows of 900 to 6000 tokens, 4 k/v heads of 8: 25.6 us with four warps, 22.9 with
+// eight; at head_dim 128 both changes lose: 64 ragged rows 123 us, 143 and 129).
+constexpr bool split_slots(int d) { return d == 256; }
+constexpr int warps(int d) { return d == 256 ? 8 : 4; }
+constexpr int max_warps = 8;
+constexpr int slots(int d) { return d == 96 ? 4 : 3; }
 constexpr int ctas_per_sm(int d) { return d == 64 ? 2 : 1; }
 constexpr int max_ctas_per_sm = 2;
+constexpr int tile_tok(int d) { return warps(d) * warp_tok(d); }
 // 16 tokens of k or v are kept as parts of 64 elements (32 for head_dim 96): a part is
 // 16 rows of 128 (64) bytes, its 16-byte chunks exclusive-or'ed with the row as the
 // copy engine's 128-byte (64-byte) swizzle does.
 constexpr int part_elems(int d) { return d % 64 == 0 ? 64 : 32; }
 constexpr int part_bytes(int d) { return kBoxTok * part_elems(d) * 2; }
 constexpr int box_bytes(int d) { return kBoxTok * d * 2; }
-constexpr int half_bytes(int d) { return warp_tok(d) * d * 2; }  // k (or v) of a stage
-constexpr int merge_cols(int d) { return d < 128 ? d : 128; }
+constexpr int half_bytes(int d) { return warp_tok(d) * d * 2; }  // keys or values of a warp's tokens
+constexpr int slot_bytes(int d) { return (split_slots(d) ? 1 : 2) * half_bytes(d); }
+constexpr int merge_cols(int d) { return d == 256 ? 64 : d; }
 constexpr bool q_in_smem(int d) { return d > 128; }
 constexpr int q_bytes(int d) { return q_in_smem(d) ? d / 16 * 32 * 24 : 0; }
 constexpr int slot_floats(int d) { return kHeads * d + 2 * kHeads; }
 
 struct Shared {  // behind the ring, the merge buffer and the q fragments
-    uint64_t full[kWarps][4];
-    uint32_t scan[kWarps], longest[kWarps];
+    uint64_t full[max_warps][4];
+    uint32_t scan[max_warps], longest[max_warps];
     Cursor first;
     uint32_t edge[2];
     int last_in;
-    uint32_t valid[kWarps][4];  // a bit per token of a stage
-    float m[kWarps][kHeads], l[kWarps][kHeads];
+    uint32_t valid[max_warps][4];  // a bit per token of a tile of the warp, by the tile's number in the run modulo 4
+    float m[max_warps][kHeads], l[max_warps][kHeads];
 };
-constexpr int ring_bytes(int d) { return kWarps * stages(d) * 2 * half_bytes(d); }
-constexpr int merge_bytes(int d) { return kWarps * kHeads * merge_cols(d) * 4; }
+constexpr int ring_bytes(int d) { return warps(d) * slots(d) * slot_bytes(d); }
+constexpr int merge_bytes(int d) { return warps(d) * kHeads * merge_cols(d) * 4; }
 constexpr int smem_bytes(int d) { return ring_bytes(d) + merge_bytes(d) + q_bytes(d) + (int)sizeof(Shared); }
 static_assert(smem_bytes(256) <= 227 * 1024 && smem_bytes(128) <= 227 * 1024 && smem_bytes(96) <= 227 * 1024 &&
               2 * (smem_bytes(64) + 1024) <= 228 * 1024, "CTAs per SM");
@@ -206,13 +215,15 @@ __device__ __forceinline__ int chunk_at(int c, int r) {
 // of o.  TILED: 16 tokens lie in one page, which the tensor maps describe as (part element,
 // slot, part, k/v head, page).
 template <int D, class T, bool TILED, bool PACK>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
+__global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     attention_kernel(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    constexpr int S = stages(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
-    constexpr int WT = warp_tok(D), TT = tile_tok(D), H = WT / kBoxTok;  // H boxes of 16 tokens a stage
+    constexpr int kWarps = warps(D), kThreads = 32 * kWarps;
+    constexpr int S = slots(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
+    constexpr int WT = warp_tok(D), TT = tile_tok(D), H = WT / kBoxTok;  // H boxes of 16 tokens a slot
     constexpr uint32_t kAll = 0xffffffffu >> (32 - WT);
-    constexpr int kBox = box_bytes(D), kHalf = half_bytes(D), kStage = 2 * kHalf, kPart = part_bytes(D);
+    constexpr int kBox = box_bytes(D), kHalf = half_bytes(D), kSlot = slot_bytes(D), kPart = part_bytes(D);
     constexpr int CP2 = part_elems(D) / 16;
+    constexpr bool SPLIT = split_slots(D);
     constexpr int MC = merge_cols(D), kRows = PACK ? 4 : kHeads;
     extern __shared__ __align__(1024) unsigned char smem[];
     float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D));
@@ -295,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     }
     Cursor cc = ld;  // the item to compute next
 
-    unsigned char* ring = smem + warp * S * kStage;
+    unsigned char* ring = smem + warp * S * kSlot;
     const T* kbase = static_cast<const T*>(p.kv.k);
     const T* vbase = static_cast<const T*>(p.kv.v);
 
@@ -304,7 +315,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     // tile, lane i < WT has that of token i.
     const int32_t* pages = p.at.table + (ld.tile < ld.stop ? sequence_of(p.at, ld.row) * p.at.table_stride : 0);
     int page = -1, in_page = 0, window = 0, window_row = -1;
-    uint32_t pending = 0;  // TILED: bit s: a copy to stage s is on its way
+    uint32_t pending = 0;  // TILED: bit s: a copy to slot s is on its way
+    bool values = false;   // SPLIT: the next load is of the tile's values
+    uint32_t have_ld = 0;  // the tile's tokens that can be loaded
+    int pg = -1, in_pg = 0, loaded = 0;
     bool failed = false;   // a bounded wait gave up: nothing more is loaded or computed
     auto look_up = [&]() {  // only starts the table's loads: what they name is checked when it is used
         if (ld.tile >= ld.stop) return;
@@ -323,61 +337,68 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
             page = pages[nth];
         }
     };
-    auto load = [&](int stage) {
+    auto load = [&](int slot) {
         if (ld.tile < ld.stop) {
             const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
-            // tokens from this lane's on, the lane's page and its slot there
-            const int left = ld.tokens - (ld.tile * TT + warp * WT + (TILED ? lane % H * kBoxTok : lane % WT));
-            int pg = page, slot = in_page;
-            if constexpr (TILED) {
-                const int from = (ld.tile - window) * H + lane % H;
-                pg = __shfl_sync(0xffffffffu, page, from);
-                slot = __shfl_sync(0xffffffffu, in_page, from);
+            if (!SPLIT || !values) {
+                // tokens from this lane's on, the lane's page and its place there
+                const int left = ld.tokens - (ld.tile * TT + warp * WT + (TILED ? lane % H * kBoxTok : lane % WT));
+                pg = page;
+                in_pg = in_page;
+                if constexpr (TILED) {
+                    const int from = (ld.tile - window) * H + lane % H;
+                    pg = __shfl_sync(0xffffffffu, page, from);
+                    in_pg = __shfl_sync(0xffffffffu, in_page, from);
+                }
+                if (left <= 0) {
+                    pg = -1;
+                } else if (pg < 0 || pg >= p.kv.n_pages) {
+                    pg = -1;
+                    if (ld.item == 0 && lane < (TILED ? H : WT)) atomicAdd(p.err, TILED ? (unsigned)min(kBoxTok, left) : 1u);
+                }
+                if constexpr (TILED) {
+                    const uint32_t mine = pg < 0 ? 0u : left >= kBoxTok ? 0xffffu : (1u << left) - 1;
+                    have_ld = __shfl_sync(0xffffffffu, mine, 0);
+                    if constexpr (H == 2) have_ld |= __shfl_sync(0xffffffffu, mine, 1) << 16;
+                } else {
+                    have_ld = __ballot_sync(0xffffffffu, pg >= 0) & kAll;
+                }
+                if (lane == 0) sh.valid[warp][loaded & 3] = have_ld;
+                ++loaded;
             }
-            if (left <= 0) {
-                pg = -1;
-            } else if (pg < 0 || pg >= p.kv.n_pages) {
-                pg = -1;
-                if (ld.item == 0 && lane < (TILED ? H : WT)) atomicAdd(p.err, TILED ? (unsigned)min(kBoxTok, left) : 1u);
-            }
-            uint32_t have;
-            if constexpr (TILED) {
-                const uint32_t mine = pg < 0 ? 0u : left >= kBoxTok ? 0xffffu : (1u << left) - 1;
-                have = __shfl_sync(0xffffffffu, mine, 0);
-                if constexpr (H == 2) have |= __shfl_sync(0xffffffffu, mine, 1) << 16;
-                if (have) {
-                    pending |= 1u << stage;
-                    uint64_t* bar = &sh.full[warp][stage];
-                    const uint32_t dst = smem_u32(ring + stage * kStage);
-                    if (lane == 0) mbar_expect(bar, 2 * kBox * ((have & 0xffffu ? 1 : 0) + (have >> 16 ? 1 : 0)));
+            if (have_ld) {
+                const uint32_t dst = smem_u32(ring + slot * kSlot);
+                if constexpr (TILED) {
+                    pending |= 1u << slot;
+                    uint64_t* bar = &sh.full[warp][slot];
+                    if (lane == 0) mbar_expect(bar, (SPLIT ? 1 : 2) * kBox * ((have_ld & 0xffffu ? 1 : 0) + (have_ld >> 16 ? 1 : 0)));
                     __syncwarp();
                     if (lane < H && pg >= 0) {
-                        tma_load(dst + lane * kBox, &kmap, slot, head, pg, bar);
-                        tma_load(dst + kHalf + lane * kBox, &vmap, slot, head, pg, bar);
+                        tma_load(dst + lane * kBox, SPLIT && values ? &vmap : &kmap, in_pg, head, pg, bar);
+                        if constexpr (!SPLIT) tma_load(dst + kHalf + lane * kBox, &vmap, in_pg, head, pg, bar);
                     }
-                }
-            } else {
-                const int64_t off = pg < 0 ? -1
-                                           : (int64_t)pg * p.kv.page_stride + (int64_t)slot * p.kv.token_stride +
-                                                 (int64_t)head * p.kv.head_stride;
-                have = __ballot_sync(0xffffffffu, pg >= 0) & kAll;
-                if (have) {
-                    const uint32_t dst = smem_u32(ring + stage * kStage);
+                } else {
+                    const T* from = SPLIT && values ? vbase : kbase;
+                    const int64_t off = pg < 0 ? -1
+                                               : (int64_t)pg * p.kv.page_stride + (int64_t)in_pg * p.kv.token_stride +
+                                                     (int64_t)head * p.kv.head_stride;
 #pragma unroll 4
                     for (int i = 0; i < WT * C / 32; ++i) {
                         const int idx = i * 32 + lane, r = idx / C, ch = idx % C;
                         const int64_t ro = __shfl_sync(0xffffffffu, off, r);
                         const uint32_t at = (uint32_t)(r / kBoxTok * kBox + chunk_at<D>(ch, r % kBoxTok));
                         const int64_t el = ro < 0 ? 0 : ro + ch * 8;
-                        cp_async16(dst + at, kbase + el, ro < 0 ? 0 : 16);
-                        cp_async16(dst + kHalf + at, vbase + el, ro < 0 ? 0 : 16);
+                        cp_async16(dst + at, from + el, ro < 0 ? 0 : 16);
+                        if constexpr (!SPLIT) cp_async16(dst + kHalf + at, vbase + el, ro < 0 ? 0 : 16);
                     }
                 }
             }
-            if (lane == 0) sh.valid[warp][stage] = have;
-            if (++ld.tile == ld.stop && next_item(p.at, p.rows, p.cap, items, TT, end, ld))
-                pages = p.at.table + sequence_of(p.at, ld.row) * p.at.table_stride;
-            look_up();
+            if (!SPLIT || values) {
+                if (++ld.tile == ld.stop && next_item(p.at, p.rows, p.cap, items, TT, end, ld))
+                    pages = p.at.table + sequence_of(p.at, ld.row) * p.at.table_stride;
+                look_up();
+            }
+            values = !values;
         }
         if constexpr (!TILED) cp_commit();
     };
@@ -386,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
 #pragma unroll
     for (int k = 0; k < CP2; ++k) {
         k_at[k] = chunk_at<D>(2 * k + ((lane >> 3) & 1), (lane & 7) + ((lane >> 4) << 3));
-        v_at[k] = chunk_at<D>(2 * k + (lane >> 4), lane & 15) + kHalf;
+        v_at[k] = chunk_at<D>(2 * k + (lane >> 4), lane & 15);
     }
 
     // q of the query heads of the item at `cc`, f32: loaded ahead of its use
@@ -422,8 +443,34 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
     constexpr bool THIRD = N == 3 && !PACK;
     constexpr int QW = THIRD ? 6 : 4;  // words per k
     uint32_t qa[q_in_smem(D) ? 1 : KS / 2][2 * QW];
-    int stage = 0;
-    uint32_t phase = 0;  // bit s: parity of stage s's next completed copy
+    int at_slot = 0, computed = 0;  // the ring's next slot, and the tiles of the run behind it
+    uint32_t phase = 0;             // bit s: parity of slot s's next completed copy
+    // The next slot, once its copy has landed (TILED: false if a bounded wait gave up).
+    auto arrive = [&](bool copied, int& cur) {
+        cur = at_slot;
+        at_slot = at_slot + 1 == S ? 0 : at_slot + 1;
+        if constexpr (TILED) {
+            if (!copied) return true;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[warp][cur], (phase >> cur) & 1))) {
+                if (lane == 0) atomicAdd(p.err + 1, 1u);
+                failed = true;
+                return false;
+            }
+            phase ^= 1u << cur;
+            pending &= ~(1u << cur);
+        } else {
+            cp_wait<S - 2>();
+            __syncwarp();
+            load(cur == 0 ? S - 1 : cur - 1);  // the slot that is read
+        }
+        return true;
+    };
+    auto refill = [&](int cur) {
+        if constexpr (TILED) {
+            __syncwarp();  // every lane has read the slot
+            load(cur);
+        }
+    };
     for (;;) {
         // ---- one item, or this run's piece of it: query heads h0..h0+nh of a row
         const int row = cc.row, tiles = cc.stop - cc.tile;
@@ -479,47 +526,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
         float m = -INFINITY, l = 0.f;  // running maximum (scaled, less kShift) and this lane's part of the sum
 
         for (int t = 0; t < tiles; ++t) {
-            const int cur = stage;
-            stage = stage + 1 == S ? 0 : stage + 1;
-            const uint32_t base = smem_u32(ring + cur * kStage);
-            uint32_t have;  // bit per token
-            if constexpr (TILED) {
-                if (failed) continue;
-                have = sh.valid[warp][cur];
-                if (have) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[warp][cur], (phase >> cur) & 1))) {
-                        if (lane == 0) atomicAdd(p.err + 1, 1u);
-                        failed = true;
-                        continue;
-                    }
-                    phase ^= 1u << cur;
-                    pending &= ~(1u << cur);
-                }
-            } else {
-                cp_wait<S - 2>();
-                __syncwarp();
-                load(cur == 0 ? S - 1 : cur - 1);  // the stage that the previous tile freed
-                have = sh.valid[warp][cur];
-            }
+            if (failed) continue;
+            const uint32_t have = sh.valid[warp][computed++ & 3];  // bit per token
+            int cur;
+            if (!arrive(have != 0, cur)) continue;
+            uint32_t base = smem_u32(ring + cur * kSlot);
             if (have == 0) {
-                if constexpr (TILED) {
-                    __syncwarp();  // every lane has read `valid`
-                    load(cur);
+                refill(cur);
+                if constexpr (SPLIT) {
+                    arrive(false, cur);
+                    refill(cur);
                 }
                 continue;
-            }
-            if (TILED && have != kAll) {
-                // slots behind the last token may hold anything, also NaN, and boxes without a page
-                // what was there before: their values are zeroed (their scores are replaced below)
-#pragma unroll
-                for (int n = 0; n < WT * C / 32; ++n) {
-                    const int i = n * 32 + lane, r = i / C;
-                    if (!((have >> r) & 1))
-                        *reinterpret_cast<uint4*>(ring + cur * kStage + kHalf + r / kBoxTok * kBox + chunk_at<D>(i % C, r % kBoxTok)) =
-                            make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
             }
 
             // ---- s = q . k: two 8-token MMA columns a box
@@ -551,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                         }
                     }
             }
+            if constexpr (SPLIT) refill(cur);
             float s[H][4];
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -599,6 +618,25 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
             l = fmaf(l, alpha, more);
 
             // ---- o = o * alpha + p . v
+            if constexpr (SPLIT) {
+                if (!arrive(true, cur)) continue;
+                base = smem_u32(ring + cur * kSlot);
+            } else {
+                base += kHalf;
+            }
+            if (TILED && have != kAll) {
+                // places behind the last token may hold anything, also NaN, and boxes without a page
+                // what was there before: their values are zeroed (their scores have been replaced)
+#pragma unroll
+                for (int n = 0; n < WT * C / 32; ++n) {
+                    const int i = n * 32 + lane, r = i / C;
+                    if (!((have >> r) & 1))
+                        *reinterpret_cast<uint4*>(ring + cur * kSlot + (SPLIT ? 0 : kHalf) + r / kBoxTok * kBox + chunk_at<D>(i % C, r % kBoxTok)) =
+                            make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
 #pragma unroll
             for (int c = 0; c < NT; c += 2) {
                 float d[2][4];
@@ -622,10 +660,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
                     o[c + j][1] = fmaf(o[c + j][1], alpha, d[j][1] + d[j][3]);
                 }
             }
-            if constexpr (TILED) {
-                __syncwarp();  // every lane has read the stage
-                load(cur);
-            }
+            refill(cur);
         }
 
         uint32_t c0 = cta, c1 = cta;
@@ -809,13 +844,13 @@ cudaError_t launch_typed(AttnArgs a, const CUtensorMap (&maps)[2], int sms, bool
     }
     const int64_t items = (int64_t)a.rows * a.n_kv * a.head_groups, tiles = items * tiles_of(a.cap, tile_tok(D));
     if (tiles + items > 0x7fffffff) return cudaErrorInvalidValue;  // the runs' arithmetic; checked by the caller
-    const int64_t ctas = tiles < (int64_t)sms * ctas_per_sm(D) ? tiles : (int64_t)sms * ctas_per_sm(D);
+    const int64_t most = (int64_t)sms * ctas_per_sm(D), ctas = tiles < most ? tiles : most;
     // With about as many items as CTAs, a short item is better left whole than shared (its
     // join takes longer than its tiles: 16 rows of 555 tokens and 8 k/v heads 15.2 -> 11.1
     // us, 230 rows of 5 to 180 tokens 15.3 -> 12.5); with fewer items every cut is wanted (one
     // row of 1000 tokens and 8 k/v heads 9.3 us, with moved cuts 11.7).
     a.snap = 2 * items >= ctas ? 2 : 0;
-    return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)ctas), kThreads, smem_bytes(D), pdl, s, a, maps[0],
+    return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)ctas), 32 * warps(D), smem_bytes(D), pdl, s, a, maps[0],
                          maps[1]);
 }
 
