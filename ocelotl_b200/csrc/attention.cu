@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     constexpr int MC = merge_cols(D), kRows = PACK ? 4 : kHeads;
     extern __shared__ __align__(1024) unsigned char smem[];
     float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D));
-    uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem + ring_bytes(D) + merge_bytes(D));
+    uint4* q_frag = reinterpret_cast<uint4*>(smem + ring_bytes(D) + merge_bytes(D));
     Shared& sh = *reinterpret_cast<Shared*>(smem + ring_bytes(D) + merge_bytes(D) + q_bytes(D));
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
@@ -512,9 +512,9 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 2 * QW; ++i) {
-                    if constexpr (!q_in_smem(D)) qa[k / 2][i] = f[i];
-                    else if (k / 2 % kWarps == warp) q_frag[(k / 2 * 2 * QW + i) * 32 + lane] = f[i];
+                for (int i = 0; i < 2 * QW; i += 4) {
+                    if constexpr (!q_in_smem(D)) qa[k / 2][i] = f[i], qa[k / 2][i + 1] = f[i + 1], qa[k / 2][i + 2] = f[i + 2], qa[k / 2][i + 3] = f[i + 3];
+                    else if (k / 2 % kWarps == warp) q_frag[(k / 2 * QW / 2 + i / 4) * 32 + lane] = make_uint4(f[i], f[i + 1], f[i + 2], f[i + 3]);
                 }
             }
         }
@@ -547,7 +547,10 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
                 uint32_t a[2 * QW];
                 if constexpr (q_in_smem(D)) {
 #pragma unroll
-                    for (int i = 0; i < 2 * QW; ++i) a[i] = q_frag[(k * QW + i) * 32 + lane];
+                    for (int i = 0; i < 2 * QW; i += 4) {
+                        const uint4 f = q_frag[(k / 2 * QW / 2 + i / 4) * 32 + lane];
+                        a[i] = f.x, a[i + 1] = f.y, a[i + 2] = f.z, a[i + 3] = f.w;
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 2 * QW; ++i) a[i] = qa[k / 2][i];
