@@ -346,7 +346,8 @@ OCL_API int ocl_qk_norm_rope(ocl_ctx* ctx, const float* qkv_dev, size_t qkv_stri
  * one sequence (drafted tokens, a prompt) are causal.  Query head h reads k/v head
  * h / (n_heads / n_kv_heads).  q_dev f32 [rows, n_heads, head_dim], rows q_stride
  * floats apart; out_dev f32 [rows, n_heads, head_dim].  scale > 0.  Accuracy: f32
- * (q and the softmax weights are not rounded to 16 bits).  Padding rows give zeros.
+ * (q and the softmax weights are not rounded to 16 bits); an infinite or NaN key or
+ * value that a row sees makes the outputs that it enters NaN.  Padding rows give zeros.
  * Tokens whose page is out of range are left out and counted as bad ids (a row with
  * none left is zeros), as are rows whose sequence is (zeros) and positions past the
  * block table (the tokens that it can hold are used).  The lengths are read on the

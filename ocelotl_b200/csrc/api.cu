@@ -10,6 +10,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 
 #include "../../include/ocelotl_cuda.h"
@@ -334,23 +335,6 @@ int take_timeouts(ocl_ctx* ctx, const char* op) {
                 "incomplete", op, n);
 }
 
-// Per-row slots and counters of the greedy pick (argmax and logit rules).
-int ensure_argmax(ocl_ctx* ctx) {
-    if (ctx->amax_counters) return OCL_OK;
-    const size_t sb = ocl::kArgmaxRowsMax * sizeof(unsigned long long), cb = ocl::kArgmaxRowsMax * sizeof(unsigned int);
-    if (!ctx->amax_slots) OCL_CUDA(ctx, cudaMalloc((void**)&ctx->amax_slots, sb), "cudaMalloc(argmax slots)");
-    OCL_CUDA(ctx, cudaMemsetAsync(ctx->amax_slots, 0, sb, ctx->stream), "memset argmax slots");
-    unsigned int* counters = nullptr;
-    OCL_CUDA(ctx, cudaMalloc((void**)&counters, cb), "cudaMalloc(argmax counters)");
-    const cudaError_t e = cudaMemsetAsync(counters, 0, cb, ctx->stream);
-    if (e != cudaSuccess) {
-        cudaFree(counters);
-        return cuda_fail(ctx, e, "memset argmax counters");
-    }
-    ctx->amax_counters = counters;
-    return OCL_OK;
-}
-
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
 // Whether two [rows, width] f32 blocks share memory (by their whole extents).
@@ -442,14 +426,23 @@ int ocl_cuda_init(int device, ocl_ctx** out) {
     if (e == cudaSuccess) e = cudaMemset(ctx->dev_flags, 0, 64);
     if (e == cudaSuccess) e = cudaHostAlloc((void**)&ctx->host_flags, 64, cudaHostAllocMapped);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer((void**)&ctx->host_flags_dev, ctx->host_flags, 0);
-    // The attention workspace has one size for every call (a few MB): made here,
-    // it never moves under a captured launch.
+    // The pick's and the attention's workspaces have one size for every call (a few
+    // MB): made here, they need no call before a capture and never move under one.
+    const size_t slot_bytes = ocl::kArgmaxRowsMax * sizeof(unsigned long long);
+    const size_t arrival_bytes = ocl::kArgmaxRowsMax * sizeof(unsigned int);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&ctx->amax_slots, slot_bytes);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&ctx->amax_counters, arrival_bytes);
+    if (e == cudaSuccess) e = cudaMemset(ctx->amax_slots, 0, slot_bytes);
+    if (e == cudaSuccess) e = cudaMemset(ctx->amax_counters, 0, arrival_bytes);
     if (e == cudaSuccess) e = cudaMalloc((void**)&ctx->attn_part, ocl::attention_part_bytes(ctx->sms));
     if (e == cudaSuccess) e = cudaMalloc((void**)&ctx->attn_counters, ocl::attention_counters(ctx->sms) * 4);
     if (e == cudaSuccess) e = cudaMemset(ctx->attn_counters, 0, ocl::attention_counters(ctx->sms) * 4);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // the zeros are there for calls on any stream
     if (e != cudaSuccess) {
         if (ctx->dev_flags) cudaFree(ctx->dev_flags);
         if (ctx->host_flags) cudaFreeHost(ctx->host_flags);
+        if (ctx->amax_slots) cudaFree(ctx->amax_slots);
+        if (ctx->amax_counters) cudaFree(ctx->amax_counters);
         if (ctx->attn_part) cudaFree(ctx->attn_part);
         if (ctx->attn_counters) cudaFree(ctx->attn_counters);
         delete ctx;
@@ -949,8 +942,6 @@ int ocl_argmax_f32(ocl_ctx* ctx, const float* logits_dev, size_t rows, size_t vo
                     "unsupported feature `argmax shape` (requested `%zu x %zu`): supported = [rows <= %d, vocab < 2^31]",
                     rows, vocab, ocl::kArgmaxRowsMax);
     DeviceGuard guard(ctx->device);
-    const int rc = ensure_argmax(ctx);
-    if (rc) return rc;
     OCL_CUDA(ctx,
              ocl::launch_argmax(logits_dev, (int64_t)rows, (int64_t)vocab, ids_dev, ctx->amax_slots,
                                 ctx->amax_counters, ctx->stream),
@@ -979,7 +970,8 @@ int ocl_rope_create(ocl_ctx* ctx, size_t rot_dim, double base, const float* fact
         steps[i] = scaled >= ldexpl(1.0L, 64) ? 0ull : (unsigned long long)scaled;
     }
     DeviceGuard guard(ctx->device);
-    ocl_rope* r = new ocl_rope();
+    ocl_rope* r = new (std::nothrow) ocl_rope();
+    if (!r) return fail(ctx, OCL_ERR_OOM, "rope_create: out of host memory");
     r->device = ctx->device;
     r->rot = (int)rot_dim;
     r->interleaved = interleaved != 0;
@@ -1101,10 +1093,6 @@ int ocl_logits_process(ocl_ctx* ctx, const float* logits, size_t in_stride, size
                       : out && overlap(logits, in_stride, out, out_stride, rows, vocab, vocab))
         return fail(ctx, OCL_ERR_INVALID, "process_logits out overlaps logits; in place needs the same pointer and row stride");
     DeviceGuard guard(ctx->device);
-    if (ids) {
-        const int rc = ensure_argmax(ctx);
-        if (rc) return rc;
-    }
     const ocl::LogitRules rules{r->history_dev, (int64_t)r->history_stride, (int64_t)r->history_max, r->history_lens_dev, r->prompt_lens_dev,
                                 r->repetition_dev, r->frequency_dev, r->presence_dev, r->bias_ids_dev,
                                 r->bias_values_dev, (int64_t)r->bias_stride, (int64_t)r->bias_count, r->allowed_dev, (int64_t)r->allowed_stride};

@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
                     for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = max(-100, min(100, 134 - (int)((__float_as_uint(top) >> 23) & 255)));
+                const int e = max(-126, min(126, 134 - (int)((__float_as_uint(top) >> 23) & 255)));
                 const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                 scale *= __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll

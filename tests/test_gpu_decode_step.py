@@ -149,3 +149,48 @@ def test_prompt_and_steps(backend, oracle, model, dtype):
     for a, b in zip(run.caches, other.caches):
         assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
     assert backend.take_device_errors() == (0, 0)
+
+
+def test_first_calls_of_a_context_may_be_captured():
+    """Nothing is allocated or set up by a first call that a capture would refuse."""
+    from ocelotl_b200 import CudaKernelBackend
+    b = CudaKernelBackend(0)
+    cache = b.kv_cache(4, 16, 1, 96, torch.float16)
+    rope = b.rope_table(96, 1e4)
+    qkv, pos = torch.randn(1, 5 * 96, device="cuda"), torch.tensor([0], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[2]], dtype=torch.int32, device="cuda")
+    logits, ids = torch.randn(1, 777, device="cuda"), torch.full((1,), -1, dtype=torch.int32, device="cuda")
+    rules = b.logit_rules()
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        b.use_current_stream()
+        out = b.paged_attention(b.qk_norm_rope(qkv, cache, pos, table, rope), cache, pos, table)
+        b.greedy_sample(logits, out=ids, rules=rules)
+    b.set_stream(None)
+    graph.replay()
+    torch.cuda.synchronize()
+    # one token: the softmax is 1 and the output is the value as cached
+    v = qkv[0, 4 * 96:].half().float()
+    assert (out[0] - v).abs().max() <= 2.0 ** -20 * v.abs().max()
+    assert ids.item() == int(logits.argmax())
+
+
+def test_two_contexts_on_two_streams(backend):
+    """A context per stream: their calls may overlap on the GPU."""
+    from ocelotl_b200 import CudaKernelBackend
+    from tests.decode_cases import paged
+    k, v, table = paged([20000], 16, 2, 128, torch.bfloat16, 3)
+    q = torch.randn(1, 8, 128, device="cuda")
+    pos = torch.tensor([19999], dtype=torch.int32, device="cuda")
+    cache = backend.kv_cache_view(k, v)
+    want = backend.paged_attention(q, cache, pos, table)
+    torch.cuda.synchronize()
+    streams, contexts, got = [torch.cuda.Stream() for _ in range(2)], [CudaKernelBackend(0) for _ in range(2)], []
+    for _ in range(20):
+        for s, b in zip(streams, contexts):
+            with torch.cuda.stream(s):
+                b.use_current_stream()
+                got.append(b.paged_attention(q, cache, pos, table))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
