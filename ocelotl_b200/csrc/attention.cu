@@ -243,12 +243,16 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     }
     grid_wait();
 
-    // ---- this CTA's run: rows' units summed over the threads, then the two cuts located
-    const int per = (p.rows + kThreads - 1) / kThreads;
-    const int r0 = min(tid * per, p.rows), r1 = min(r0 + per, p.rows);
+    // ---- this CTA's run: the rows' units summed over the threads, then its two cuts
+    // located, one by either half of the CTA (which both sum all rows)
+    constexpr int kHalfThreads = kThreads / 2, kHalfWarps = kWarps / 2;
+    const int side = warp / kHalfWarps, per = (p.rows + kHalfThreads - 1) / kHalfThreads;
+    const int r0 = min(tid % kHalfThreads * per, p.rows), r1 = min(r0 + per, p.rows);
     uint32_t mine = 0, longest = 0;
+    int first_tokens = 0;
     for (int r = r0; r < r1; ++r) {
-        const int tiles = tiles_of(row_tokens(p.at, p.cap, r), TT);
+        const int tokens = row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
+        if (r == r0) first_tokens = tokens;
         if (tiles) mine += item_units(tiles);
         longest = max(longest, (uint32_t)tiles);
     }
@@ -264,8 +268,8 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     __syncthreads();
     uint32_t total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) upto += sh.scan[w];
+    for (int w = 0; w < kHalfWarps; ++w) {
+        if (w < warp % kHalfWarps) upto += sh.scan[w];
         total += sh.scan[w];
         longest = max(longest, sh.longest[w]);
     }
@@ -274,19 +278,17 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     const Runs runs = runs_of(total, gridDim.x, max(1u, (uint32_t)(sqrtf(0.1f * (float)longest) + 0.999f)), p.snap);
     const uint32_t cta = blockIdx.x;
     const bool active = total > 0 && cta < runs.P;
-    if (active) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t cut = run_cut(runs, cta + i);
-            uint32_t at = upto - mine;
-            if (cut < at || cut >= upto) continue;
+    {
+        const uint32_t cut = run_cut(runs, cta + side);
+        uint32_t at = upto - mine;
+        if (active && cut >= at && cut < upto) {
             for (int r = r0;; ++r) {
-                const int tokens = row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
+                const int tokens = r == r0 ? first_tokens : row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
                 const uint32_t all = tiles ? item_units(tiles) : 0, off = cut - at;
                 if (off < all * items) {
                     const uint32_t item = off / all, u = off - item * all, moved = moved_cut(runs, u, tiles);
-                    sh.edge[i] = cut - u + moved;
-                    if (i == 0) sh.first = {r, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
+                    sh.edge[side] = cut - u + moved;
+                    if (side == 0) sh.first = {r, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
                     break;
                 }
                 at += all * items;

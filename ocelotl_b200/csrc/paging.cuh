@@ -73,7 +73,7 @@ OCL_HD uint32_t item_units(int tiles) { return (uint32_t)(tiles + kItemCost); }
 OCL_HD Runs runs_of(uint32_t total, uint32_t ctas, uint32_t min_share, int snap) {
     Runs r;
     r.total = total;
-    r.P = total / min_share;
+    r.P = min_share > 1 ? total / min_share : total;
     r.P = r.P < 1 ? 1 : r.P < ctas ? r.P : ctas;
     r.share = total / r.P;
     r.rest = total - r.share * r.P;
