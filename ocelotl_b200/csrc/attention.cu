@@ -158,6 +158,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
         if (clock64() - t0 > 2000000000LL) return false;
     return true;
 }
+__device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int in_page, int head, int page, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], "
@@ -309,6 +314,7 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     Cursor cc = ld;  // the item to compute next
 
     unsigned char* ring = smem + warp * S * kSlot;
+    const uint32_t n_pages = (uint32_t)p.kv.n_pages;  // below 2^31
     const T* kbase = static_cast<const T*>(p.kv.k);
     const T* vbase = static_cast<const T*>(p.kv.v);
 
@@ -317,10 +323,12 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     // tile, lane i < WT has that of token i.
     const int32_t* pages = p.at.table + (ld.tile < ld.stop ? sequence_of(p.at, ld.row) * p.at.table_stride : 0);
     int page = -1, in_page = 0, window = 0, window_row = -1;
+    bool fresh = false, wanted = false, window_ok = false;  // TILED: a window not yet checked, this lane's part, its result
     uint32_t pending = 0;  // TILED: bit s: a copy to slot s is on its way
+    uint32_t full = 0;     // bit s: slot s holds (SPLIT: the keys of) all of the warp's tokens; else sh.valid says which
     bool values = false;   // SPLIT: the next load is of the tile's values
     uint32_t have_ld = 0;  // the tile's tokens that can be loaded
-    int pg = -1, in_pg = 0, loaded = 0;
+    int box_page[H], box_slot[H], loaded = 0;  // TILED: the places of its boxes; else [0]: this lane's token's page
     bool failed = false;   // a bounded wait gave up: nothing more is loaded or computed
     auto look_up = [&]() {  // only starts the table's loads: what they name is checked when it is used
         if (ld.tile >= ld.stop) return;
@@ -333,7 +341,9 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
         } else {
             tok += lane % WT;
         }
-        if (tok < ld.tokens) {
+        fresh = true;
+        wanted = tok < ld.tokens;
+        if (wanted) {
             const uint32_t nth = quotient((uint32_t)tok, p.page_size);
             in_page = (int)((uint32_t)tok - nth * p.page_size.d);
             page = pages[nth];
@@ -342,48 +352,68 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     auto load = [&](int slot) {
         if (ld.tile < ld.stop) {
             const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
+            const int left = ld.tokens - (ld.tile * TT + warp * WT);  // tokens from the warp's first on
             if (!SPLIT || !values) {
-                // tokens from this lane's on, the lane's page and its place there
-                const int left = ld.tokens - (ld.tile * TT + warp * WT + (TILED ? lane % H * kBoxTok : lane % WT));
-                pg = page;
-                in_pg = in_page;
+                bool all = false;  // TILED: all of the warp's tokens are there, and so are the window's pages
                 if constexpr (TILED) {
-                    const int from = (ld.tile - window) * H + lane % H;
-                    pg = __shfl_sync(0xffffffffu, page, from);
-                    in_pg = __shfl_sync(0xffffffffu, in_page, from);
+                    if (fresh) {
+                        fresh = false;
+                        window_ok = __all_sync(0xffffffffu, !wanted || (uint32_t)page < n_pages);
+                    }
+                    all = left >= WT && window_ok;
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        box_page[h] = __shfl_sync(0xffffffffu, page, (ld.tile - window) * H + h);
+                        box_slot[h] = __shfl_sync(0xffffffffu, in_page, (ld.tile - window) * H + h);
+                    }
                 }
-                if (left <= 0) {
-                    pg = -1;
-                } else if (pg < 0 || pg >= p.kv.n_pages) {
-                    pg = -1;
-                    if (ld.item == 0 && lane < (TILED ? H : WT)) atomicAdd(p.err, TILED ? (unsigned)min(kBoxTok, left) : 1u);
-                }
-                if constexpr (TILED) {
-                    const uint32_t mine = pg < 0 ? 0u : left >= kBoxTok ? 0xffffu : (1u << left) - 1;
-                    have_ld = __shfl_sync(0xffffffffu, mine, 0);
-                    if constexpr (H == 2) have_ld |= __shfl_sync(0xffffffffu, mine, 1) << 16;
+                if (all) {
+                    have_ld = kAll;
+                    full |= 1u << slot;
                 } else {
-                    have_ld = __ballot_sync(0xffffffffu, pg >= 0) & kAll;
+                    uint32_t bad = 0;  // tokens without a page
+                    if constexpr (TILED) {
+                        have_ld = 0;
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const uint32_t seen = (uint32_t)min(max(left - h * kBoxTok, 0), kBoxTok);
+                            const bool ok = (uint32_t)box_page[h] < n_pages;
+                            have_ld |= ok ? ((1u << seen) - 1) << (kBoxTok * h) : 0u;
+                            bad += ok ? 0u : seen;
+                        }
+                        bad = lane == 0 ? bad : 0u;
+                    } else {
+                        const bool mine = left > lane % WT, ok = (uint32_t)page < n_pages;
+                        box_page[0] = mine && ok ? page : -1;
+                        have_ld = __ballot_sync(0xffffffffu, mine && ok) & kAll;
+                        bad = mine && !ok && lane < WT;
+                    }
+                    if (bad && ld.item == 0) atomicAdd(p.err, bad);
+                    if (lane == 0) sh.valid[warp][loaded & 3] = have_ld;
+                    full &= ~(1u << slot);
                 }
-                if (lane == 0) sh.valid[warp][loaded & 3] = have_ld;
                 ++loaded;
             }
             if (have_ld) {
                 const uint32_t dst = smem_u32(ring + slot * kSlot);
                 if constexpr (TILED) {
                     pending |= 1u << slot;
-                    uint64_t* bar = &sh.full[warp][slot];
-                    if (lane == 0) mbar_expect(bar, (SPLIT ? 1 : 2) * kBox * ((have_ld & 0xffffu ? 1 : 0) + (have_ld >> 16 ? 1 : 0)));
-                    __syncwarp();
-                    if (lane < H && pg >= 0) {
-                        tma_load(dst + lane * kBox, SPLIT && values ? &vmap : &kmap, in_pg, head, pg, bar);
-                        if constexpr (!SPLIT) tma_load(dst + kHalf + lane * kBox, &vmap, in_pg, head, pg, bar);
+                    if (elect_one()) {
+                        uint64_t* bar = &sh.full[warp][slot];
+                        mbar_expect(bar, (SPLIT ? 1 : 2) * kBox * ((have_ld & 1) + (H == 2 ? have_ld >> 16 & 1 : 0)));
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            if (!((have_ld >> (kBoxTok * h)) & 1)) continue;
+                            tma_load(dst + h * kBox, SPLIT && values ? &vmap : &kmap, box_slot[h], head, box_page[h], bar);
+                            if constexpr (!SPLIT) tma_load(dst + kHalf + h * kBox, &vmap, box_slot[h], head, box_page[h], bar);
+                        }
                     }
+                    __syncwarp();
                 } else {
                     const T* from = SPLIT && values ? vbase : kbase;
-                    const int64_t off = pg < 0 ? -1
-                                               : (int64_t)pg * p.kv.page_stride + (int64_t)in_pg * p.kv.token_stride +
-                                                     (int64_t)head * p.kv.head_stride;
+                    const int64_t off = box_page[0] < 0 ? -1
+                                                        : (int64_t)box_page[0] * p.kv.page_stride +
+                                                              (int64_t)in_page * p.kv.token_stride + (int64_t)head * p.kv.head_stride;
 #pragma unroll 4
                     for (int i = 0; i < WT * C / 32; ++i) {
                         const int idx = i * 32 + lane, r = idx / C, ch = idx % C;
@@ -529,7 +559,8 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
 
         for (int t = 0; t < tiles; ++t) {
             if (failed) continue;
-            const uint32_t have = sh.valid[warp][computed++ & 3];  // bit per token
+            const uint32_t have = (full >> at_slot) & 1 ? kAll : sh.valid[warp][computed & 3];  // bit per token
+            ++computed;
             int cur;
             if (!arrive(have != 0, cur)) continue;
             uint32_t base = smem_u32(ring + cur * kSlot);
