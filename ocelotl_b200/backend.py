@@ -567,7 +567,7 @@ class CudaKernelBackend:
             self._check(rc)
         return out
 
-    def _logits_call(self, op: str, logits: torch.Tensor, rules: LogitRules, out, ids) -> None:
+    def _logits_call(self, op: str, logits: torch.Tensor, rules: LogitRules, out, ids, allocate: bool) -> torch.Tensor | None:
         check_tensor(logits, op, "logits", torch.float32, self.torch_device, 2)
         if not isinstance(rules, LogitRules) or rules.device != self.torch_device:
             raise _kernel_err(f"{op} rules must be LogitRules on {self.torch_device}")
@@ -584,12 +584,15 @@ class CudaKernelBackend:
             check_tensor(ids, op, "ids", torch.int32, self.torch_device, 1)
             if ids.shape[0] != rows:
                 raise _kernel_err(f"{op} ids.len()={ids.shape[0]} does not match rows={rows}")
+        if out is None and allocate:
+            out = self._alloc(logits, rows, vocab)
         rc = self._lib.ocl_logits_process(
             self._ctx, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, rules.ref,
             None if out is None else out.data_ptr(),
             0 if out is None else out.stride(0) if rows > 1 else vocab, None if ids is None else ids.data_ptr())
         if rc:
             self._check(rc)
+        return out
 
     def process_logits(self, logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None,
                        ids: torch.Tensor | None = None) -> torch.Tensor:
@@ -598,11 +601,7 @@ class CudaKernelBackend:
         out may be `logits` itself.  With ids (int32 [rows]) the greedy pick of the
         result is written there in the same launch.
         """
-        if out is None:
-            check_tensor(logits, "process_logits", "logits", torch.float32, self.torch_device, 2)
-            out = self._alloc(logits, *logits.shape)
-        self._logits_call("process_logits", logits, rules, out, ids)
-        return out
+        return self._logits_call("process_logits", logits, rules, out, ids, True)
 
     # -- greedy sampling (crates/runtime/src/sampling.rs:29) ----------------------
     def greedy_sample(self, logits, out: torch.Tensor | None = None, rules: LogitRules | None = None):
@@ -623,7 +622,7 @@ class CudaKernelBackend:
                 logits = logits.unsqueeze(0)
             if out is None:
                 out = self._alloc(logits, logits.shape[0], dtype=torch.int32)
-            self._logits_call("greedy_sample", logits, rules, None, out)
+            self._logits_call("greedy_sample", logits, rules, None, out, False)
             return out
         if not isinstance(logits, torch.Tensor):
             arr = np.ascontiguousarray(logits, dtype=np.float32).reshape(-1)
