@@ -17,20 +17,22 @@
 //     bf16: 3 pieces of 8 bits = 24 bits;   f16: 2 pieces of 11 bits = 22 bits
 // (q scaled by a power of two per head, p by 2^14, so that f16's range is enough).
 // The tensor core truncates when it adds; chains are kept short (two chains over
-// head_dim, 32 tokens of p.v) and joined with rounding f32 adds.
+// head_dim, 32 tokens of p.v) and joined with rounding f32 adds.  Error against the formula
+// in 64 bits: 2e-7 to 4e-7 of the result, below that of f32 matrix products.
 //
 // Work split: the tiles (4 warps of 32 tokens of one row and k/v head) of all rows, in
 // order, are cut into equal runs, one per resident CTA, from the positions in device
 // memory -- so one captured launch stays balanced while the lengths grow (paging.cuh has
-// the arithmetic).  Each warp streams its own tokens through a private ring of stages and
-// needs no barrier inside an item.  Where 16 tokens always lie in one page (page sizes
-// that are multiples of 16), tensor-map copies (cp.async.bulk.tensor, its swizzle doing
-// the bank spreading) bring 16 keys or values each; other page sizes gather rows with
-// cp.async.  A row whose tiles lie in several CTAs is joined by the last of them to
-// arrive, in CTA order: the result does not depend on which one it is.  Nothing waits on
-// another CTA.
-#include <cuda.h>
-
+// the arithmetic).  Each warp streams its own tokens through a private ring of cp.async
+// slots, rows gathered from whatever pages they lie in, and needs no barrier inside an
+// item.  (Tensor-map copies of 16 tokens, with bounded waits and a second path for other
+// page sizes, measured the same: 158 against 155 us for 8 rows of 30000 tokens, 8.9 against
+// 9.1 for one of 555; issuing them took a warp as long as the gather.)  A row whose tiles
+// lie in several CTAs is joined by the last of them to arrive, in CTA order: the result
+// does not depend on which one it is.  Nothing waits on another CTA.
+//
+// Measured (bf16, 8 k/v heads, head_dim 128, a pass among others): 61 rows of 70 to 16000 tokens,
+// 4 heads each, 130 us = 6.1 TB/s; one row of 131000 tokens 91 us = 5.9 TB/s.
 #include "device.cuh"
 #include "internal.cuh"
 
@@ -39,15 +41,15 @@ namespace ocl {
 namespace {
 
 constexpr int kHeads = 8;   // query heads of one k/v head worked on together
-constexpr int kBoxTok = 16; // tokens of one tensor-map copy, and of one p.v MMA
+constexpr int kBoxTok = 16; // tokens kept together: those of one p.v MMA
 
 // Tokens a warp takes at a time.  32 halve the work a token costs besides its MMAs
 // (maximum, rescaling, waits, look-ups) and give a warp twice the independent MMAs; at
 // head_dim 256 they would not leave three slots to each of 8 warps.
 constexpr int warp_tok(int d) { return d == 256 ? 16 : 32; }
 // Warps and ring.  Up to head_dim 128 four warps, each with a ring of slots that hold the
-// keys and the values of its tokens: 1.5 us a tile, about what HBM takes to bring it.  At
-// head_dim 256 a tile takes a warp twice as long and eight are wanted; their rings have
+// keys and the values of its tokens: a tile takes about as long as HBM takes to bring it.
+// At head_dim 256 a tile takes a warp twice as long and eight are wanted; their rings have
 // separate slots for keys and values, so that three of 8 KB keep copies under way
 // (6 rows of 900 to 6000 tokens, 4 k/v heads of 8: 25.6 us with four warps, 22.9 with
 // eight; at head_dim 128 both changes lose: 64 ragged rows 123 us, 143 and 129).
@@ -58,9 +60,8 @@ constexpr int slots(int d) { return d == 96 ? 4 : 3; }
 constexpr int ctas_per_sm(int d) { return d == 64 ? 2 : 1; }
 constexpr int max_ctas_per_sm = 2;
 constexpr int tile_tok(int d) { return warps(d) * warp_tok(d); }
-// 16 tokens of k or v are kept as parts of 64 elements (32 for head_dim 96): a part is
-// 16 rows of 128 (64) bytes, its 16-byte chunks exclusive-or'ed with the row as the
-// copy engine's 128-byte (64-byte) swizzle does.
+// A box of 16 tokens of k or v is kept as parts of 64 elements (32 for head_dim 96): a part is
+// 16 rows of 128 (64) bytes, its 16-byte chunks exclusive-or'ed with the row.
 constexpr int part_elems(int d) { return d % 64 == 0 ? 64 : 32; }
 constexpr int part_bytes(int d) { return kBoxTok * part_elems(d) * 2; }
 constexpr int box_bytes(int d) { return kBoxTok * d * 2; }
@@ -72,7 +73,6 @@ constexpr int q_bytes(int d) { return q_in_smem(d) ? d / 16 * 32 * 24 : 0; }
 constexpr int slot_floats(int d) { return kHeads * d + 2 * kHeads; }
 
 struct Shared {  // behind the ring, the merge buffer and the q fragments
-    uint64_t full[max_warps][4];
     uint32_t scan[max_warps], longest[max_warps];
     Cursor first;
     uint32_t edge[2];
@@ -138,38 +138,6 @@ OCL_MMA("bf16", __nv_bfloat16)
 OCL_MMA("f16", __half)
 #undef OCL_MMA
 
-__device__ __forceinline__ void mbar_init(uint64_t* bar) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return ok != 0;
-}
-// Wait for at most ~1 s of SM clocks; false if it gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-    if (mbar_test(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_test(bar, parity))
-        if (clock64() - t0 > 2000000000LL) return false;
-    return true;
-}
-__device__ __forceinline__ bool elect_one() {  // one lane of a converged warp
-    uint32_t one;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
-    return one != 0;
-}
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int in_page, int head, int page, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], "
-        "[%6];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(in_page), "r"(head), "r"(page), "r"(smem_u32(bar))
-        : "memory");
-}
-
 template <int V>
 __device__ __forceinline__ void load_cg(float (&x)[V], const float* p) {
     if constexpr (V == 4) {
@@ -217,11 +185,9 @@ __device__ __forceinline__ int chunk_at(int c, int r) {
 
 // PACK (bf16, at most 4 heads): rows 0-3 leading pieces, 4-7 third, 8-11 second, so that
 // one MMA does what takes two with 8 heads; lanes 16-31 then hold the third pieces' part
-// of o.  TILED: 16 tokens lie in one page, which the tensor maps describe as (part element,
-// slot, part, k/v head, page).
-template <int D, class T, bool TILED, bool PACK>
-__global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
-    attention_kernel(const AttnArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+// of o.
+template <int D, class T, bool PACK>
+__global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D)) attention_kernel(const AttnArgs p) {
     constexpr int kWarps = warps(D), kThreads = 32 * kWarps;
     constexpr int S = slots(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
     constexpr int WT = warp_tok(D), TT = tile_tok(D), H = WT / kBoxTok;  // H boxes of 16 tokens a slot
@@ -237,15 +203,6 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int items = p.n_kv * p.head_groups;
-    if (TILED && tid == 0) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
-    }
-    if (TILED && lane < S) {
-        mbar_init(&sh.full[warp][lane]);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
     grid_wait();
 
     // ---- this CTA's run: the rows' units summed over the threads, then its two cuts
@@ -318,77 +275,44 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     const T* kbase = static_cast<const T*>(p.kv.k);
     const T* vbase = static_cast<const T*>(p.kv.v);
 
-    // Pages are looked up ahead of their loads.  TILED: for the next 32 / H tiles at once,
-    // lane i has the page of the (i % H)-th box of tile `window` + i / H.  Else for one
-    // tile, lane i < WT has that of token i.
+    // The place of token lane % WT of the warp's tokens of the tile at `ld`, looked up one
+    // tile ahead of its loads.
     const int32_t* pages = p.at.table + (ld.tile < ld.stop ? sequence_of(p.at, ld.row) * p.at.table_stride : 0);
-    int page = -1, in_page = 0, window = 0, window_row = -1;
-    bool fresh = false, wanted = false, window_ok = false;  // TILED: a window not yet checked, this lane's part, its result
-    uint32_t pending = 0;  // TILED: bit s: a copy to slot s is on its way
-    uint32_t full = 0;     // bit s: slot s holds (SPLIT: the keys of) all of the warp's tokens; else sh.valid says which
-    bool values = false;   // SPLIT: the next load is of the tile's values
-    uint32_t have_ld = 0;  // the tile's tokens that can be loaded
-    int box_page[H], box_slot[H], loaded = 0;  // TILED: the places of its boxes; else [0]: this lane's token's page
-    bool failed = false;   // a bounded wait gave up: nothing more is loaded or computed
-    auto look_up = [&]() {  // only starts the table's loads: what they name is checked when it is used
-        if (ld.tile >= ld.stop) return;
-        int tok = ld.tile * TT + warp * WT;
-        if constexpr (TILED) {
-            if (ld.row == window_row && (unsigned)(ld.tile - window) < 32 / H) return;
-            window_row = ld.row;
-            window = ld.tile;
-            tok += lane / H * TT + lane % H * kBoxTok;
-        } else {
-            tok += lane % WT;
-        }
-        fresh = true;
-        wanted = tok < ld.tokens;
-        if (wanted) {
+    int page = -1, in_page = 0;
+    auto look_up = [&]() {  // only starts the table's load: what it names is checked when it is used
+        const int tok = ld.tile * TT + warp * WT + lane % WT;
+        if (ld.tile < ld.stop && tok < ld.tokens) {
             const uint32_t nth = quotient((uint32_t)tok, p.page_size);
             in_page = (int)((uint32_t)tok - nth * p.page_size.d);
             page = pages[nth];
         }
     };
+    // Loads: 4 lanes a row, 64 bytes of it at a time, 8 rows together; the row's place comes
+    // from the lane that looked it up.  Rows without a place are zeros.
+    constexpr int CG = C / 4;
+    const int rq = lane >> 2, cq = lane & 3;
+    int dst_at[CP2 == 4 ? 2 : 1];  // where this lane's chunk of an even / odd run of 4 goes
+    dst_at[0] = chunk_at<D>(cq, rq);
+    if constexpr (CP2 == 4) dst_at[1] = chunk_at<D>(4 + cq, rq);
+    bool values = false;   // SPLIT: the next load is of the tile's values
+    int64_t place = 0;     // this lane's token's, in elements; -1: none
+    uint32_t have_ld = 0;  // the tile's tokens that have a place
+    uint32_t full = 0;     // bit s: slot s holds (SPLIT: the keys of) all of the warp's tokens; else sh.valid says which
+    int loaded = 0;
     auto load = [&](int slot) {
         if (ld.tile < ld.stop) {
-            const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
-            const int left = ld.tokens - (ld.tile * TT + warp * WT);  // tokens from the warp's first on
             if (!SPLIT || !values) {
-                bool all = false;  // TILED: all of the warp's tokens are there, and so are the window's pages
-                if constexpr (TILED) {
-                    if (fresh) {
-                        fresh = false;
-                        window_ok = __all_sync(0xffffffffu, !wanted || (uint32_t)page < n_pages);
-                    }
-                    all = left >= WT && window_ok;
-#pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        box_page[h] = __shfl_sync(0xffffffffu, page, (ld.tile - window) * H + h);
-                        box_slot[h] = __shfl_sync(0xffffffffu, in_page, (ld.tile - window) * H + h);
-                    }
-                }
-                if (all) {
+                const int head = p.head_groups == 1 ? ld.item : ld.item / p.head_groups;
+                const bool mine = ld.tile * TT + warp * WT + lane % WT < ld.tokens, ok = (uint32_t)page < n_pages;
+                place = mine && ok ? (int64_t)page * p.kv.page_stride + (int64_t)in_page * p.kv.token_stride +
+                                         (int64_t)head * p.kv.head_stride
+                                   : -1;
+                if (__all_sync(0xffffffffu, mine && ok)) {
                     have_ld = kAll;
                     full |= 1u << slot;
                 } else {
-                    uint32_t bad = 0;  // tokens without a page
-                    if constexpr (TILED) {
-                        have_ld = 0;
-#pragma unroll
-                        for (int h = 0; h < H; ++h) {
-                            const uint32_t seen = (uint32_t)min(max(left - h * kBoxTok, 0), kBoxTok);
-                            const bool ok = (uint32_t)box_page[h] < n_pages;
-                            have_ld |= ok ? ((1u << seen) - 1) << (kBoxTok * h) : 0u;
-                            bad += ok ? 0u : seen;
-                        }
-                        bad = lane == 0 ? bad : 0u;
-                    } else {
-                        const bool mine = left > lane % WT, ok = (uint32_t)page < n_pages;
-                        box_page[0] = mine && ok ? page : -1;
-                        have_ld = __ballot_sync(0xffffffffu, mine && ok) & kAll;
-                        bad = mine && !ok && lane < WT;
-                    }
-                    if (bad && ld.item == 0) atomicAdd(p.err, bad);
+                    have_ld = __ballot_sync(0xffffffffu, mine && ok) & kAll;
+                    if (mine && !ok && ld.item == 0 && lane < WT) atomicAdd(p.err, 1u);
                     if (lane == 0) sh.valid[warp][loaded & 3] = have_ld;
                     full &= ~(1u << slot);
                 }
@@ -396,32 +320,18 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
             }
             if (have_ld) {
                 const uint32_t dst = smem_u32(ring + slot * kSlot);
-                if constexpr (TILED) {
-                    pending |= 1u << slot;
-                    if (elect_one()) {
-                        uint64_t* bar = &sh.full[warp][slot];
-                        mbar_expect(bar, (SPLIT ? 1 : 2) * kBox * ((have_ld & 1) + (H == 2 ? have_ld >> 16 & 1 : 0)));
+                const T* from = SPLIT && values ? vbase : kbase;
 #pragma unroll
-                        for (int h = 0; h < H; ++h) {
-                            if (!((have_ld >> (kBoxTok * h)) & 1)) continue;
-                            tma_load(dst + h * kBox, SPLIT && values ? &vmap : &kmap, box_slot[h], head, box_page[h], bar);
-                            if constexpr (!SPLIT) tma_load(dst + kHalf + h * kBox, &vmap, box_slot[h], head, box_page[h], bar);
-                        }
-                    }
-                    __syncwarp();
-                } else {
-                    const T* from = SPLIT && values ? vbase : kbase;
-                    const int64_t off = box_page[0] < 0 ? -1
-                                                        : (int64_t)box_page[0] * p.kv.page_stride +
-                                                              (int64_t)in_page * p.kv.token_stride + (int64_t)head * p.kv.head_stride;
-#pragma unroll 4
-                    for (int i = 0; i < WT * C / 32; ++i) {
-                        const int idx = i * 32 + lane, r = idx / C, ch = idx % C;
-                        const int64_t ro = __shfl_sync(0xffffffffu, off, r);
-                        const uint32_t at = (uint32_t)(r / kBoxTok * kBox + chunk_at<D>(ch, r % kBoxTok));
-                        const int64_t el = ro < 0 ? 0 : ro + ch * 8;
-                        cp_async16(dst + at, from + el, ro < 0 ? 0 : 16);
-                        if constexpr (!SPLIT) cp_async16(dst + kHalf + at, vbase + el, ro < 0 ? 0 : 16);
+                for (int rg = 0; rg < WT / 8; ++rg) {
+                    const int64_t row = __shfl_sync(0xffffffffu, place, rg * 8 + rq);
+                    const int bytes = row < 0 ? 0 : 16;
+                    const int64_t el = (row < 0 ? 0 : row) + cq * 8;
+                    const uint32_t to = dst + rg / 2 * kBox + rg % 2 * 8 * part_elems(D) * 2;
+#pragma unroll
+                    for (int cg = 0; cg < CG; ++cg) {
+                        const uint32_t at = to + (CP2 == 4 ? cg / 2 : cg) * kPart + dst_at[CP2 == 4 ? cg % 2 : 0];
+                        cp_async16(at, from + el + cg * 32, bytes);
+                        if constexpr (!SPLIT) cp_async16(at + kHalf, vbase + el + cg * 32, bytes);
                     }
                 }
             }
@@ -432,7 +342,7 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
             }
             values = !values;
         }
-        if constexpr (!TILED) cp_commit();
+        cp_commit();
     };
     // lane constants of the operand reads: chunk 2k + hi of this lane's row, per k within a part
     int k_at[CP2], v_at[CP2];
@@ -458,7 +368,7 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     look_up();
     if (cc.tile < cc.stop) load_q();
 #pragma unroll
-    for (int s = 0; s < (TILED ? S : S - 1); ++s) load(s);
+    for (int s = 0; s < S - 1; ++s) load(s);
 
     // rows without tokens are zeros; rows whose place is out of range are counted
     for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -476,32 +386,14 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
     constexpr int QW = THIRD ? 6 : 4;  // words per k
     uint32_t qa[q_in_smem(D) ? 1 : KS / 2][2 * QW];
     int at_slot = 0, computed = 0;  // the ring's next slot, and the tiles of the run behind it
-    uint32_t phase = 0;             // bit s: parity of slot s's next completed copy
-    // The next slot, once its copy has landed (TILED: false if a bounded wait gave up).
-    auto arrive = [&](bool copied, int& cur) {
-        cur = at_slot;
+    // The next slot, its copies landed; the load that refills the one before it is started.
+    auto arrive = [&]() {
+        const int cur = at_slot;
         at_slot = at_slot + 1 == S ? 0 : at_slot + 1;
-        if constexpr (TILED) {
-            if (!copied) return true;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[warp][cur], (phase >> cur) & 1))) {
-                if (lane == 0) atomicAdd(p.err + 1, 1u);
-                failed = true;
-                return false;
-            }
-            phase ^= 1u << cur;
-            pending &= ~(1u << cur);
-        } else {
-            cp_wait<S - 2>();
-            __syncwarp();
-            load(cur == 0 ? S - 1 : cur - 1);  // the slot that is read
-        }
-        return true;
-    };
-    auto refill = [&](int cur) {
-        if constexpr (TILED) {
-            __syncwarp();  // every lane has read the slot
-            load(cur);
-        }
+        cp_wait<S - 2>();
+        __syncwarp();  // every lane's copies are in, and every lane has read the slot before
+        load(cur == 0 ? S - 1 : cur - 1);
+        return cur;
     };
     for (;;) {
         // ---- one item, or this run's piece of it: query heads h0..h0+nh of a row
@@ -558,18 +450,11 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
         float m = -INFINITY, l = 0.f;  // running maximum (scaled, less kShift) and this lane's part of the sum
 
         for (int t = 0; t < tiles; ++t) {
-            if (failed) continue;
             const uint32_t have = (full >> at_slot) & 1 ? kAll : sh.valid[warp][computed & 3];  // bit per token
             ++computed;
-            int cur;
-            if (!arrive(have != 0, cur)) continue;
-            uint32_t base = smem_u32(ring + cur * kSlot);
+            uint32_t base = smem_u32(ring + arrive() * kSlot);
             if (have == 0) {
-                refill(cur);
-                if constexpr (SPLIT) {
-                    arrive(false, cur);
-                    refill(cur);
-                }
+                if constexpr (SPLIT) arrive();
                 continue;
             }
 
@@ -605,7 +490,6 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
                         }
                     }
             }
-            if constexpr (SPLIT) refill(cur);
             float s[H][4];
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -654,25 +538,7 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
             l = fmaf(l, alpha, more);
 
             // ---- o = o * alpha + p . v
-            if constexpr (SPLIT) {
-                if (!arrive(true, cur)) continue;
-                base = smem_u32(ring + cur * kSlot);
-            } else {
-                base += kHalf;
-            }
-            if (TILED && have != kAll) {
-                // places behind the last token may hold anything, also NaN, and boxes without a page
-                // what was there before: their values are zeroed (their scores have been replaced)
-#pragma unroll
-                for (int n = 0; n < WT * C / 32; ++n) {
-                    const int i = n * 32 + lane, r = i / C;
-                    if (!((have >> r) & 1))
-                        *reinterpret_cast<uint4*>(ring + cur * kSlot + (SPLIT ? 0 : kHalf) + r / kBoxTok * kBox + chunk_at<D>(i % C, r % kBoxTok)) =
-                            make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-            }
+            base = SPLIT ? smem_u32(ring + arrive() * kSlot) : base + kHalf;
 #pragma unroll
             for (int c = 0; c < NT; c += 2) {
                 float d[2][4];
@@ -696,7 +562,6 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
                     o[c + j][1] = fmaf(o[c + j][1], alpha, d[j][1] + d[j][3]);
                 }
             }
-            refill(cur);
         }
 
         uint32_t c0 = cta, c1 = cta;
@@ -828,53 +693,17 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D))
         }
         if (!more) break;
     }
-    if constexpr (TILED) {
-        if (failed)  // copies in flight must not land after the CTA has gone
-            for (int i = 0; i < S; ++i)
-                if ((pending >> i) & 1) mbar_wait(&sh.full[warp][i], (phase >> i) & 1);
-    } else {
-        cp_wait<0>();
-    }
+    cp_wait<0>();
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static const EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-                       q == cudaDriverEntryPointSuccess
-                   ? reinterpret_cast<EncodeTiledFn>(p)
-                   : nullptr;
-    }();
-    return fn;
-}
-
-template <int D>
-bool encode(CUtensorMap* map, void* base, const KvCache& kv) {
-    constexpr int PE = part_elems(D);
-    // the stride of a dimension of size 1 is never used, but has to be a legal one
-    auto bytes = [](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride : (int64_t)D) * 2; };
-    const cuuint64_t dims[5] = {PE, (cuuint64_t)kv.page_size, D / PE, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_pages};
-    const cuuint64_t strides[4] = {(cuuint64_t)kv.token_stride * 2, PE * 2, bytes(kv.n_kv, kv.head_stride),
-                                   bytes(kv.n_pages, kv.page_stride)};
-    const cuuint32_t box[5] = {PE, kBoxTok, D / PE, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
-    return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       PE == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <int D, class T, bool TILED, bool PACK>
-cudaError_t launch_typed(AttnArgs a, const CUtensorMap (&maps)[2], int sms, bool pdl, cudaStream_t s) {
+template <int D, class T, bool PACK>
+cudaError_t launch_typed(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
     static bool configured[kMaxDevices] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices || !configured[dev]) {
-        e = cudaFuncSetAttribute(attention_kernel<D, T, TILED, PACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
+        e = cudaFuncSetAttribute(attention_kernel<D, T, PACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) configured[dev] = true;
     }
@@ -886,25 +715,14 @@ cudaError_t launch_typed(AttnArgs a, const CUtensorMap (&maps)[2], int sms, bool
     // us, 230 rows of 5 to 180 tokens 15.3 -> 12.5); with fewer items every cut is wanted (one
     // row of 1000 tokens and 8 k/v heads 9.3 us, with moved cuts 11.7).
     a.snap = 2 * items >= ctas ? 2 : 0;
-    return launch_kernel(attention_kernel<D, T, TILED, PACK>, dim3((unsigned)ctas), 32 * warps(D), smem_bytes(D), pdl, s, a, maps[0],
-                         maps[1]);
-}
-
-template <int D, bool TILED>
-cudaError_t launch_tiled(const AttnArgs& a, const CUtensorMap (&maps)[2], int sms, bool pdl, cudaStream_t s) {
-    if (a.kv.type != kKvBf16) return launch_typed<D, __half, TILED, false>(a, maps, sms, pdl, s);
-    return a.group <= 4 ? launch_typed<D, __nv_bfloat16, TILED, true>(a, maps, sms, pdl, s)
-                        : launch_typed<D, __nv_bfloat16, TILED, false>(a, maps, sms, pdl, s);
+    return launch_kernel(attention_kernel<D, T, PACK>, dim3((unsigned)ctas), 32 * warps(D), smem_bytes(D), pdl, s, a);
 }
 
 template <int D>
 cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
-    CUtensorMap maps[2] = {};
-    // strides of 2^40 bytes and more do not fit a tensor map
-    const bool fits = a.kv.token_stride < (1ll << 39) && a.kv.head_stride < (1ll << 39) && a.kv.page_stride < (1ll << 39);
-    if (a.kv.page_size % kBoxTok == 0 && fits && encode_fn() && encode<D>(&maps[0], a.kv.k, a.kv) && encode<D>(&maps[1], a.kv.v, a.kv))
-        return launch_tiled<D, true>(a, maps, sms, pdl, s);
-    return launch_tiled<D, false>(a, maps, sms, pdl, s);
+    if (a.kv.type != kKvBf16) return launch_typed<D, __half, false>(a, sms, pdl, s);
+    return a.group <= 4 ? launch_typed<D, __nv_bfloat16, true>(a, sms, pdl, s)
+                        : launch_typed<D, __nv_bfloat16, false>(a, sms, pdl, s);
 }
 
 }  // namespace

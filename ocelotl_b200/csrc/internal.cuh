@@ -162,7 +162,7 @@ cudaError_t launch_qk_norm_rope(const float* qkv, int64_t qkv_stride, int64_t ro
 
 // out f32 [rows, n_heads, head_dim]: attention of row r over tokens
 // 0..positions[r] of its sequence.  part / counters: workspace of the joined
-// lengths (attention_workspace_bytes; counters zero between launches).
+// lengths, of a fixed size for a GPU (counters zero between launches).
 size_t attention_part_bytes(int sms);
 size_t attention_counters(int sms);
 cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t rows, int64_t n_heads, const KvCache& kv,
