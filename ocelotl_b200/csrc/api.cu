@@ -1041,12 +1041,12 @@ int ocl_paged_attention(ocl_ctx* ctx, const float* q, size_t q_stride, size_t ro
     if (rows == 0) return OCL_OK;
     if (!q || !out) return fail(ctx, OCL_ERR_INVALID, "paged_attention q/out pointer is null");
     if (misaligned(q) || misaligned(out)) return fail(ctx, OCL_ERR_INVALID, "paged_attention q and out must be 16-byte aligned");
-    // the work split counts 64-token tiles of every row, k/v head and group of 8 query heads in 31 bits
+    // the work split counts 16-token tiles of every row, k/v head and group of 8 query heads in 31 bits
     const double tiles = (double)rows * cache->n_kv_heads * ((n_heads / cache->n_kv_heads + 7) / 8) *
-                         ((double)at->max_pages * cache->page_size / 64 + 2);
+                         ((double)at->max_pages * cache->page_size / 16 + 2);
     if (tiles > 2147483647.0)
         return fail(ctx, OCL_ERR_UNSUPPORTED, "unsupported feature `paged_attention size` (requested `%zu rows, %zu k/v heads, "
-                    "block table of %zu tokens`): supported = [rows * heads * tokens / 64 < 2^31]", rows, cache->n_kv_heads,
+                    "block table of %zu tokens`): supported = [rows * heads * tokens / 16 < 2^31]", rows, cache->n_kv_heads,
                     at->max_pages * cache->page_size);
     const size_t width = n_heads * cache->head_dim;
     if (overlap(q, q_stride, out, width, rows, width, width))

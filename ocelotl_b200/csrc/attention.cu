@@ -57,9 +57,11 @@ constexpr bool split_slots(int d) { return d == 256; }
 constexpr int warps(int d) { return d == 256 ? 8 : 4; }
 constexpr int max_warps = 8;
 constexpr int slots(int d) { return d == 96 ? 4 : 3; }
-constexpr int ctas_per_sm(int d) { return d == 64 ? 2 : 1; }
-constexpr int max_ctas_per_sm = 2;
-constexpr int tile_tok(int d) { return warps(d) * warp_tok(d); }
+// CTAs of w warps that an SM holds.  With one warp a CTA, items are not shared by warps
+// (many_items below).
+constexpr int ctas_per_sm(int d, int w) { return w > 1 ? (d == 64 ? 2 : 1) : d == 64 ? 8 : d == 256 ? 5 : 4; }
+constexpr int max_ctas_per_sm = 8;
+constexpr int tile_tok(int d, int w) { return w * warp_tok(d); }
 // A box of 16 tokens of k or v is kept as parts of 64 elements (32 for head_dim 96): a part is
 // 16 rows of 128 (64) bytes, its 16-byte chunks exclusive-or'ed with the row.
 constexpr int part_elems(int d) { return d % 64 == 0 ? 64 : 32; }
@@ -80,11 +82,12 @@ struct Shared {  // behind the ring, the merge buffer and the q fragments
     uint32_t valid[max_warps][4];  // a bit per token of a tile of the warp, by the tile's number in the run modulo 4
     float m[max_warps][kHeads], l[max_warps][kHeads];
 };
-constexpr int ring_bytes(int d) { return warps(d) * slots(d) * slot_bytes(d); }
-constexpr int merge_bytes(int d) { return warps(d) * kHeads * merge_cols(d) * 4; }
-constexpr int smem_bytes(int d) { return ring_bytes(d) + merge_bytes(d) + q_bytes(d) + (int)sizeof(Shared); }
-static_assert(smem_bytes(256) <= 227 * 1024 && smem_bytes(128) <= 227 * 1024 && smem_bytes(96) <= 227 * 1024 &&
-              2 * (smem_bytes(64) + 1024) <= 228 * 1024, "CTAs per SM");
+constexpr int ring_bytes(int d, int w) { return w * slots(d) * slot_bytes(d); }
+constexpr int merge_bytes(int d, int w) { return w * kHeads * merge_cols(d) * 4; }
+constexpr int smem_bytes(int d, int w) { return ring_bytes(d, w) + merge_bytes(d, w) + q_bytes(d) + (int)sizeof(Shared); }
+constexpr bool fits(int d, int w) { return ctas_per_sm(d, w) * (smem_bytes(d, w) + 1024) <= 228 * 1024; }
+static_assert(fits(64, 4) && fits(96, 4) && fits(128, 4) && fits(256, 8) && fits(64, 1) && fits(96, 1) && fits(128, 1) && fits(256, 1),
+              "CTAs per SM");
 
 struct AttnArgs {
     const float* q;
@@ -186,20 +189,20 @@ __device__ __forceinline__ int chunk_at(int c, int r) {
 // PACK (bf16, at most 4 heads): rows 0-3 leading pieces, 4-7 third, 8-11 second, so that
 // one MMA does what takes two with 8 heads; lanes 16-31 then hold the third pieces' part
 // of o.
-template <int D, class T, bool PACK>
-__global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D)) attention_kernel(const AttnArgs p) {
-    constexpr int kWarps = warps(D), kThreads = 32 * kWarps;
+template <int D, class T, bool PACK, int W>
+__global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(const AttnArgs p) {
+    constexpr int kWarps = W, kThreads = 32 * kWarps;
     constexpr int S = slots(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
-    constexpr int WT = warp_tok(D), TT = tile_tok(D), H = WT / kBoxTok;  // H boxes of 16 tokens a slot
+    constexpr int WT = warp_tok(D), TT = tile_tok(D, W), H = WT / kBoxTok;  // H boxes of 16 tokens a slot
     constexpr uint32_t kAll = 0xffffffffu >> (32 - WT);
     constexpr int kBox = box_bytes(D), kHalf = half_bytes(D), kSlot = slot_bytes(D), kPart = part_bytes(D);
     constexpr int CP2 = part_elems(D) / 16;
     constexpr bool SPLIT = split_slots(D);
     constexpr int MC = merge_cols(D), kRows = PACK ? 4 : kHeads;
     extern __shared__ __align__(1024) unsigned char smem[];
-    float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D));
-    uint4* q_frag = reinterpret_cast<uint4*>(smem + ring_bytes(D) + merge_bytes(D));
-    Shared& sh = *reinterpret_cast<Shared*>(smem + ring_bytes(D) + merge_bytes(D) + q_bytes(D));
+    float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D, W));
+    uint4* q_frag = reinterpret_cast<uint4*>(smem + ring_bytes(D, W) + merge_bytes(D, W));
+    Shared& sh = *reinterpret_cast<Shared*>(smem + ring_bytes(D, W) + merge_bytes(D, W) + q_bytes(D));
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int items = p.n_kv * p.head_groups;
@@ -207,11 +210,12 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D)) attention_kerne
 
     // ---- this CTA's run: the rows' units summed over the threads, then its two cuts
     // located, one by either half of the CTA (which both sum all rows)
-    constexpr int kHalfThreads = kThreads / 2, kHalfWarps = kWarps / 2;
+    constexpr int kSides = kWarps > 1 ? 2 : 1, kHalfThreads = kThreads / kSides, kHalfWarps = kWarps / kSides;
     const int side = warp / kHalfWarps, per = (p.rows + kHalfThreads - 1) / kHalfThreads;
     const int r0 = min(tid % kHalfThreads * per, p.rows), r1 = min(r0 + per, p.rows);
     uint32_t mine = 0, longest = 0;
     int first_tokens = 0;
+#pragma unroll 4
     for (int r = r0; r < r1; ++r) {
         const int tokens = row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
         if (r == r0) first_tokens = tokens;
@@ -240,8 +244,8 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D)) attention_kerne
     const Runs runs = runs_of(total, gridDim.x, max(1u, (uint32_t)(sqrtf(0.1f * (float)longest) + 0.999f)), p.snap);
     const uint32_t cta = blockIdx.x;
     const bool active = total > 0 && cta < runs.P;
-    {
-        const uint32_t cut = run_cut(runs, cta + side);
+    for (int i = side; i < 2; i += kSides) {
+        const uint32_t cut = run_cut(runs, cta + i);
         uint32_t at = upto - mine;
         if (active && cut >= at && cut < upto) {
             for (int r = r0;; ++r) {
@@ -249,8 +253,8 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D)) attention_kerne
                 const uint32_t all = tiles ? item_units(tiles) : 0, off = cut - at;
                 if (off < all * items) {
                     const uint32_t item = off / all, u = off - item * all, moved = moved_cut(runs, u, tiles);
-                    sh.edge[side] = cut - u + moved;
-                    if (side == 0) sh.first = {r, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
+                    sh.edge[i] = cut - u + moved;
+                    if (i == 0) sh.first = {r, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
                     break;
                 }
                 at += all * items;
@@ -696,33 +700,51 @@ __global__ void __launch_bounds__(32 * warps(D), ctas_per_sm(D)) attention_kerne
     cp_wait<0>();
 }
 
-template <int D, class T, bool PACK>
+template <int D, class T, bool PACK, int W>
 cudaError_t launch_typed(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
     static bool configured[kMaxDevices] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices || !configured[dev]) {
-        e = cudaFuncSetAttribute(attention_kernel<D, T, PACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D));
+        e = cudaFuncSetAttribute(attention_kernel<D, T, PACK, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D, W));
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) configured[dev] = true;
     }
-    const int64_t items = (int64_t)a.rows * a.n_kv * a.head_groups, tiles = items * tiles_of(a.cap, tile_tok(D));
+    const int64_t items = (int64_t)a.rows * a.n_kv * a.head_groups, tiles = items * tiles_of(a.cap, tile_tok(D, W));
     if (tiles + items > 0x7fffffff) return cudaErrorInvalidValue;  // the runs' arithmetic; checked by the caller
-    const int64_t most = (int64_t)sms * ctas_per_sm(D), ctas = tiles < most ? tiles : most;
+    const int64_t most = (int64_t)sms * ctas_per_sm(D, W), ctas = tiles < most ? tiles : most;
     // With about as many items as CTAs, a short item is better left whole than shared (its
     // join takes longer than its tiles: 16 rows of 555 tokens and 8 k/v heads 15.2 -> 11.1
     // us, 230 rows of 5 to 180 tokens 15.3 -> 12.5); with fewer items every cut is wanted (one
     // row of 1000 tokens and 8 k/v heads 9.3 us, with moved cuts 11.7).
     a.snap = 2 * items >= ctas ? 2 : 0;
-    return launch_kernel(attention_kernel<D, T, PACK>, dim3((unsigned)ctas), 32 * warps(D), smem_bytes(D), pdl, s, a);
+    return launch_kernel(attention_kernel<D, T, PACK, W>, dim3((unsigned)ctas), 32 * W, smem_bytes(D, W), pdl, s, a);
+}
+
+// Many items: one warp to each, so that short ones leave no warp idle and need no join of
+// warps.  Measured against the wide CTAs, us (k/v heads x rows, tokens):
+//   head_dim 128:  8 x 64, 10 11.2 -> 5.9, 100 12.8 -> 10.3, 2000 93 -> 94;  8 x 1000, 10 113 -> 47, 400 324 -> 277
+//                  8 x 32, 100 8.4 -> 14.5 (too few: what is not shared by warps is shared by CTAs)
+//   head_dim 64:   8 x 64, 100 7.6 -> 14.1;  8 x 128, 100 12.3 -> 9.1, 2000 91 -> 96
+//   head_dim 256:  4 x 128, 100 29.7 -> 25.2, 400 66 -> 63, 2000 189 -> 211
+// so at 64 and 256 only where the block table bounds the lengths.
+bool many_items(int d, int64_t items, int cap, int sms) {
+    if (d == 64) return items >= 6 * (int64_t)sms && cap <= 256;
+    return items >= 3 * (int64_t)sms && (d != 256 || cap <= 512);
+}
+
+template <int D, class T, bool PACK>
+cudaError_t launch_warps(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
+    if (many_items(D, (int64_t)a.rows * a.n_kv * a.head_groups, a.cap, sms)) return launch_typed<D, T, PACK, 1>(a, sms, pdl, s);
+    return launch_typed<D, T, PACK, warps(D)>(a, sms, pdl, s);
 }
 
 template <int D>
 cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
-    if (a.kv.type != kKvBf16) return launch_typed<D, __half, false>(a, sms, pdl, s);
-    return a.group <= 4 ? launch_typed<D, __nv_bfloat16, true>(a, sms, pdl, s)
-                        : launch_typed<D, __nv_bfloat16, false>(a, sms, pdl, s);
+    if (a.kv.type != kKvBf16) return launch_warps<D, __half, false>(a, sms, pdl, s);
+    return a.group <= 4 ? launch_warps<D, __nv_bfloat16, true>(a, sms, pdl, s)
+                        : launch_warps<D, __nv_bfloat16, false>(a, sms, pdl, s);
 }
 
 }  // namespace
@@ -730,8 +752,10 @@ cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
 size_t attention_part_bytes(int sms) {
     size_t most = 0;
     for (int d : {64, 96, 128, 256}) {
-        const size_t b = (size_t)sms * ctas_per_sm(d) * 2 * slot_floats(d) * 4;
-        most = b > most ? b : most;
+        for (int w : {1, warps(d)}) {
+            const size_t b = (size_t)sms * ctas_per_sm(d, w) * 2 * slot_floats(d) * 4;
+            most = b > most ? b : most;
+        }
     }
     return most;
 }

@@ -50,11 +50,13 @@ OCL_HD bool place_of(const int32_t* pages, int64_t max_pages, int64_t n_pages, c
 }
 
 // Tokens that a row sees: 0 for a padding row or one without a sequence, at most
-// `cap`, what a row of the block table can hold.
+// `cap`, what a row of the block table can hold.  Without branches, so that a thread's
+// loads of several rows are under way together.
 OCL_HD int row_tokens(const KvRows& at, int cap, int64_t row) {
     const int pos = at.positions[row];
-    if (pos < 0 || sequence_of(at, row) < 0) return 0;
-    return pos >= cap ? cap : pos + 1;
+    const bool there = pos >= 0 && sequence_of(at, row) >= 0;
+    const int seen = pos < cap ? pos : cap - 1;
+    return there ? seen + 1 : 0;
 }
 
 OCL_HD int tiles_of(int tokens, int tile_tok) { return (tokens + tile_tok - 1) / tile_tok; }

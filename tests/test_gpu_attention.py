@@ -78,6 +78,16 @@ def test_many_short_rows(backend):
     check(backend, [(i * 37) % 150 for i in range(400)], 2, 7, 64, 16, torch.float16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_many_items(backend, dim, dtype):
+    """Enough rows and heads that every warp takes items of its own; some rows long, some empty."""
+    lengths = [(i * 53) % 200 for i in range(240)]
+    check(backend, lengths, 8, 3, dim, 16, dtype, seed=dim)
+    if dim in (96, 128):
+        check(backend, [0, 3000, 1] + lengths, 8, 6, dim, 24, dtype, seed=dim)
+
+
 @pytest.mark.parametrize("scale,sharp", [(1e-6, 1.0), (1.0, 1.0), (0.0884, 8.0)])
 def test_flat_and_peaked_weights(backend, scale, sharp):
     for dtype in (torch.bfloat16, torch.float16):
