@@ -447,8 +447,12 @@ class CudaKernelBackend:
                  dtype: torch.dtype = torch.bfloat16) -> PagedKvCache:
         """A zeroed paged cache of one layer: k and v [n_pages, n_kv_heads, page_size, head_dim]."""
         shape = (n_pages, n_kv_heads, page_size, head_dim)
-        return PagedKvCache(torch.zeros(shape, dtype=dtype, device=self.torch_device),
-                            torch.zeros(shape, dtype=dtype, device=self.torch_device))
+        with self._kernel_stream():  # the zeros come before what the kernels write
+            kernels = torch.cuda.current_stream(self.torch_device)
+            cache = PagedKvCache(torch.zeros(shape, dtype=dtype, device=self.torch_device),
+                                 torch.zeros(shape, dtype=dtype, device=self.torch_device))
+        torch.cuda.current_stream(self.torch_device).wait_stream(kernels)  # and before what the caller writes
+        return cache
 
     def kv_cache_view(self, k: torch.Tensor, v: torch.Tensor) -> PagedKvCache:
         """A cache over existing tensors [n_pages, n_kv_heads, page_size, head_dim], of any page and token strides."""
@@ -476,16 +480,19 @@ class CudaKernelBackend:
         """The rules of a batch of requests (see LogitRules), as process_logits and greedy_sample take them."""
         return LogitRules(self.torch_device, **parts)
 
+    def _kernel_stream(self):
+        """torch's context of the stream that the kernels run on."""
+        s = self._stream
+        return torch.cuda.stream(torch.cuda.default_stream(self.torch_device) if s == 0 else
+                                 torch.cuda.ExternalStream(s, device=self.torch_device))
+
     def _alloc(self, like: torch.Tensor, *shape: int, dtype: torch.dtype | None = None) -> torch.Tensor:
         """Device memory for an output, allocated on the stream that the kernels run on."""
-        s = self._stream
-        if _raw_stream(self.device_index) == s:
+        if _raw_stream(self.device_index) == self._stream:
             if dtype is None:
                 return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(*shape)
             return torch.empty(shape, dtype=dtype, device=self.torch_device)
-        stream = torch.cuda.default_stream(self.torch_device) if s == 0 else \
-            torch.cuda.ExternalStream(s, device=self.torch_device)
-        with torch.cuda.stream(stream):
+        with self._kernel_stream():
             return torch.empty(shape, dtype=dtype or like.dtype, device=self.torch_device)
 
     def _out(self, out, like: torch.Tensor, op: str, *shape: int) -> torch.Tensor:

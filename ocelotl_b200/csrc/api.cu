@@ -977,6 +977,7 @@ int ocl_rope_create(ocl_ctx* ctx, size_t rot_dim, double base, const float* fact
     r->interleaved = interleaved != 0;
     cudaError_t e = cudaMalloc((void**)&r->steps, sizeof steps);
     if (e == cudaSuccess) e = cudaMemcpy(r->steps, steps, rot_dim / 2 * sizeof steps[0], cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // in place for calls on any stream
     if (e != cudaSuccess) {
         if (r->steps) cudaFree(r->steps);
         delete r;

@@ -18,6 +18,10 @@
 //
 // The greedy pick is argmax.cu's: one 64-bit key per run, the last run of a row
 // writes the id.
+//
+// Measured in a graph: 190 rows of 151936 (histories up to 8000, 40 biases, masks, pick) 72 us
+// = 3.2 TB/s of logits, of which the history's second and later reads take 15, the pick 8 and
+// biases and masks 7; one row of 128256 4.1 us.
 #include "device.cuh"
 #include "internal.cuh"
 

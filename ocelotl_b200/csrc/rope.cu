@@ -15,6 +15,10 @@
 //
 // One warp per head, one or more CTAs per row (the host splits the heads of few
 // rows over CTAs); the row's cos and sin are computed once per CTA.
+//
+// Bound: the floats in and out and the cache's bytes, HBM where rows are many; few rows are
+// the launch and three dependent loads (position, table, head).  Measured in a graph (32 + 8
+// heads of 128): 8190 rows 62 us = 5.9 TB/s, one row 1.7 us.
 #include "device.cuh"
 #include "internal.cuh"
 

@@ -194,3 +194,25 @@ def test_two_contexts_on_two_streams(backend):
                 got.append(b.paged_attention(q, cache, pos, table))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("busy", ["current", "kernels"])
+def test_new_cache_is_zeroed_before_either_stream_writes(busy):
+    """kv_cache's zeros precede the kernels' writes and the caller's, whichever stream is behind."""
+    from ocelotl_b200 import CudaKernelBackend
+    b, side = CudaKernelBackend(0), torch.cuda.Stream()
+    qkv, pos = torch.ones(1, 3 * 64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    b.set_stream(side)
+    b.qk_norm_rope(qkv, b.kv_cache(1, 16, 1, 64), pos, table, None)  # modules are loaded
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side if busy == "kernels" else torch.cuda.current_stream()):
+        torch.cuda._sleep(50_000_000)  # some 30 ms
+    cache = b.kv_cache(1, 16, 1, 64)
+    if busy == "kernels":
+        cache.k.fill_(1.0)
+        cache.v.fill_(1.0)
+    else:
+        b.qk_norm_rope(qkv, cache, pos, table, None)
+    torch.cuda.synchronize()
+    assert (cache.k[0, 0, 0] == 1).all() and (cache.v[0, 0, 0] == 1).all()
