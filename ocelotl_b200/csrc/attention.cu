@@ -33,6 +33,8 @@
 //
 // Measured (bf16, 8 k/v heads, head_dim 128, a pass among others): 61 rows of 70 to 16000 tokens,
 // 4 heads each, 130 us = 6.1 TB/s; one row of 131000 tokens 91 us = 5.9 TB/s.
+#include <type_traits>
+
 #include "device.cuh"
 #include "internal.cuh"
 
@@ -43,6 +45,12 @@ namespace {
 constexpr int kHeads = 8;   // query heads of one k/v head worked on together
 constexpr int kBoxTok = 16; // tokens kept together: those of one p.v MMA
 
+// How the 8 rows of a piece's MMA rows are used:
+enum Mode {
+    kPlain,   // the query heads of a row (kHeads at a time)
+    kPacked,  // bf16, at most 4 of them: two pieces side by side
+    kShared,  // those of several rows of one sequence: 8, 4 or 2 rows of 1, 2 or 4 heads
+};
 // Tokens a warp takes at a time.  32 halve the work a token costs besides its MMAs
 // (maximum, rescaling, waits, look-ups) and give a warp twice the independent MMAs; at
 // head_dim 256 they would not leave three slots to each of 8 warps.
@@ -55,7 +63,6 @@ constexpr int warp_tok(int d) { return d == 256 ? 16 : 32; }
 // eight; at head_dim 128 both changes lose: 64 ragged rows 123 us, 143 and 129).
 constexpr bool split_slots(int d) { return d == 256; }
 constexpr int warps(int d) { return d == 256 ? 8 : 4; }
-constexpr int max_warps = 8;
 constexpr int slots(int d) { return d == 96 ? 4 : 3; }
 // CTAs of w warps that an SM holds.  With one warp a CTA, items are not shared by warps
 // (many_items below).
@@ -74,17 +81,19 @@ constexpr bool q_in_smem(int d) { return d > 128; }
 constexpr int q_bytes(int d) { return q_in_smem(d) ? d / 16 * 32 * 24 : 0; }
 constexpr int slot_floats(int d) { return kHeads * d + 2 * kHeads; }
 
+template <int W>
 struct Shared {  // behind the ring, the merge buffer and the q fragments
-    uint32_t scan[max_warps], longest[max_warps];
+    uint32_t scan[W], longest[W];
     Cursor first;
     uint32_t edge[2];
     int last_in;
-    uint32_t valid[max_warps][4];  // a bit per token of a tile of the warp, by the tile's number in the run modulo 4
-    float m[max_warps][kHeads], l[max_warps][kHeads];
+    uint32_t valid[W][4];  // a bit per token of a tile of the warp, by the tile's number in the run modulo 4
+    float m[W][kHeads], l[W][kHeads], top[W][kHeads];
 };
 constexpr int ring_bytes(int d, int w) { return w * slots(d) * slot_bytes(d); }
 constexpr int merge_bytes(int d, int w) { return w * kHeads * merge_cols(d) * 4; }
-constexpr int smem_bytes(int d, int w) { return ring_bytes(d, w) + merge_bytes(d, w) + q_bytes(d) + (int)sizeof(Shared); }
+constexpr int shared_bytes(int w) { return (int)(w == 8 ? sizeof(Shared<8>) : w == 4 ? sizeof(Shared<4>) : sizeof(Shared<1>)); }
+constexpr int smem_bytes(int d, int w) { return ring_bytes(d, w) + merge_bytes(d, w) + q_bytes(d) + shared_bytes(w); }
 constexpr bool fits(int d, int w) { return ctas_per_sm(d, w) * (smem_bytes(d, w) + 1024) <= 228 * 1024; }
 static_assert(fits(64, 4) && fits(96, 4) && fits(128, 4) && fits(256, 8) && fits(64, 1) && fits(96, 1) && fits(128, 1) && fits(256, 1),
               "CTAs per SM");
@@ -99,6 +108,7 @@ struct AttnArgs {
     int cap;      // tokens a row of the block table can hold
     float scale;  // in units of log2
     int snap;     // tiles that a cut moves at most to reach an item's edge
+    int head_shift;  // kShared: query heads of a row, as a power of two
     float* out;
     float* part;
     unsigned int* counters;
@@ -177,6 +187,15 @@ __device__ __forceinline__ void cut(uint32_t (&w)[N], float a, float b) {
     }
 }
 
+// Whether one of eight 16-bit elements is an infinity or a NaN.
+template <class T>
+__device__ __forceinline__ bool not_finite(uint4 w, T) {
+    constexpr uint32_t kLow = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u, kHigh = kLow << 16;
+    bool odd = false;
+    for (const uint32_t x : {w.x, w.y, w.z, w.w}) odd |= (x & kLow) == kLow || (x & kHigh) == kHigh;
+    return odd;
+}
+
 // Byte offset, within the k (or v) half of a stage, of 16-byte chunk `c` of row `r`:
 // 8 rows of one chunk column (an ldmatrix) fall into different banks.
 template <int D>
@@ -189,20 +208,31 @@ __device__ __forceinline__ int chunk_at(int c, int r) {
 // PACK (bf16, at most 4 heads): rows 0-3 leading pieces, 4-7 third, 8-11 second, so that
 // one MMA does what takes two with 8 heads; lanes 16-31 then hold the third pieces' part
 // of o.
-template <int D, class T, bool PACK, int W>
+//
+// SHARE: an item has several rows of one sequence, which read its tokens together: from
+// shared memory, the L2 and HBM once for all of them.  Each row has its own length; in the
+// tiles where one ends, its scores are masked, and values that it does not see are zeroed
+// in shared memory before its p.v (0 * NaN would not be 0), longest row first.
+template <int D, class T, int MODE, int W>
 __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(const AttnArgs p) {
     constexpr int kWarps = W, kThreads = 32 * kWarps;
+    constexpr bool PACK = MODE == kPacked, SHARE = MODE == kShared;
     constexpr int S = slots(D), KS = D / 16, NT = D / 8, C = D / 8, N = kPieces<T>;
     constexpr int WT = warp_tok(D), TT = tile_tok(D, W), H = WT / kBoxTok;  // H boxes of 16 tokens a slot
     constexpr uint32_t kAll = 0xffffffffu >> (32 - WT);
     constexpr int kBox = box_bytes(D), kHalf = half_bytes(D), kSlot = slot_bytes(D), kPart = part_bytes(D);
     constexpr int CP2 = part_elems(D) / 16;
-    constexpr bool SPLIT = split_slots(D);
+    constexpr bool SPLIT = split_slots(D), QS = q_in_smem(D);
     constexpr int MC = merge_cols(D), kRows = PACK ? 4 : kHeads;
+    constexpr bool THIRD = N == 3 && !PACK;               // third pieces of two k steps in one fragment
+    constexpr int QV = THIRD ? 3 : 2;                     // 16-byte vectors of q's pieces per two k steps
+    constexpr int XP = QS ? KS / 2 / kWarps : KS / 2;     // pairs of k steps that a warp cuts up
+    static_assert(!QS || KS / 2 % kWarps == 0, "pairs of k steps by warp");
     extern __shared__ __align__(1024) unsigned char smem[];
     float* merge_o = reinterpret_cast<float*>(smem + ring_bytes(D, W));
     uint4* q_frag = reinterpret_cast<uint4*>(smem + ring_bytes(D, W) + merge_bytes(D, W));
-    Shared& sh = *reinterpret_cast<Shared*>(smem + ring_bytes(D, W) + merge_bytes(D, W) + q_bytes(D));
+    using Sh = Shared<W>;
+    Sh& sh = *reinterpret_cast<Sh*>(smem + ring_bytes(D, W) + merge_bytes(D, W) + q_bytes(D));
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int items = p.n_kv * p.head_groups;
@@ -211,16 +241,35 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
     // ---- this CTA's run: the rows' units summed over the threads, then its two cuts
     // located, one by either half of the CTA (which both sum all rows)
     constexpr int kSides = kWarps > 1 ? 2 : 1, kHalfThreads = kThreads / kSides, kHalfWarps = kWarps / kSides;
-    const int side = warp / kHalfWarps, per = (p.rows + kHalfThreads - 1) / kHalfThreads;
+    const int side = warp / kHalfWarps, most = (p.rows + kHalfThreads - 1) / kHalfThreads;
+    const int per = SHARE ? (most + p.at.together - 1) & -p.at.together : most;
     const int r0 = min(tid % kHalfThreads * per, p.rows), r1 = min(r0 + per, p.rows);
     uint32_t mine = 0, longest = 0;
     int first_tokens = 0;
+    if constexpr (!SHARE) {
 #pragma unroll 4
-    for (int r = r0; r < r1; ++r) {
-        const int tokens = row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
-        if (r == r0) first_tokens = tokens;
-        if (tiles) mine += item_units(tiles);
-        longest = max(longest, (uint32_t)tiles);
+        for (int r = r0; r < r1; ++r) {
+            const int tokens = row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
+            if (r == r0) first_tokens = tokens;
+            if (tiles) mine += item_units(tiles);
+            longest = max(longest, (uint32_t)tiles);
+        }
+    } else {
+        int seq = 0, tokens = 0;  // of the item so far
+        auto item_ends = [&]() {
+            const int tiles = tiles_of(tokens, TT);
+            if (tiles) mine += item_units(tiles);
+            longest = max(longest, (uint32_t)tiles);
+            tokens = 0;
+        };
+#pragma unroll 4
+        for (int r = r0; r < r1; ++r) {
+            const int n = row_tokens(p.at, p.cap, r), of = p.at.seqs[r];
+            if ((r & (p.at.together - 1)) == 0 || of != seq) item_ends();
+            tokens = max(tokens, n);
+            seq = of;
+        }
+        item_ends();
     }
     mine *= items;
     longest = __reduce_max_sync(0xffffffffu, longest);
@@ -248,16 +297,19 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         const uint32_t cut = run_cut(runs, cta + i);
         uint32_t at = upto - mine;
         if (active && cut >= at && cut < upto) {
-            for (int r = r0;; ++r) {
-                const int tokens = r == r0 ? first_tokens : row_tokens(p.at, p.cap, r), tiles = tiles_of(tokens, TT);
+            for (int r = r0;;) {
+                int next = r + 1;
+                const int tokens = SHARE ? item_tokens(p.at, p.cap, p.rows, r, next) : r == r0 ? first_tokens : row_tokens(p.at, p.cap, r);
+                const int tiles = tiles_of(tokens, TT);
                 const uint32_t all = tiles ? item_units(tiles) : 0, off = cut - at;
                 if (off < all * items) {
                     const uint32_t item = off / all, u = off - item * all, moved = moved_cut(runs, u, tiles);
                     sh.edge[i] = cut - u + moved;
-                    if (i == 0) sh.first = {r, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
+                    if (i == 0) sh.first = {r, next, (int)item, tokens, tiles, moved ? (int)moved - kItemCost : 0, 0, cut - u};
                     break;
                 }
                 at += all * items;
+                r = next;
             }
         }
     }
@@ -356,17 +408,29 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         v_at[k] = chunk_at<D>(2 * k + (lane >> 4), lane & 15);
     }
 
-    // q of the query heads of the item at `cc`, f32: loaded ahead of its use
-    float2 x[KS][2];
+    // q of the query heads of the item at `cc`, f32: loaded ahead of its use, with what each
+    // of its rows sees.  With the fragments in shared memory a warp has only those k steps
+    // that it cuts up.
+    float2 x[XP][2][2];
+    int sees = 0, least = 0;  // tokens that the row of this lane's q sees, and the fewest that one of the rows sees
     auto load_q = [&]() {
         const int kvh = p.head_groups == 1 ? cc.item : cc.item / p.head_groups, hg = cc.item - kvh * p.head_groups;
-        const int nh = min(kHeads, p.group - hg * kHeads), hq = PACK ? g & 3 : g;
-        const float* qr = p.q + (int64_t)cc.row * p.q_stride + (int64_t)(kvh * p.group + hg * kHeads + hq) * D + c4 * 2;
+        const int nh = min(kHeads, p.group - hg * kHeads);
+        const int member = SHARE ? g >> p.head_shift : 0, hq = SHARE ? g & ((1 << p.head_shift) - 1) : PACK ? g & 3 : g;
+        const bool used = hq < nh && (!SHARE || member < cc.next - cc.row);
+        const float* qr = p.q + (int64_t)(cc.row + member) * p.q_stride + (int64_t)(kvh * p.group + hg * kHeads + hq) * D + c4 * 2;
+        if constexpr (SHARE) {
+            sees = used ? row_tokens(p.at, p.cap, cc.row + member) : 0;
+            least = __reduce_min_sync(0xffffffffu, used ? sees : 0x7fffffff);
+        }
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int i = 0; i < XP; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                x[k][j] = hq < nh ? *reinterpret_cast<const float2*>(qr + k * 16 + j * 8) : make_float2(0.f, 0.f);
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    x[i][k][j] = used ? *reinterpret_cast<const float2*>(qr + (2 * (QS ? i * kWarps + warp : i) + k) * 16 + j * 8)
+                                      : make_float2(0.f, 0.f);
     };
 
     look_up();
@@ -386,9 +450,7 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
     // A fragments of q: [k][0..3] = rows g, g + 8 at (k = 2c, 2c+1), then at (2c+8, 2c+9).  The
     // third pieces of two k steps share one fragment, in rows 0-7 and 8-15: each step's MMA
     // reads its own half of the result.
-    constexpr bool THIRD = N == 3 && !PACK;
-    constexpr int QW = THIRD ? 6 : 4;  // words per k
-    uint32_t qa[q_in_smem(D) ? 1 : KS / 2][2 * QW];
+    uint32_t qa[QS ? 1 : KS / 2][4 * QV];
     int at_slot = 0, computed = 0;  // the ring's next slot, and the tiles of the run behind it
     // The next slot, its copies landed; the load that refills the one before it is started.
     auto arrive = [&]() {
@@ -404,46 +466,52 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         const int row = cc.row, tiles = cc.stop - cc.tile;
         const bool whole = tiles == cc.tiles;
         const int kvh = p.head_groups == 1 ? cc.item : cc.item / p.head_groups, hg = cc.item - kvh * p.head_groups;
-        const int h0 = kvh * p.group + hg * kHeads, nh = min(kHeads, p.group - hg * kHeads);
+        const int h0 = kvh * p.group + hg * kHeads, nh = min(kHeads, p.group - hg * kHeads), item_rows = cc.next - cc.row;
         float scale = p.scale;
-        {
-            if constexpr (N == 2) {
-                // f16 pieces: bring the head's largest |q| into [2^7, 2^8)
-                float top = 0.f;
+        if constexpr (N == 2) {
+            // f16 pieces: bring the head's largest |q| into [2^7, 2^8)
+            float top = 0.f;
 #pragma unroll
-                for (int k = 0; k < KS; ++k)
+            for (int i = 0; i < XP; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = max(-126, min(126, 134 - (int)((__float_as_uint(top) >> 23) & 255)));
-                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-                scale *= __uint_as_float((uint32_t)(127 - e) << 23);
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int k = 0; k < KS; ++k)
+                    for (int j = 0; j < 2; ++j) top = fmaxf(top, fmaxf(fabsf(x[i][k][j].x), fabsf(x[i][k][j].y)));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if constexpr (QS && kWarps > 1) {
+                if (c4 == 0) sh.top[warp][g] = top;
+                __syncthreads();
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) x[k][j].x *= up, x[k][j].y *= up;
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.top[w][g]);
             }
+            const int e = max(-126, min(126, 134 - (int)((__float_as_uint(top) >> 23) & 255)));
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+            scale *= __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-            for (int k = 0; k < KS; k += 2) {
-                uint32_t f[2 * QW];
+            for (int i = 0; i < XP; ++i)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t w[2][N];
-                    cut<N, T>(w[0], x[k + i][0].x, x[k + i][0].y);
-                    cut<N, T>(w[1], x[k + i][1].x, x[k + i][1].y);
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        f[4 * i + 2 * j] = PACK && g >= 4 ? w[j][N - 1] : w[j][0];
-                        f[4 * i + 2 * j + 1] = PACK && g >= 4 ? 0u : w[j][1];
-                        if constexpr (THIRD) f[8 + 2 * j + i] = w[j][2];
-                    }
+                    for (int j = 0; j < 2; ++j) x[i][k][j].x *= up, x[i][k][j].y *= up;
+        }
+#pragma unroll
+        for (int i = 0; i < XP; ++i) {
+            uint32_t f[4 * QV];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t w[N];
+                    cut<N, T>(w, x[i][k][j].x, x[i][k][j].y);
+                    f[4 * k + 2 * j] = PACK && g >= 4 ? w[N - 1] : w[0];
+                    f[4 * k + 2 * j + 1] = PACK && g >= 4 ? 0u : w[1];
+                    if constexpr (THIRD) f[8 + 2 * j + k] = w[2];
                 }
 #pragma unroll
-                for (int i = 0; i < 2 * QW; i += 4) {
-                    if constexpr (!q_in_smem(D)) qa[k / 2][i] = f[i], qa[k / 2][i + 1] = f[i + 1], qa[k / 2][i + 2] = f[i + 2], qa[k / 2][i + 3] = f[i + 3];
-                    else if (k / 2 % kWarps == warp) q_frag[(k / 2 * QW / 2 + i / 4) * 32 + lane] = make_uint4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-                }
+            for (int v = 0; v < QV; ++v) {
+                if constexpr (QS) q_frag[((i * kWarps + warp) * QV + v) * 32 + lane] = make_uint4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
+                else qa[i][4 * v] = f[4 * v], qa[i][4 * v + 1] = f[4 * v + 1], qa[i][4 * v + 2] = f[4 * v + 2], qa[i][4 * v + 3] = f[4 * v + 3];
             }
         }
         __syncthreads();  // q_frag is written; the previous item's merge buffers are read
@@ -461,21 +529,23 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                 if constexpr (SPLIT) arrive();
                 continue;
             }
+            const int t0 = (cc.tile + t) * TT + warp * WT;  // the first token
+            const bool ragged = SHARE && t0 + WT > least;   // one of the rows ends in these
 
             // ---- s = q . k: two 8-token MMA columns a box
             float acc[H][2][2][4], low[H][2][2][4];
 #pragma unroll
             for (int k = 0; k < KS; k += 2) {
-                uint32_t a[2 * QW];
-                if constexpr (q_in_smem(D)) {
+                uint32_t a[4 * QV];
+                if constexpr (QS) {
 #pragma unroll
-                    for (int i = 0; i < 2 * QW; i += 4) {
-                        const uint4 f = q_frag[(k / 2 * QW / 2 + i / 4) * 32 + lane];
-                        a[i] = f.x, a[i + 1] = f.y, a[i + 2] = f.z, a[i + 3] = f.w;
+                    for (int v = 0; v < QV; ++v) {
+                        const uint4 f = q_frag[(k / 2 * QV + v) * 32 + lane];
+                        a[4 * v] = f.x, a[4 * v + 1] = f.y, a[4 * v + 2] = f.z, a[4 * v + 3] = f.w;
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 2 * QW; ++i) a[i] = qa[k / 2][i];
+                    for (int i = 0; i < 4 * QV; ++i) a[i] = qa[k / 2][i];
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -505,12 +575,14 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                     s[h][i] += acc[h][j][0][e] + acc[h][j][1][e];
                     if constexpr (PACK) s[h][i] += __shfl_xor_sync(0xffffffffu, s[h][i], 16);
                 }
-            if (have != kAll) {
+            if (have != kAll || ragged) {
 #pragma unroll
                 for (int h = 0; h < H; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!((have >> (16 * h + 8 * (i >> 1) + 2 * c4 + (i & 1))) & 1)) s[h][i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i) {
+                        const int tok = 16 * h + 8 * (i >> 1) + 2 * c4 + (i & 1);
+                        if (!((have >> tok) & 1) || (SHARE && t0 + tok >= sees)) s[h][i] = -INFINITY;
+                    }
             }
             float top = -INFINITY;
 #pragma unroll
@@ -541,29 +613,60 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
             }
             l = fmaf(l, alpha, more);
 
-            // ---- o = o * alpha + p . v
-            base = SPLIT ? smem_u32(ring + arrive() * kSlot) : base + kHalf;
+            // ---- o = o * alpha + p . v; with `some` for the rows that see `only` of these tokens
+            const uint32_t v_at_slot = SPLIT ? arrive() * kSlot : base - smem_u32(ring) + kHalf;
+            base = smem_u32(ring) + v_at_slot;
+            auto add_values = [&](auto some, int only) {
+                const bool mine = !decltype(some)::value || min(sees - t0, WT) == only;
 #pragma unroll
-            for (int c = 0; c < NT; c += 2) {
-                float d[2][4];
+                for (int c = 0; c < NT; c += 2) {
+                    float d[2][4];
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    uint32_t b[4];
-                    ldmatrix4_t(b, base + h * kBox + c / 2 / CP2 * kPart + v_at[c / 2 % CP2]);
+                    for (int h = 0; h < H; ++h) {
+                        uint32_t b[4];
+                        ldmatrix4_t(b, base + h * kBox + c / 2 / CP2 * kPart + v_at[c / 2 % CP2]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if constexpr (THIRD) {
-                            if (h == 0) mma0(d[j], pa[h][0][2], 0u, pa[h][1][2], 0u, b[2 * j], b[2 * j + 1], T());
-                            else mma(d[j], pa[h][0][2], 0u, pa[h][1][2], 0u, b[2 * j], b[2 * j + 1], T());
+                        for (int j = 0; j < 2; ++j) {
+                            if constexpr (THIRD) {
+                                if (h == 0) mma0(d[j], pa[h][0][2], 0u, pa[h][1][2], 0u, b[2 * j], b[2 * j + 1], T());
+                                else mma(d[j], pa[h][0][2], 0u, pa[h][1][2], 0u, b[2 * j], b[2 * j + 1], T());
+                            }
+                            if (h == 0 && !THIRD) mma0(d[j], pa[h][0][0], pa[h][0][1], pa[h][1][0], pa[h][1][1], b[2 * j], b[2 * j + 1], T());
+                            else mma(d[j], pa[h][0][0], pa[h][0][1], pa[h][1][0], pa[h][1][1], b[2 * j], b[2 * j + 1], T());
                         }
-                        if (h == 0 && !THIRD) mma0(d[j], pa[h][0][0], pa[h][0][1], pa[h][1][0], pa[h][1][1], b[2 * j], b[2 * j + 1], T());
-                        else mma(d[j], pa[h][0][0], pa[h][0][1], pa[h][1][0], pa[h][1][1], b[2 * j], b[2 * j + 1], T());
                     }
-                }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    o[c + j][0] = fmaf(o[c + j][0], alpha, d[j][0] + d[j][2]);
-                    o[c + j][1] = fmaf(o[c + j][1], alpha, d[j][1] + d[j][3]);
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (mine) o[c + j][e] = fmaf(o[c + j][e], alpha, d[j][e] + d[j][e + 2]);
+                }
+            };
+            if constexpr (!SHARE) {
+                add_values(std::false_type(), 0);
+            } else {
+                // Weights of 0 leave out what a row does not see, but for infinities and NaN.
+                const int first = max(0, least - t0);
+                unsigned char* const v_rows = ring + v_at_slot;
+                auto value_at = [&](int i) {  // i-th 16 bytes of the rows that not all see
+                    const int tok = first + i / C;
+                    return reinterpret_cast<uint4*>(v_rows + tok / kBoxTok * kBox + chunk_at<D>(i % C, tok % kBoxTok));
+                };
+                bool odd = false;
+                if (ragged)
+                    for (int i = lane; i < (WT - first) * C; i += 32) odd |= not_finite(*value_at(i), T());
+                if (!__any_sync(0xffffffffu, odd)) {
+                    add_values(std::false_type(), 0);
+                } else {
+                    // the rows that see most of these tokens first; then the values that no other sees are zeroed
+                    const int n = min(sees - t0, WT);
+                    for (int only = __reduce_max_sync(0xffffffffu, n); only > 0;) {
+                        add_values(std::true_type(), only);
+                        __syncwarp();
+                        only = __reduce_max_sync(0xffffffffu, n < only ? n : 0);
+                        for (int i = lane + max(0, only - first) * C; i < (WT - first) * C; i += 32) *value_at(i) = make_uint4(0, 0, 0, 0);
+                        __syncwarp();
+                    }
                 }
             }
         }
@@ -578,6 +681,12 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (c4 == 0) sh.m[warp][g] = m, sh.l[warp][g] = l;
+        // the row (from the item's first on) and query head that MMA row h holds; false: none
+        auto holds = [&](int h, int& member, int& head) {
+            member = SHARE ? h >> p.head_shift : 0;
+            head = SHARE ? h & ((1 << p.head_shift) - 1) : h;
+            return head < nh && (!SHARE || member < item_rows);
+        };
         float* slot = p.part + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * slot_floats(D);
 #pragma unroll
         for (int col0 = 0; col0 < D; col0 += MC) {
@@ -608,10 +717,11 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                     sum += sh.l[w][h] * f;
                     a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
                 }
-                if (h >= nh) continue;
+                int member, head;
+                if (!holds(h, member, head)) continue;
                 if (whole) {
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    *reinterpret_cast<float4*>(p.out + ((int64_t)row * p.n_heads + h0 + h) * D + col0 + col) =
+                    *reinterpret_cast<float4*>(p.out + ((int64_t)(row + member) * p.n_heads + h0 + head) * D + col0 + col) =
                         make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
                 } else {
                     __stcg(reinterpret_cast<float4*>(slot + h * D + col0 + col), a);
@@ -641,7 +751,9 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                 auto part_of = [&](int i) { return i == 0 ? first : rest + (size_t)(2 * i) * slot_floats(D); };
                 constexpr int V = D % 128 == 0 ? 4 : D == 64 ? 2 : 1, L = D / (32 * V);  // floats a load, loads a lane
                 constexpr int B = 16 / L;
-                for (int h = warp; h < nh; h += kWarps) {
+                for (int h = warp; h < kRows; h += kWarps) {
+                    int member, head;
+                    if (!holds(h, member, head)) continue;
                     float top = -INFINITY, sum = 0.f, acc[L][V] = {};
                     for (int i0 = 0; i0 < parts; i0 += 32) {
                         float m_i = -INFINITY, l_i = 0.f;
@@ -687,7 +799,7 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
 #pragma unroll
                     for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    float* to = p.out + ((int64_t)row * p.n_heads + h0 + h) * D + lane * V;
+                    float* to = p.out + ((int64_t)(row + member) * p.n_heads + h0 + head) * D + lane * V;
 #pragma unroll
                     for (int j = 0; j < L; ++j)
 #pragma unroll
@@ -700,14 +812,15 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
     cp_wait<0>();
 }
 
-template <int D, class T, bool PACK, int W>
+template <int D, class T, int MODE, int W>
 cudaError_t launch_typed(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
+    constexpr int kSmem = smem_bytes(D, W);
     static bool configured[kMaxDevices] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= kMaxDevices || !configured[dev]) {
-        e = cudaFuncSetAttribute(attention_kernel<D, T, PACK, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(D, W));
+        e = cudaFuncSetAttribute(attention_kernel<D, T, MODE, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return e;
         if (dev < kMaxDevices) configured[dev] = true;
     }
@@ -718,8 +831,8 @@ cudaError_t launch_typed(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
     // join takes longer than its tiles: 16 rows of 555 tokens and 8 k/v heads 15.2 -> 11.1
     // us, 230 rows of 5 to 180 tokens 15.3 -> 12.5); with fewer items every cut is wanted (one
     // row of 1000 tokens and 8 k/v heads 9.3 us, with moved cuts 11.7).
-    a.snap = 2 * items >= ctas ? 2 : 0;
-    return launch_kernel(attention_kernel<D, T, PACK, W>, dim3((unsigned)ctas), 32 * W, smem_bytes(D, W), pdl, s, a);
+    a.snap = 2 * (items / a.at.together) >= ctas ? 2 : 0;
+    return launch_kernel(attention_kernel<D, T, MODE, W>, dim3((unsigned)ctas), 32 * W, kSmem, pdl, s, a);
 }
 
 // Many items: one warp to each, so that short ones leave no warp idle and need no join of
@@ -727,24 +840,46 @@ cudaError_t launch_typed(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
 //   head_dim 128:  8 x 64, 10 11.2 -> 5.9, 100 12.8 -> 10.3, 2000 93 -> 94;  8 x 1000, 10 113 -> 47, 400 324 -> 277
 //                  8 x 32, 100 8.4 -> 14.5 (too few: what is not shared by warps is shared by CTAs)
 //   head_dim 64:   8 x 64, 100 7.6 -> 14.1;  8 x 128, 100 12.3 -> 9.1, 2000 91 -> 96
-//   head_dim 256:  4 x 128, 100 29.7 -> 25.2, 400 66 -> 63, 2000 189 -> 211
+//   head_dim 256:  4 x 128, 100 29.7 -> 25.2, 400 66 -> 63, 2000 189 -> 211;  4 x 800, 100 119 -> 78;
+//                  4 x 512, 1 to 512 145 -> 161
 // so at 64 and 256 only where the block table bounds the lengths.
 bool many_items(int d, int64_t items, int cap, int sms) {
     if (d == 64) return items >= 6 * (int64_t)sms && cap <= 256;
-    return items >= 3 * (int64_t)sms && (d != 256 || cap <= 512);
+    return items >= 3 * (int64_t)sms && (d != 256 || cap <= 256);
 }
 
-template <int D, class T, bool PACK>
+template <int D, class T, int MODE>
 cudaError_t launch_warps(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
-    if (many_items(D, (int64_t)a.rows * a.n_kv * a.head_groups, a.cap, sms)) return launch_typed<D, T, PACK, 1>(a, sms, pdl, s);
-    return launch_typed<D, T, PACK, warps(D)>(a, sms, pdl, s);
+    if (many_items(D, (int64_t)(a.rows / a.at.together) * a.n_kv * a.head_groups, a.cap, sms)) return launch_typed<D, T, MODE, 1>(a, sms, pdl, s);
+    return launch_typed<D, T, MODE, warps(D)>(a, sms, pdl, s);
+}
+
+// Several rows of a sequence together: where the rows outnumber the block table's sequences,
+// so that some must share one, and the tiles that the table allows are four to a CTA or more.
+// Measured without and with, us (sequences x rows of each, tokens):
+//   8 k/v heads of 4, head_dim 128, bf16:  6 x 4, 3000 48 -> 38;  64 x 2, 1000 95 -> 65;  1 x 512, 512 87 -> 88;
+//                                          8 x 100, 100 53 -> 58
+//   8 of 2, head_dim 64:  6 x 4, 3000 27 -> 15;  1 x 512, 512 57 -> 26;  16 x 2, 100 (too few) 5.3 -> 6.8
+//   8 of 1, head_dim 128: 1 x 4, 30000 69 -> 34;  8 x 100, 100 50 -> 29
+// and 64 x 1, 1000 with no two rows of a sequence 55 -> 64 (8 of 4).  Rows of 5 or more heads
+// stay by themselves: two sets of 8 in one warp took as long as two items (4 k/v heads of 8,
+// head_dim 256, 6 x 4 of 3000 54 -> 59 us: a warp's instructions are the bound, not its loads).
+template <int D, class T>
+cudaError_t launch_dim(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
+    const int64_t tiles = (int64_t)a.rows * a.n_kv * tiles_of(a.cap, tile_tok(D, warps(D)));
+    if (a.group <= 4 && a.at.seqs && a.rows > a.at.n_seqs && tiles >= 4 * sms * ctas_per_sm(D, warps(D))) {
+        a.head_shift = a.group > 2 ? 2 : a.group - 1;
+        a.at.together = kHeads >> a.head_shift;
+        return launch_warps<D, T, kShared>(a, sms, pdl, s);
+    }
+    if constexpr (kPieces<T> == 3)
+        if (a.group <= 4) return launch_warps<D, T, kPacked>(a, sms, pdl, s);
+    return launch_warps<D, T, kPlain>(a, sms, pdl, s);
 }
 
 template <int D>
-cudaError_t launch_dim(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
-    if (a.kv.type != kKvBf16) return launch_warps<D, __half, false>(a, sms, pdl, s);
-    return a.group <= 4 ? launch_warps<D, __nv_bfloat16, true>(a, sms, pdl, s)
-                        : launch_warps<D, __nv_bfloat16, false>(a, sms, pdl, s);
+cudaError_t launch_type(const AttnArgs& a, int sms, bool pdl, cudaStream_t s) {
+    return a.kv.type == kKvBf16 ? launch_dim<D, __nv_bfloat16>(a, sms, pdl, s) : launch_dim<D, __half>(a, sms, pdl, s);
 }
 
 }  // namespace
@@ -783,10 +918,10 @@ cudaError_t launch_paged_attention(const float* q, int64_t q_stride, int64_t row
     a.counters = counters;
     a.err = err;
     switch (kv.head_dim) {
-        case 64: return launch_dim<64>(a, sms, pdl, s);
-        case 96: return launch_dim<96>(a, sms, pdl, s);
-        case 128: return launch_dim<128>(a, sms, pdl, s);
-        case 256: return launch_dim<256>(a, sms, pdl, s);
+        case 64: return launch_type<64>(a, sms, pdl, s);
+        case 96: return launch_type<96>(a, sms, pdl, s);
+        case 128: return launch_type<128>(a, sms, pdl, s);
+        case 256: return launch_type<256>(a, sms, pdl, s);
     }
     return cudaErrorInvalidValue;
 }

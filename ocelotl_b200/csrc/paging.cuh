@@ -16,6 +16,7 @@ namespace ocl {
 struct KvRows {
     const int32_t *positions, *seqs, *table;
     int64_t n_seqs, max_pages, table_stride;
+    int together = 1;  // rows that an item may have (see item_tokens); 1 where seqs is null
 };
 
 // The row's sequence, or -1 if the block table has none such.
@@ -57,6 +58,22 @@ OCL_HD int row_tokens(const KvRows& at, int cap, int64_t row) {
     const bool there = pos >= 0 && sequence_of(at, row) >= 0;
     const int seen = pos < cap ? pos : cap - 1;
     return there ? seen + 1 : 0;
+}
+
+// The rows of an item: of each `together` (a power of two) rows from a multiple of it on,
+// those that follow one another in the same sequence.  Tokens that the item which starts
+// with `row` reads, the most that a row of it sees; `next` is the next item's first row.
+OCL_HD int item_tokens(const KvRows& at, int cap, int rows, int row, int& next) {
+    int most = row_tokens(at, cap, row);
+    next = row + 1;
+    if (at.together > 1) {
+        const int all = (row | (at.together - 1)) + 1, behind = all < rows ? all : rows, seq = at.seqs[row];
+        for (; next < behind && at.seqs[next] == seq; ++next) {
+            const int tokens = row_tokens(at, cap, next);
+            most = tokens > most ? tokens : most;
+        }
+    }
+    return most;
 }
 
 OCL_HD int tiles_of(int tokens, int tile_tok) { return (tokens + tile_tok - 1) / tile_tok; }
@@ -102,7 +119,8 @@ OCL_HD void item_runs(const Runs& r, uint32_t begin, int tiles, uint32_t& c0, ui
 
 // A place in the order of all tiles.
 struct Cursor {
-    int row, item;   // item of the row: k/v head and group of query heads
+    int row, next;   // first row of the item, and of the next one
+    int item;        // item of the rows: k/v head and group of query heads
     int tokens, tiles;
     int tile, stop;  // next tile, and where this run's piece of the item ends
     uint32_t begin;  // the item's first unit
@@ -122,8 +140,8 @@ OCL_HD bool next_item(const KvRows& at, int rows, int cap, int items, int tile_t
         c.item = 0;
         c.tokens = 0;
         do {
-            ++c.row;
-        } while (c.row < rows && (c.tokens = row_tokens(at, cap, c.row)) == 0);
+            c.row = c.next;
+        } while (c.row < rows && (c.tokens = item_tokens(at, cap, rows, c.row, c.next)) == 0);
         c.tiles = tiles_of(c.tokens, tile_tok);
     }
     set_stop(c, end);

@@ -4,8 +4,8 @@
 using namespace ocl;
 constexpr int kTile = 64;
 
-static uint32_t units_of(const KvRows& at, int cap, int items, int r) {
-    const int tokens = row_tokens(at, cap, r);
+static uint32_t units_of(const KvRows& at, int cap, int items, int rows, int r, int& next) {
+    const int tokens = item_tokens(at, cap, rows, r, next);
     return tokens ? item_units(tiles_of(tokens, kTile)) * (uint32_t)items : 0;
 }
 
@@ -13,13 +13,13 @@ static uint32_t units_of(const KvRows& at, int cap, int items, int r) {
 // writes (row, item, tile, cta) to out; returns the number of tiles, or a negative
 // code where two runs disagree about an item that they share.
 extern "C" long long walk(const int32_t* positions, const int32_t* seqs, long long n_seqs, int rows, int cap, int items,
-                          unsigned ctas, unsigned min_share, int snap, int32_t* out, long long room) {
-    const KvRows at{positions, seqs, nullptr, n_seqs, 0, 0};
+                          unsigned ctas, unsigned min_share, int snap, int together, int32_t* out, long long room) {
+    const KvRows at{positions, seqs, nullptr, n_seqs, 0, 0, together};
     uint32_t total = 0;
     long long tiles = 0;
-    for (int r = 0; r < rows; ++r) {
-        total += units_of(at, cap, items, r);
-        tiles += (long long)tiles_of(row_tokens(at, cap, r), kTile) * items;
+    for (int r = 0, next; r < rows; r = next) {
+        total += units_of(at, cap, items, rows, r, next);
+        tiles += (long long)tiles_of(item_tokens(at, cap, rows, r, next), kTile) * items;
     }
     if (!total) return 0;
     const Runs runs = runs_of(total, ctas, min_share, snap);
@@ -33,12 +33,12 @@ extern "C" long long walk(const int32_t* positions, const int32_t* seqs, long lo
             const uint32_t cut = run_cut(runs, c + i);
             edge[i] = total;
             uint32_t before = 0;
-            for (int r = 0; r < rows; ++r) {
-                const uint32_t n = units_of(at, cap, items, r);
+            for (int r = 0, next; r < rows; r = next) {
+                const uint32_t n = units_of(at, cap, items, rows, r, next);
                 if (cut < before + n) {
                     Cursor e{};
                     e.row = r;
-                    e.tokens = row_tokens(at, cap, r);
+                    e.tokens = item_tokens(at, cap, rows, r, e.next);
                     e.tiles = tiles_of(e.tokens, kTile);
                     const uint32_t all = item_units(e.tiles), off = cut - before, u = off % all;
                     e.item = (int)(off / all);

@@ -134,6 +134,78 @@ def test_several_rows_of_one_sequence_are_causal(backend):
     assert (got[6] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 8, 9])
+def test_drafted_rows_and_prompts(backend, group, dim, dtype):
+    """Runs of rows of one sequence, which are worked on together: drafted tokens, a prompt, padding between
+    them, positions out of order; long enough to be split, and short."""
+    lengths, rows = [900, 40, 3000, 7], []
+    rows += [(0, 900 - 5 + i) for i in range(5)] + [(1, p) for p in range(40)] + [(1, -1)] * 3
+    rows += [(2, p) for p in (2999, 2998, 0, 17, 31, 32, 1500)] + [(3, p) for p in (6, -1, 2)] + [(0, 64)]
+    k, v, table = paged(lengths, 16, 2, dim, dtype, group)
+    table = torch.nn.functional.pad(table, (0, 2000), value=-1)  # room for long sequences
+    seqs, pos = (torch.tensor([r[i] for r in rows], dtype=torch.int32, device="cuda") for i in range(2))
+    q = torch.randn(len(rows), 2 * group, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(dim))
+    cache = backend.kv_cache_view(k, v)
+    for n in (len(rows), 5, 2, 1):
+        out = torch.full((n, 2 * group, dim), float("nan"), device="cuda")
+        backend.paged_attention(q[:n], cache, pos[:n], table, seqs=seqs[:n], out=out)
+        backend.synchronize()
+        want, bound = attention_reference(q[:n], k, v, pos[:n], table, dim ** -0.5, seqs[:n])
+        assert ((out.double() - want).abs() <= bound).all(), n
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group", [2, 4, 8])
+def test_rows_of_a_sequence_do_not_see_later_tokens(backend, group, dim):
+    """What a later row of the sequence sees, NaN and infinities too, does not reach an earlier one."""
+    for dtype in (torch.bfloat16, torch.float16):
+        k, v, table = paged([50], 16, 1, dim, dtype, 3)
+        table = torch.nn.functional.pad(table, (0, 5000), value=-1)  # room for long sequences
+        slot = table[0, 3].long(), 0, 0  # token 48
+        seqs, pos = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.tensor([46, 47, 48, 49], dtype=torch.int32, device="cuda")
+        q = torch.randn(4, group, dim, device="cuda")
+        want, bound = attention_reference(q, k, v, pos, table, dim ** -0.5, seqs)
+        for t, bad in ((k, float("nan")), (v, float("nan")), (v, float("inf"))):
+            old = t[slot].clone()
+            t[slot] = bad
+            got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, seqs=seqs)
+            backend.synchronize()
+            t[slot] = old
+            assert ((got[:2].double() - want[:2]).abs() <= bound[:2]).all()
+            assert not torch.isfinite(got[2:]).any()
+
+
+def test_drafted_rows_over_many_ctas(backend):
+    for group, dim, dtype in ((8, 256, torch.bfloat16), (5, 128, torch.float16), (4, 128, torch.bfloat16), (1, 64, torch.float16)):
+        k, v, table = paged([9000, 20000], 16, 2, dim, dtype, 3)
+        pos = torch.tensor([8999 - 4 + i for i in range(5)] + [19999 - 4 + i for i in range(5)], dtype=torch.int32, device="cuda")
+        seqs = torch.tensor([0] * 5 + [1] * 5, dtype=torch.int32, device="cuda")
+        q = torch.randn(10, 2 * group, dim, device="cuda")
+        got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, seqs=seqs)
+        backend.synchronize()
+        want, bound = attention_reference(q, k, v, pos, table, dim ** -0.5, seqs)
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_many_items_of_several_rows(backend):
+    """Enough prompts that a warp takes whole items."""
+    for group, dim in ((4, 128), (2, 64), (4, 256)):
+        n = 20
+        lengths = [n] * 120
+        k, v, table = paged(lengths, 16, 8, dim, torch.bfloat16, 3)
+        pos = torch.arange(n, dtype=torch.int32, device="cuda").repeat(120)
+        seqs = torch.arange(120, dtype=torch.int32, device="cuda").repeat_interleave(n)
+        q = torch.randn(n * 120, 8 * group, dim, device="cuda")
+        got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, seqs=seqs)
+        backend.synchronize()
+        for s in (0, 7, 119):
+            at = slice(s * n, (s + 1) * n)
+            want, bound = attention_reference(q[at], k, v, pos[at], table, dim ** -0.5, seqs[at])
+            assert ((got[at].double() - want).abs() <= bound).all()
+
+
 def test_strided_queries_tables_and_neighbours(backend):
     k, v, table = paged([90, 200], 16, 2, 64, torch.bfloat16, 7)
     wide = torch.full((2, 40), 12345, dtype=torch.int32, device="cuda")

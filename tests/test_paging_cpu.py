@@ -17,20 +17,20 @@ def lib(tmp_path_factory):
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", str(HERE / "paging_host.cpp"), "-o", str(so)], check=True)
     lib = C.CDLL(str(so))
     lib.walk.restype = C.c_longlong
-    lib.walk.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_uint, C.c_uint, C.c_int, C.c_void_p, C.c_longlong]
+    lib.walk.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_uint, C.c_uint, C.c_int, C.c_int, C.c_void_p, C.c_longlong]
     lib.place.argtypes = [C.c_void_p] + [C.c_longlong] * 3 + [C.c_uint, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p]
     lib.wrong_quotient.restype = C.c_longlong
     lib.wrong_quotient.argtypes = [C.c_uint] + [C.c_longlong] * 3
     return lib
 
 
-def walk(lib, positions, cap, items, ctas, snap=0, min_share=1, seqs=None, n_seqs=None):
+def walk(lib, positions, cap, items, ctas, snap=0, min_share=1, seqs=None, n_seqs=None, together=1):
     pos = np.asarray(positions, np.int32)
     sq = None if seqs is None else np.asarray(seqs, np.int32)
     room = int(sum(-(-(min(p + 1, cap)) // TILE) for p in pos.astype(int) if p >= 0)) * items + 1
     out = np.full((room, 4), -1, np.int32)
     n = lib.walk(pos.ctypes.data, None if sq is None else sq.ctypes.data, len(pos) if n_seqs is None else n_seqs, len(pos),
-                 cap, items, ctas, min_share, snap, out.ctypes.data, room)
+                 cap, items, ctas, min_share, snap, together, out.ctypes.data, room)
     assert n >= 0, n
     return out[:n]
 
@@ -77,6 +77,26 @@ def test_short_items_are_not_shared(lib):
 def test_rows_of_unknown_sequences_have_no_tiles(lib):
     got = walk(lib, [100, 100, 100, 100], 1000, 2, 10, seqs=[0, -1, 2, 1], n_seqs=2)
     assert sorted(set(got[:, 0].tolist())) == [0, 3]
+
+
+@pytest.mark.parametrize("together", [2, 4, 8])
+def test_rows_of_a_sequence_share_items(lib, together):
+    rng = np.random.default_rng(together)
+    for _ in range(100):
+        rows, n_seqs, items = int(rng.integers(1, 50)), int(rng.integers(1, 6)), int(rng.integers(1, 5))
+        seqs = np.repeat(rng.integers(-1, n_seqs + 1, rows), rng.integers(1, 12, rows))[:rows]  # -1 and n_seqs are unknown
+        pos = np.where(rng.random(rows) < 0.2, -1, rng.integers(0, int(rng.choice([2, 70, 900, 9000])), rows))
+        cap = int(rng.integers(1, 9000))
+        got = walk(lib, pos, cap, items, int(rng.integers(1, 300)), int(rng.integers(0, 4)), int(rng.integers(1, 4)), seqs, n_seqs, together)
+        want, r = [], 0
+        while r < rows:
+            n = 1
+            while r + n < rows and (r + n) % together and seqs[r + n] == seqs[r]:
+                n += 1
+            tokens = max(min(int(p) + 1, cap) for p in pos[r:r + n]) if 0 <= seqs[r] < n_seqs else 0
+            want += [(r, i, t) for i in range(items) for t in range(-(-tokens // TILE))]
+            r += n
+        assert [tuple(x[:3]) for x in got.tolist()] == want
 
 
 def test_place_of(lib):
