@@ -60,7 +60,8 @@ constexpr int warp_tok(int d) { return d == 256 ? 16 : 32; }
 // At head_dim 256 a tile takes a warp twice as long and eight are wanted; their rings have
 // separate slots for keys and values, so that three of 8 KB keep copies under way
 // (6 rows of 900 to 6000 tokens, 4 k/v heads of 8: 25.6 us with four warps, 22.9 with
-// eight; at head_dim 128 both changes lose: 64 ragged rows 123 us, 143 and 129).
+// eight; at head_dim 128 both changes lose: 64 ragged rows 123 us, 143 and 129; sixteen warps
+// at 256, two to the halves of 16 tokens' elements: 64 rows of 1000 tokens 63 us, of eight 55).
 constexpr bool split_slots(int d) { return d == 256; }
 constexpr int warps(int d) { return d == 256 ? 8 : 4; }
 constexpr int slots(int d) { return d == 96 ? 4 : 3; }
@@ -288,9 +289,13 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         total += sh.scan[w];
         longest = max(longest, sh.longest[w]);
     }
-    // Pieces of an item cost their join: about a tenth of a tile's time each, so the
-    // longest item is cut into no more than sqrt(10 * tiles) of them.
-    const Runs runs = runs_of(total, gridDim.x, max(1u, (uint32_t)(sqrtf(0.1f * (float)longest) + 0.999f)), p.snap);
+    // Pieces of an item cost their join: about a twentieth of a tile's time each, so the
+    // longest item is cut into no more than sqrt(20 * tiles) of them (one row of 2000 tokens,
+    // head_dim 256: 15.0 us with sqrt(10 * tiles), 12.8, 12.8 with sqrt(40 * tiles)).
+    // Items of one or two tiles are left
+    // whole (200 tokens: 8.9 us cut in two, 7.0 whole).
+    const Runs runs = runs_of(total, gridDim.x, max(1u, (uint32_t)(sqrtf(0.05f * (float)longest) + 0.999f)),
+                              longest <= 2 ? max(p.snap, 1) : p.snap);
     const uint32_t cta = blockIdx.x;
     const bool active = total > 0 && cta < runs.P;
     for (int i = side; i < 2; i += kSides) {
@@ -510,8 +515,8 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                 }
 #pragma unroll
             for (int v = 0; v < QV; ++v) {
-                if constexpr (QS) q_frag[((i * kWarps + warp) * QV + v) * 32 + lane] = make_uint4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
-                else qa[i][4 * v] = f[4 * v], qa[i][4 * v + 1] = f[4 * v + 1], qa[i][4 * v + 2] = f[4 * v + 2], qa[i][4 * v + 3] = f[4 * v + 3];
+                if constexpr (!QS) qa[i][4 * v] = f[4 * v], qa[i][4 * v + 1] = f[4 * v + 1], qa[i][4 * v + 2] = f[4 * v + 2], qa[i][4 * v + 3] = f[4 * v + 3];
+                else q_frag[((i * kWarps + warp) * QV + v) * 32 + lane] = make_uint4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
             }
         }
         __syncthreads();  // q_frag is written; the previous item's merge buffers are read
@@ -681,6 +686,10 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (c4 == 0) sh.m[warp][g] = m, sh.l[warp][g] = l;
+        if (MC < D && !more) {  // the ring is free
+            cp_wait<0>();
+            __syncthreads();
+        }
         // the row (from the item's first on) and query head that MMA row h holds; false: none
         auto holds = [&](int h, int& member, int& head) {
             member = SHARE ? h >> p.head_shift : 0;
@@ -688,18 +697,20 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
             return head < nh && (!SHARE || member < item_rows);
         };
         float* slot = p.part + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * slot_floats(D);
+        auto merge = [&](auto columns, float* buffer) {  // so many columns at a time
+            constexpr int kCols = decltype(columns)::value;
 #pragma unroll
-        for (int col0 = 0; col0 < D; col0 += MC) {
+        for (int col0 = 0; col0 < D; col0 += kCols) {
             if (col0) __syncthreads();  // the previous columns are read
 #pragma unroll
-            for (int t = 0; t < MC / 8; ++t)
-                *reinterpret_cast<float2*>(merge_o + (warp * kHeads + g) * MC + ((t * 8 + c4 * 2) ^ ((g & 3) << 3))) =
+            for (int t = 0; t < kCols / 8; ++t)
+                *reinterpret_cast<float2*>(buffer + (warp * kHeads + g) * kCols + ((t * 8 + c4 * 2) ^ ((g & 3) << 3))) =
                     make_float2(o[col0 / 8 + t][0], o[col0 / 8 + t][1]);
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < (kRows * MC / 4 + kThreads - 1) / kThreads; ++i) {
-                const int idx = i * kThreads + tid, h = idx / (MC / 4), col = idx % (MC / 4) * 4;
-                if (idx >= kRows * MC / 4) break;
+            for (int i = 0; i < (kRows * kCols / 4 + kThreads - 1) / kThreads; ++i) {
+                const int idx = i * kThreads + tid, h = idx / (kCols / 4), col = idx % (kCols / 4) * 4;
+                if (idx >= kRows * kCols / 4) break;
                 float top = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][h]);
@@ -709,9 +720,9 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     const float f = ex2(sh.m[w][h] - ref);
-                    float4 x = *reinterpret_cast<const float4*>(merge_o + (w * kHeads + h) * MC + (col ^ ((h & 3) << 3)));
+                    float4 x = *reinterpret_cast<const float4*>(buffer + (w * kHeads + h) * kCols + (col ^ ((h & 3) << 3)));
                     if constexpr (PACK) {  // h + 4 has the same swizzle
-                        const float4 z = *reinterpret_cast<const float4*>(merge_o + (w * kHeads + h + 4) * MC + (col ^ ((h & 3) << 3)));
+                        const float4 z = *reinterpret_cast<const float4*>(buffer + (w * kHeads + h + 4) * kCols + (col ^ ((h & 3) << 3)));
                         x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
                     }
                     sum += sh.l[w][h] * f;
@@ -732,78 +743,103 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                 }
             }
         }
+        };
+        if constexpr (MC < D) {
+            if (more) merge(std::integral_constant<int, MC>(), merge_o);
+            else merge(std::integral_constant<int, D>(), reinterpret_cast<float*>(smem));
+        } else {
+            merge(std::integral_constant<int, MC>(), merge_o);
+        }
         if (!whole) {
             __syncthreads();
             if (tid == 0) {
-                __threadfence();
-                sh.last_in = atomicAdd(p.counters + c0, 1u) == (unsigned)(c1 - c0);
+                unsigned int before;  // releases this CTA's part, acquires those of the CTAs before
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + c0) : "memory");
+                sh.last_in = before == c1 - c0;
                 if (sh.last_in) p.counters[c0] = 0;
-                __threadfence();
             }
             __syncthreads();
             if (sh.last_in) {
                 // ---- this CTA is the last one of the item: join all, in CTA order
-                // A warp takes a head: lane i holds the maximum and the sum of the i-th CTA, then
-                // every lane adds its columns, 16 CTAs' loads in flight.
+                // A warp takes a head, two together where there are as many: lane i holds the maximum
+                // and the sum of the i-th CTA, then every lane adds its columns, B CTAs' loads in flight.
                 const int parts = (int)(c1 - c0) + 1;
                 const float* first = p.part + (size_t)(2 * c0 + 1) * slot_floats(D);
                 const float* rest = p.part + (size_t)(2 * c0) * slot_floats(D);
                 auto part_of = [&](int i) { return i == 0 ? first : rest + (size_t)(2 * i) * slot_floats(D); };
                 constexpr int V = D % 128 == 0 ? 4 : D == 64 ? 2 : 1, L = D / (32 * V);  // floats a load, loads a lane
-                constexpr int B = 16 / L;
-                for (int h = warp; h < kRows; h += kWarps) {
-                    int member, head;
-                    if (!holds(h, member, head)) continue;
-                    float top = -INFINITY, sum = 0.f, acc[L][V] = {};
+                constexpr int U = kRows >= 2 * kWarps ? 2 : 1, B = D == 96 ? 4 : 16 / L / U;
+                for (int n = warp; n < kRows; n += U * kWarps) {
+                    int h[U];
+                    int64_t to[U];  // -1: not a head of the item
+                    float top[U], sum[U], weight[U], acc[U][L][V] = {};
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        int member, head;
+                        h[u] = n + u * kWarps;
+                        to[u] = holds(h[u], member, head) ? ((int64_t)(row + member) * p.n_heads + h0 + head) * D + lane * V : -1;
+                        top[u] = -INFINITY, sum[u] = weight[u] = 0.f;
+                    }
                     for (int i0 = 0; i0 < parts; i0 += 32) {
-                        float m_i = -INFINITY, l_i = 0.f;
-                        if (i0 + lane < parts) {
-                            m_i = __ldcg(part_of(i0 + lane) + kHeads * D + h);
-                            l_i = __ldcg(part_of(i0 + lane) + kHeads * D + kHeads + h);
+                        float m_i[U], l_i[U];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            m_i[u] = -INFINITY, l_i[u] = 0.f;
+                            if (i0 + lane < parts) {
+                                m_i[u] = __ldcg(part_of(i0 + lane) + kHeads * D + h[u]);
+                                l_i[u] = __ldcg(part_of(i0 + lane) + kHeads * D + kHeads + h[u]);
+                            }
                         }
                         const int n32 = min(32, parts - i0);
-                        float weight = 0.f;
                         for (int b = 0; b < n32; b += B) {
-                            float part[B][L][V];
+                            float part_o[U][B][L][V];
 #pragma unroll
                             for (int i = 0; i < B; ++i) {
-                                const float* from = part_of(i0 + min(b + i, n32 - 1)) + h * D + lane * V;
+                                const float* from = part_of(i0 + min(b + i, n32 - 1));
 #pragma unroll
-                                for (int j = 0; j < L; ++j) load_cg<V>(part[i][j], from + j * 32 * V);
-                            }
-                            if (b == 0) {  // the maximum over these CTAs, behind the loads
-                                float t = m_i;
+                                for (int u = 0; u < U; ++u)
 #pragma unroll
-                                for (int s = 16; s; s >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, s));
-                                t = fmaxf(t, top);
-                                const float ref = t == -INFINITY ? 0.f : t, alpha = ex2(top - ref);
-                                top = t;
-                                weight = ex2(m_i - ref);
-                                sum = fmaf(sum, alpha, l_i * weight);
-#pragma unroll
-                                for (int j = 0; j < L; ++j)
-#pragma unroll
-                                    for (int e = 0; e < V; ++e) acc[j][e] *= alpha;
+                                    for (int j = 0; j < L; ++j) load_cg<V>(part_o[u][i][j], from + h[u] * D + lane * V + j * 32 * V);
                             }
 #pragma unroll
-                            for (int i = 0; i < B; ++i) {
-                                const float f = __shfl_sync(0xffffffffu, weight, (b + i) & 31);
-                                const bool in = b + i < n32;
+                            for (int u = 0; u < U; ++u) {
+                                if (b == 0) {  // the maximum over these CTAs, behind the loads
+                                    float t = m_i[u];
 #pragma unroll
-                                for (int j = 0; j < L; ++j)
+                                    for (int s = 16; s; s >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, s));
+                                    t = fmaxf(t, top[u]);
+                                    const float ref = t == -INFINITY ? 0.f : t, less = ex2(top[u] - ref);
+                                    top[u] = t;
+                                    weight[u] = ex2(m_i[u] - ref);
+                                    sum[u] = fmaf(sum[u], less, l_i[u] * weight[u]);
 #pragma unroll
-                                    for (int e = 0; e < V; ++e) acc[j][e] = fmaf(in ? part[i][j][e] : 0.f, in ? f : 0.f, acc[j][e]);
+                                    for (int j = 0; j < L; ++j)
+#pragma unroll
+                                        for (int e = 0; e < V; ++e) acc[u][j][e] *= less;
+                                }
+#pragma unroll
+                                for (int i = 0; i < B; ++i) {
+                                    const float f = __shfl_sync(0xffffffffu, weight[u], (b + i) & 31);
+                                    const bool in = b + i < n32;
+#pragma unroll
+                                    for (int j = 0; j < L; ++j)
+#pragma unroll
+                                        for (int e = 0; e < V; ++e) acc[u][j][e] = fmaf(in ? part_o[u][i][j][e] : 0.f, in ? f : 0.f, acc[u][j][e]);
+                                }
                             }
                         }
                     }
 #pragma unroll
-                    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    float* to = p.out + ((int64_t)(row + member) * p.n_heads + h0 + head) * D + lane * V;
+                    for (int u = 0; u < U; ++u) {
 #pragma unroll
-                    for (int j = 0; j < L; ++j)
+                        for (int s = 16; s; s >>= 1) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], s);
+                        const float inv = sum[u] == 0.f ? 0.f : 1.0f / sum[u];
+                        if (to[u] < 0) continue;
 #pragma unroll
-                        for (int e = 0; e < V; ++e) to[j * 32 * V + e] = acc[j][e] * inv;
+                        for (int j = 0; j < L; ++j)
+#pragma unroll
+                            for (int e = 0; e < V; ++e) p.out[to[u] + j * 32 * V + e] = acc[u][j][e] * inv;
+                    }
                 }
             }
         }
@@ -826,7 +862,7 @@ cudaError_t launch_typed(AttnArgs a, int sms, bool pdl, cudaStream_t s) {
     }
     const int64_t items = (int64_t)a.rows * a.n_kv * a.head_groups, tiles = items * tiles_of(a.cap, tile_tok(D, W));
     if (tiles + items > 0x7fffffff) return cudaErrorInvalidValue;  // the runs' arithmetic; checked by the caller
-    const int64_t most = (int64_t)sms * ctas_per_sm(D, W), ctas = tiles < most ? tiles : most;
+    const int64_t most = (int64_t)sms * ctas_per_sm(D, W), ctas = tiles + items < most ? tiles + items : most;
     // With about as many items as CTAs, a short item is better left whole than shared (its
     // join takes longer than its tiles: 16 rows of 555 tokens and 8 k/v heads 15.2 -> 11.1
     // us, 230 rows of 5 to 180 tokens 15.3 -> 12.5); with fewer items every cut is wanted (one
