@@ -307,7 +307,8 @@ typedef struct ocl_kv_cache {
  * of sequence seqs_dev[r], or of sequence r when seqs_dev is NULL (then rows <=
  * n_seqs).  A negative position is a padding row.  block_table_dev is int32
  * [n_seqs, max_pages] with rows table_stride apart; entries behind a sequence's
- * last page are not read.  max_pages * page_size bounds a sequence's length. */
+ * last page are not read.  max_pages * page_size bounds a sequence's length.  None
+ * of these arrays may change while a call runs. */
 typedef struct ocl_kv_rows {
     const int32_t* positions_dev;
     const int32_t* seqs_dev;
@@ -350,7 +351,8 @@ OCL_API int ocl_qk_norm_rope(ocl_ctx* ctx, const float* qkv_dev, size_t qkv_stri
  * value that a row sees makes the outputs that it enters NaN.  Padding rows give zeros.
  * Tokens whose page is out of range are left out and counted as bad ids (a row with
  * none left is zeros), as are rows whose sequence is (zeros) and positions past the
- * block table (the tokens that it can hold are used).  The lengths are read on the
+ * block table (the tokens that it can hold are used); rows of one sequence that follow one
+ * another may read it together and then count a page's tokens once.  The lengths are read on the
  * device: a captured launch follows them.  Uses a fixed workspace of the context,
  * so launches of one context must not overlap on the GPU. */
 OCL_API int ocl_paged_attention(ocl_ctx* ctx, const float* q_dev, size_t q_stride, size_t rows, size_t n_heads,
