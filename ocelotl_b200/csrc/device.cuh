@@ -12,7 +12,6 @@ namespace ocl {
 // here before its first read or write of memory that another kernel uses, so a
 // kernel's own completion implies that of all kernels before it.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <class... KArgs, class... Args>
 cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, bool pdl, cudaStream_t s,

@@ -272,6 +272,32 @@ def test_captured_launch_follows_the_positions(backend):
         assert torch.equal(eager, out)
 
 
+def test_captured_launch_of_rows_of_a_sequence(backend):
+    """Which rows belong together, and how long they are, is read on the device at every replay."""
+    k, v, table = paged([1500, 1500], 16, 2, 128, torch.bfloat16, 8)
+    table = torch.nn.functional.pad(table, (0, 2000), value=-1)
+    cache = backend.kv_cache_view(k, v)
+    q = torch.randn(6, 8, 128, device="cuda")
+    pos, seqs = (torch.zeros(6, dtype=torch.int32, device="cuda") for _ in range(2))
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph):
+            backend.use_current_stream()
+            backend.paged_attention(q, cache, pos, table, seqs=seqs, out=out)
+    finally:
+        backend.set_stream(None)
+    for of, at in (([0] * 6, [9, 10, 11, 12, 13, 14]), ([0, 1] * 3, [1499, 1499, 3, -1, 700, 701]),
+                   ([1, 1, 1, 0, 0, 0], [1497, 1498, 1499, -1, -1, 0]), ([0, 0, 0, 0, 1, 1], [63, 64, 31, 32, 127, 128])):
+        pos.copy_(torch.tensor(at, dtype=torch.int32))
+        seqs.copy_(torch.tensor(of, dtype=torch.int32))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, bound = attention_reference(q, k, v, pos, table, 128 ** -0.5, seqs)
+        assert ((out.double() - want).abs() <= bound).all(), (of, at)
+
+
 def test_on_a_side_stream(backend):
     k, v, table = paged([900], 16, 2, 128, torch.bfloat16, 9)
     stream = torch.cuda.Stream()
