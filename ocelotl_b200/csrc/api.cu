@@ -426,7 +426,7 @@ int ocl_cuda_init(int device, ocl_ctx** out) {
     if (e == cudaSuccess) e = cudaMemset(ctx->dev_flags, 0, 64);
     if (e == cudaSuccess) e = cudaHostAlloc((void**)&ctx->host_flags, 64, cudaHostAllocMapped);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer((void**)&ctx->host_flags_dev, ctx->host_flags, 0);
-    // The pick's and the attention's workspaces have one size for every call (a few
+    // The pick's and the attention's workspaces have one size for every call (some 13
     // MB): made here, they need no call before a capture and never move under one.
     const size_t slot_bytes = ocl::kArgmaxRowsMax * sizeof(unsigned long long);
     const size_t arrival_bytes = ocl::kArgmaxRowsMax * sizeof(unsigned int);

@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         const bool more = cc.tile < cc.stop;
         if (more) load_q();
 
-        // ---- join the four warps
+        // ---- join the warps
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (c4 == 0) sh.m[warp][g] = m, sh.l[warp][g] = l;
@@ -700,49 +700,49 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
         auto merge = [&](auto columns, float* buffer) {  // so many columns at a time
             constexpr int kCols = decltype(columns)::value;
 #pragma unroll
-        for (int col0 = 0; col0 < D; col0 += kCols) {
-            if (col0) __syncthreads();  // the previous columns are read
+            for (int col0 = 0; col0 < D; col0 += kCols) {
+                if (col0) __syncthreads();  // the previous columns are read
 #pragma unroll
-            for (int t = 0; t < kCols / 8; ++t)
-                *reinterpret_cast<float2*>(buffer + (warp * kHeads + g) * kCols + ((t * 8 + c4 * 2) ^ ((g & 3) << 3))) =
-                    make_float2(o[col0 / 8 + t][0], o[col0 / 8 + t][1]);
-            __syncthreads();
+                for (int t = 0; t < kCols / 8; ++t)
+                    *reinterpret_cast<float2*>(buffer + (warp * kHeads + g) * kCols + ((t * 8 + c4 * 2) ^ ((g & 3) << 3))) =
+                        make_float2(o[col0 / 8 + t][0], o[col0 / 8 + t][1]);
+                __syncthreads();
 #pragma unroll
-            for (int i = 0; i < (kRows * kCols / 4 + kThreads - 1) / kThreads; ++i) {
-                const int idx = i * kThreads + tid, h = idx / (kCols / 4), col = idx % (kCols / 4) * 4;
-                if (idx >= kRows * kCols / 4) break;
-                float top = -INFINITY;
+                for (int i = 0; i < (kRows * kCols / 4 + kThreads - 1) / kThreads; ++i) {
+                    const int idx = i * kThreads + tid, h = idx / (kCols / 4), col = idx % (kCols / 4) * 4;
+                    if (idx >= kRows * kCols / 4) break;
+                    float top = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][h]);
-                const float ref = top == -INFINITY ? 0.f : top;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                float sum = 0.f;
+                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][h]);
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float sum = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float f = ex2(sh.m[w][h] - ref);
-                    float4 x = *reinterpret_cast<const float4*>(buffer + (w * kHeads + h) * kCols + (col ^ ((h & 3) << 3)));
-                    if constexpr (PACK) {  // h + 4 has the same swizzle
-                        const float4 z = *reinterpret_cast<const float4*>(buffer + (w * kHeads + h + 4) * kCols + (col ^ ((h & 3) << 3)));
-                        x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float f = ex2(sh.m[w][h] - ref);
+                        float4 x = *reinterpret_cast<const float4*>(buffer + (w * kHeads + h) * kCols + (col ^ ((h & 3) << 3)));
+                        if constexpr (PACK) {  // h + 4 has the same swizzle
+                            const float4 z = *reinterpret_cast<const float4*>(buffer + (w * kHeads + h + 4) * kCols + (col ^ ((h & 3) << 3)));
+                            x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
+                        }
+                        sum += sh.l[w][h] * f;
+                        a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
                     }
-                    sum += sh.l[w][h] * f;
-                    a.x += x.x * f; a.y += x.y * f; a.z += x.z * f; a.w += x.w * f;
-                }
-                int member, head;
-                if (!holds(h, member, head)) continue;
-                if (whole) {
-                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    *reinterpret_cast<float4*>(p.out + ((int64_t)(row + member) * p.n_heads + h0 + head) * D + col0 + col) =
-                        make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-                } else {
-                    __stcg(reinterpret_cast<float4*>(slot + h * D + col0 + col), a);
-                    if (col0 + col == 0) {
-                        __stcg(slot + kHeads * D + h, top);
-                        __stcg(slot + kHeads * D + kHeads + h, sum);
+                    int member, head;
+                    if (!holds(h, member, head)) continue;
+                    if (whole) {
+                        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                        *reinterpret_cast<float4*>(p.out + ((int64_t)(row + member) * p.n_heads + h0 + head) * D + col0 + col) =
+                            make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+                    } else {
+                        __stcg(reinterpret_cast<float4*>(slot + h * D + col0 + col), a);
+                        if (col0 + col == 0) {
+                            __stcg(slot + kHeads * D + h, top);
+                            __stcg(slot + kHeads * D + kHeads + h, sum);
+                        }
                     }
                 }
             }
-        }
         };
         if constexpr (MC < D) {
             if (more) merge(std::integral_constant<int, MC>(), merge_o);
