@@ -27,6 +27,7 @@ runs them between the calls.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -137,7 +138,7 @@ class AttentionPlan:
     scale: float
     rot_dim: int
     rope_base: float
-    rope_scale: float            # every frequency is divided by it (linear position scaling)
+    rope_scale: float            # every frequency is divided by it (linear position scaling, 1 = none)
     rope_factors: str | None     # tensor of per-pair frequency divisors
     interleaved: bool            # pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2)
     eps: float
@@ -147,6 +148,26 @@ class AttentionPlan:
 
 # How an architecture's files pair the elements that a rotation turns together.
 ROPE_INTERLEAVED = {"llama": True, "qwen2": False, "qwen3": False}
+
+
+def _rope_scale(m: Manifest, arch: str) -> float:
+    """Linear position scaling of a file: 1 where it states none.
+
+    A factor without a type is linear; a type of "none" wins over a factor beside it.
+    Older files have `rope.scale_linear` in place of `rope.scaling.factor`.
+    """
+    kind = m.metadata.get(f"{arch}.rope.scaling.type")
+    if kind not in (None, "none", "linear"):
+        raise UnsupportedError("rope scaling", str(kind), ["none", "linear"])
+    if kind == "none":
+        return 1.0
+    for key in (f"{arch}.rope.scaling.factor", f"{arch}.rope.scale_linear"):
+        if key in m.metadata:
+            f = m.metadata[key]
+            if isinstance(f, bool) or not isinstance(f, (int, float)) or not 0 < f < math.inf:
+                raise InvalidRequestError("metadata", f"`{key}` must be a positive finite number, is {f!r}")
+            return float(f)
+    return 1.0
 
 
 def attention_plan(m: Manifest, p: ModelPlan) -> AttentionPlan:
@@ -171,9 +192,7 @@ def attention_plan(m: Manifest, p: ModelPlan) -> AttentionPlan:
     for feature in ("attention.sliding_window", "attn_logit_softcapping"):
         if m.metadata.get(f"{arch}.{feature}"):
             raise UnsupportedError(feature, str(m.metadata[f"{arch}.{feature}"]), ["none"])
-    scaling = m.metadata.get(f"{arch}.rope.scaling.type", "none")
-    if scaling not in ("none", "linear"):
-        raise UnsupportedError("rope scaling", str(scaling), ["none", "linear"])
+    rope_scale = _rope_scale(m, arch)
     for lp in p.layers:
         if lp.qkv_rows != [heads * dim, kv * dim, kv * dim]:
             raise InvalidRequestError("tensor", f"layer {lp.index}: q/k/v rows {lp.qkv_rows} are not {heads} + 2 * {kv} heads of {dim}")
@@ -199,7 +218,7 @@ def attention_plan(m: Manifest, p: ModelPlan) -> AttentionPlan:
     return AttentionPlan(
         heads, kv, dim, float(m.metadata.get(f"{arch}.attention.scale", 0.0)) or dim ** -0.5, rot,
         float(m.metadata.get(f"{arch}.rope.freq_base", 10000.0)),
-        float(m.metadata.get(f"{arch}.rope.scaling.factor", 1.0)) if scaling == "linear" else 1.0, factors,
+        rope_scale, factors,
         ROPE_INTERLEAVED[arch], float(need(f"{arch}.attention.layer_norm_rms_epsilon")), norms("q"), norms("k"))
 
 

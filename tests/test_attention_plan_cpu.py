@@ -62,3 +62,32 @@ def test_norms_of_another_shape(tmp_path):
     m = manifest(tmp_path, extra=[f32("blk.0.attn_q_norm.weight", 32)])
     with pytest.raises(InvalidRequestError, match="attn_q_norm"):
         attention_plan(m, plan(m))
+
+
+def llama(**meta):
+    return {**{k.replace("qwen3", "llama"): v for k, v in META.items()}, "general.architecture": "llama",
+            **{"llama.rope." + k.replace("__", "."): v for k, v in meta.items()}}
+
+
+@pytest.mark.parametrize("stated,scale", [
+    ({"scaling__factor": 4.0}, 4.0), ({"scale_linear": 4.0}, 4.0), ({"scaling__type": "linear", "scale_linear": 2.5}, 2.5),
+    ({"scaling__factor": 2.0, "scale_linear": 8.0}, 2.0), ({"scaling__factor": 8}, 8.0), ({"scaling__type": "linear"}, 1.0),
+    ({"scaling__type": "none", "scaling__factor": 4.0, "scale_linear": 4.0}, 1.0), ({"scaling__factor": 1.0}, 1.0), ({}, 1.0),
+])
+def test_position_scaling_that_a_file_states(tmp_path, stated, scale):
+    """A factor is linear scaling unless a type says otherwise; the older key counts where the newer is missing."""
+    m = manifest(tmp_path, llama(**stated))
+    assert attention_plan(m, plan(m)).rope_scale == scale
+
+
+@pytest.mark.parametrize("stated,error", [
+    ({"scaling__type": "linear", "scaling__factor": 0.0}, InvalidRequestError), ({"scaling__factor": 0.0}, InvalidRequestError),
+    ({"scaling__factor": -2.0}, InvalidRequestError), ({"scale_linear": float("nan")}, InvalidRequestError),
+    ({"scale_linear": float("inf")}, InvalidRequestError), ({"scaling__factor": "4"}, InvalidRequestError),
+    ({"scaling__factor": [4.0]}, InvalidRequestError), ({"scaling__type": "yarn", "scaling__factor": 4.0}, UnsupportedError),
+    ({"scaling__type": "yarn", "scale_linear": 4.0}, UnsupportedError),
+])
+def test_position_scaling_that_is_refused(tmp_path, stated, error):
+    m = manifest(tmp_path, llama(**stated))
+    with pytest.raises(error, match="scal"):
+        attention_plan(m, plan(m))

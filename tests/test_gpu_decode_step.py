@@ -216,3 +216,35 @@ def test_new_cache_is_zeroed_before_either_stream_writes(busy):
         b.qk_norm_rope(qkv, cache, pos, table, None)
     torch.cuda.synchronize()
     assert (cache.k[0, 0, 0] == 1).all() and (cache.v[0, 0, 0] == 1).all()
+
+
+@pytest.mark.parametrize("stated", [{"llama.rope.scaling.factor": 4.0}, {"llama.rope.scale_linear": 4.0},
+                                    {"llama.rope.scaling.type": "linear", "llama.rope.scaling.factor": 4.0}])
+def test_step_of_a_file_with_scaled_positions(backend, tmp_path, stated):
+    """A decode step at the angles that the file asks for, however it states them."""
+    from ocelotl_b200 import gguf
+    from ocelotl_b200.model import QuantizedDecoderLinears
+    from tests.gguf_writer import write_gguf
+    from tests.model_files import decoder_tensors
+    from tests.test_gpu_rope import UNITS
+    f = tmp_path / "scaled.gguf"
+    write_gguf(f, decoder_tensors(n_layers=1))
+    m = gguf.inspect(f)
+    m.metadata.update({k.replace("qwen3", "llama"): v for k, v in META.items()} | {"general.architecture": "llama"} | stated)
+    model = QuantizedDecoderLinears(backend, m)
+    cache = model.kv_caches(40, PAGE)[0]
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(1))[:39].to(torch.int32).cuda()[None]
+    g = torch.Generator("cuda").manual_seed(2)
+    qkv = torch.randn(600, (HEADS + 2 * KV_HEADS) * DIM, device="cuda", generator=g)
+    pos, seqs = torch.arange(600, dtype=torch.int32, device="cuda"), torch.zeros(600, dtype=torch.int32, device="cuda")
+    q = torch.empty(600, HEADS, DIM, device="cuda")
+    model.attention(0, qkv[:599], cache, pos[:599], table, seqs=seqs[:599], q=q[:599])  # the prompt
+    got = model.attention(0, qkv[599:], cache, pos[599:], table, q=q[599:])             # one token more
+    backend.synchronize()
+    (want_q, size), (want_k, k_size), _ = rope_reference(qkv, HEADS, KV_HEADS, DIM, pos, DIM, 1e6, True, None, None, 1e-5, [4.0] * (DIM // 2))
+    assert ((q.double() - want_q).abs() <= UNITS * size).all()
+    k = cache.k[table[0].long()[pos.long() // PAGE], :, pos.long() % PAGE].double()
+    half = torch.finfo(torch.bfloat16).eps / 2
+    assert ((k - want_k).abs() <= half * want_k.abs() * (1 + half) + UNITS * k_size * (1 + half) + 1e-38).all()
+    want, bound = attention_reference(q[599:], cache.k, cache.v, pos[599:], table, DIM ** -0.5)
+    assert ((got.view(want.shape).double() - want).abs() <= bound).all()
