@@ -332,11 +332,11 @@ OCL_API int ocl_rope_free(ocl_rope* rope);
  * heads, as the fused projection gives them.  q_norm_dev / k_norm_dev f32
  * [head_dim] or NULL (no norm): x * rsqrt(mean(x^2) + eps) * w.  rope NULL = no
  * rotation.  q_out_dev f32 [rows, n_heads, head_dim]; k and v are rounded to the
- * cache's type at the row's place.  A padding row's q is zeros and nothing is
- * cached.  A position, sequence or page out of range caches nothing and bumps the
- * counter that ocl_take_device_errors reports as bad ids.  Rows of one call must
- * stand at different places.  qkv, norms and q_out 16-byte aligned, qkv_stride a
- * multiple of 4. */
+ * cache's type at the row's place (f16: 65520 and above to an infinity).  A padding
+ * row's q is zeros and nothing is cached.  A position, sequence or page out of range
+ * caches nothing and bumps the counter that ocl_take_device_errors reports as bad ids.
+ * Rows of one call must stand at different places.  qkv, norms and q_out 16-byte
+ * aligned, qkv_stride a multiple of 4. */
 OCL_API int ocl_qk_norm_rope(ocl_ctx* ctx, const float* qkv_dev, size_t qkv_stride, size_t rows, size_t n_heads,
                              const ocl_kv_cache* cache, const ocl_kv_rows* at, const float* q_norm_dev,
                              const float* k_norm_dev, float eps, const ocl_rope* rope, float* q_out_dev);
@@ -347,8 +347,10 @@ OCL_API int ocl_qk_norm_rope(ocl_ctx* ctx, const float* qkv_dev, size_t qkv_stri
  * one sequence (drafted tokens, a prompt) are causal.  Query head h reads k/v head
  * h / (n_heads / n_kv_heads).  q_dev f32 [rows, n_heads, head_dim], rows q_stride
  * floats apart; out_dev f32 [rows, n_heads, head_dim].  scale > 0.  Accuracy: f32
- * (q and the softmax weights are not rounded to 16 bits); an infinite or NaN key or
- * value that a row sees makes the outputs that it enters NaN.  Padding rows give zeros.
+ * (q and the softmax weights are not rounded to 16 bits).  An infinite or NaN key that a
+ * row sees makes the outputs of its heads NaN, whatever its score's sign, and so does a
+ * query that is one or a score past f32's range; an infinite or NaN value makes its own
+ * element of them NaN.  Padding rows give zeros.
  * Tokens whose page is out of range are left out and counted as bad ids (a row with
  * none left is zeros), as are rows whose sequence is (zeros) and positions past the
  * block table (the tokens that it can hold are used); rows of one sequence that follow one

@@ -176,6 +176,11 @@ __device__ __forceinline__ float ex2(float x) {  // 2 units, 0 below 2^-126
     return y;
 }
 
+// x, or NaN where it is infinite.  An infinite key or value meets each piece of its other
+// factor by itself, so the sum is an infinity or NaN by the signs of low-order pieces: either
+// becomes NaN, so that a score of minus infinity does not leave its token out silently.
+__device__ __forceinline__ float finite_or_nan(float x) { return fmaf(x, 0.f, x); }
+
 // Two floats as N packed pairs of 16-bit pieces, leading piece first.
 template <int N, class T>
 __device__ __forceinline__ void cut(uint32_t (&w)[N], float a, float b) {
@@ -579,6 +584,7 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                     if constexpr (THIRD) s[h][i] += low[h][j][0][e] + low[h][j][1][e + 2];
                     s[h][i] += acc[h][j][0][e] + acc[h][j][1][e];
                     if constexpr (PACK) s[h][i] += __shfl_xor_sync(0xffffffffu, s[h][i], 16);
+                    s[h][i] = finite_or_nan(s[h][i]);
                 }
             if (have != kAll || ragged) {
 #pragma unroll
@@ -733,7 +739,7 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
                     if (whole) {
                         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                         *reinterpret_cast<float4*>(p.out + ((int64_t)(row + member) * p.n_heads + h0 + head) * D + col0 + col) =
-                            make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+                            make_float4(finite_or_nan(a.x * inv), finite_or_nan(a.y * inv), finite_or_nan(a.z * inv), finite_or_nan(a.w * inv));
                     } else {
                         __stcg(reinterpret_cast<float4*>(slot + h * D + col0 + col), a);
                         if (col0 + col == 0) {
@@ -838,7 +844,7 @@ __global__ void __launch_bounds__(32 * W, ctas_per_sm(D, W)) attention_kernel(co
 #pragma unroll
                         for (int j = 0; j < L; ++j)
 #pragma unroll
-                            for (int e = 0; e < V; ++e) p.out[to[u] + j * 32 * V + e] = acc[u][j][e] * inv;
+                            for (int e = 0; e < V; ++e) p.out[to[u] + j * 32 * V + e] = finite_or_nan(acc[u][j][e] * inv);
                     }
                 }
             }

@@ -394,3 +394,54 @@ def test_refusals(backend):
         backend.kv_cache(4, 16, 2, 80)
     with pytest.raises(KernelError):
         backend.kv_cache_view(k, v[:, :, :8])
+
+
+# (k/v heads, query heads of each, head_dim, type, rows of each sequence, tokens): the layouts of the query heads
+# (up to 4 of them, more, rows of a sequence together), one warp to an item, and items that several CTAs share.
+LAYOUTS = [(2, 4, 128, torch.bfloat16, 1, 90), (2, 4, 64, torch.float16, 1, 90), (2, 7, 96, torch.bfloat16, 1, 90),
+           (2, 8, 256, torch.float16, 1, 90), (2, 8, 256, torch.bfloat16, 1, 90), (2, 4, 128, torch.bfloat16, 4, 90),
+           (2, 2, 64, torch.float16, 4, 90), (2, 1, 256, torch.bfloat16, 4, 90), (8, 3, 128, torch.bfloat16, 100, 30),
+           (2, 4, 128, torch.bfloat16, 1, 20000), (2, 8, 128, torch.float16, 1, 20000), (2, 4, 128, torch.float16, 4, 20000)]
+
+
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("kv_heads,group,dim,dtype,rows,n", LAYOUTS)
+def test_infinite_key_that_a_row_sees_makes_its_heads_nan(backend, kv_heads, group, dim, dtype, rows, n, bad):
+    """Whatever the signs of the query: a score of minus infinity does not leave its token out silently."""
+    k, v, table = paged([n, n], 16, kv_heads, dim, dtype, 3)
+    if rows > 1:
+        table = torch.nn.functional.pad(table, (0, 3000), value=-1)  # room for long sequences
+    seqs = torch.arange(2, dtype=torch.int32, device="cuda").repeat_interleave(rows)
+    pos = (n - rows + torch.arange(rows, dtype=torch.int32, device="cuda")).clamp(min=0).repeat(2)
+    q = torch.randn(2 * rows, kv_heads * group, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    want, bound = attention_reference(q, k, v, pos, table, dim ** -0.5, seqs)
+    at = n - 5  # a token that only later rows of sequence 0 see
+    k[table[0, at // 16].long(), 1, at % 16, 9] = bad
+    got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, seqs=seqs if rows > 1 else None)
+    backend.synchronize()
+    hit = torch.zeros(2 * rows, kv_heads, group, dtype=torch.bool, device="cuda")
+    hit[:rows, 1] = (pos[:rows] >= at)[:, None]
+    hit = hit.view(2 * rows, kv_heads * group)
+    assert torch.isnan(got[hit]).all()
+    assert ((got.double() - want).abs() <= bound)[~hit].all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("kv_heads,group,dim,dtype,rows,n", LAYOUTS)
+def test_infinite_value_that_a_row_sees_makes_its_element_nan(backend, kv_heads, group, dim, dtype, rows, n, bad):
+    k, v, table = paged([n, n], 16, kv_heads, dim, dtype, 3)
+    if rows > 1:
+        table = torch.nn.functional.pad(table, (0, 3000), value=-1)  # room for long sequences
+    seqs = torch.arange(2, dtype=torch.int32, device="cuda").repeat_interleave(rows)
+    pos = (n - rows + torch.arange(rows, dtype=torch.int32, device="cuda")).clamp(min=0).repeat(2)
+    q = torch.randn(2 * rows, kv_heads * group, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    want, bound = attention_reference(q, k, v, pos, table, dim ** -0.5, seqs)
+    at = n - 5
+    v[table[0, at // 16].long(), 1, at % 16, 9] = bad
+    got = backend.paged_attention(q, backend.kv_cache_view(k, v), pos, table, seqs=seqs if rows > 1 else None)
+    backend.synchronize()
+    hit = torch.zeros(2 * rows, kv_heads, group, dim, dtype=torch.bool, device="cuda")
+    hit[:rows, 1, :, 9] = (pos[:rows] >= at)[:, None]
+    hit = hit.view(got.shape)
+    assert torch.isnan(got[hit]).all()
+    assert ((got.double() - want).abs() <= bound)[~hit].all()
