@@ -16,7 +16,7 @@ quantized in HBM and run through the fused dequant-GEMV (`linear_d`), with
   request has them, the embedding as a Q8_0 row gather;
 * between qkv and o, head norms, rotation and the paged cache write in one launch
   (`qk_norm_rope`) and the attention over the cache in another (`paged_attention`),
-  set up from the file's metadata at their first use.
+  set up from the file's metadata when the model is made.
 
 Tensor names follow the GGUF convention for these models (token_embd.weight,
 blk.N.attn_{q,k,v}.{weight,bias}, blk.N.attn_output.weight,
@@ -274,6 +274,13 @@ class QuantizedDecoderLinears:
         self.embed_table = upload_quant_tensor(backend, manifest, self.plan.embed)
         self.head_w = self.embed_table if self.plan.head == self.plan.embed else \
             upload_quant_tensor(backend, manifest, self.plan.head)
+        # Made here, so that the first attention() copies and allocates nothing but its outputs and may
+        # be a captured one.  A file whose metadata does not serve attention keeps its linear layers:
+        # what asks for attention raises the reason then.
+        try:
+            self._attention_parts()
+        except Exception:
+            pass
 
     # -- per layer ----------------------------------------------------------
     def qkv(self, i: int, x, rows: int, out) -> None:
@@ -281,7 +288,7 @@ class QuantizedDecoderLinears:
         self.backend.linear_dev(L["qkv"], x, rows, out, bias=L["qkv_bias"])
 
     def _attention_parts(self):
-        """(plan, rotation table, q norms, k norms), from the file at the first use."""
+        """(plan, rotation table, q norms, k norms), made with the model; raises why there are none."""
         if self._attention is None:
             import torch
             m, a = self._manifest, attention_plan(self._manifest, self.plan)

@@ -248,3 +248,31 @@ def test_step_of_a_file_with_scaled_positions(backend, tmp_path, stated):
     assert ((k - want_k).abs() <= half * want_k.abs() * (1 + half) + UNITS * k_size * (1 + half) + 1e-38).all()
     want, bound = attention_reference(q[599:], cache.k, cache.v, pos[599:], table, DIM ** -0.5)
     assert ((got.view(want.shape).double() - want).abs() <= bound).all()
+
+
+def test_first_attention_of_a_decoder_may_be_captured(backend, model):
+    """Over the caller's own caches, with nothing called before."""
+    from ocelotl_b200.model import QuantizedDecoderLinears
+    from tests.test_gpu_rope import UNITS
+    fresh = QuantizedDecoderLinears(backend, model._manifest)
+    k, v = (torch.zeros(4, KV_HEADS, PAGE, DIM, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cache = backend.kv_cache_view(k, v)
+    qkv = torch.randn(1, (HEADS + 2 * KV_HEADS) * DIM, device="cuda")
+    pos, table = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor([[2]], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            backend.use_current_stream()
+            out = fresh.attention(1, qkv, cache, pos, table)
+    finally:
+        backend.set_stream(None)
+    graph.replay()
+    torch.cuda.synchronize()
+    plan, _, qn, kn = fresh._attention_parts()
+    _, (want, size), _ = rope_reference(qkv, HEADS, KV_HEADS, DIM, pos, DIM, 1e6, plan.interleaved, qn[1], kn[1], plan.eps)
+    half = torch.finfo(torch.bfloat16).eps / 2
+    assert ((k[2, :, 0].double() - want[0]).abs() <= half * want[0].abs() * (1 + half) + UNITS * size[0] * (1 + half) + 1e-38).all()
+    # one token: the softmax is 1 and the output is the value as cached
+    cached = qkv[0, 5 * DIM:].bfloat16().float()
+    assert ((out.view(HEADS, DIM) - cached).abs() <= 2.0 ** -20 * cached.abs().max()).all()
