@@ -189,9 +189,11 @@ def attention_plan(m: Manifest, p: ModelPlan) -> AttentionPlan:
     dim = m.metadata.get(f"{arch}.attention.key_length", p.hidden // heads)
     if m.metadata.get(f"{arch}.attention.value_length", dim) != dim:
         raise UnsupportedError("attention value_length", str(m.metadata[f"{arch}.attention.value_length"]), [f"key_length={dim}"])
-    for feature in ("attention.sliding_window", "attn_logit_softcapping"):
+    for feature in ("attention.sliding_window", "attn_logit_softcapping", "attention.clamp_kqv", "attention.max_alibi_bias"):
         if m.metadata.get(f"{arch}.{feature}"):
             raise UnsupportedError(feature, str(m.metadata[f"{arch}.{feature}"]), ["none"])
+    if not m.metadata.get(f"{arch}.attention.causal", True):
+        raise UnsupportedError("attention.causal", "False", ["True"])
     rope_scale = _rope_scale(m, arch)
     for lp in p.layers:
         if lp.qkv_rows != [heads * dim, kv * dim, kv * dim]:

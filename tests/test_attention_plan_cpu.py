@@ -91,3 +91,12 @@ def test_position_scaling_that_is_refused(tmp_path, stated, error):
     m = manifest(tmp_path, llama(**stated))
     with pytest.raises(error, match="scal"):
         attention_plan(m, plan(m))
+
+
+@pytest.mark.parametrize("key,value", [("attention.causal", False), ("attention.clamp_kqv", 8.0), ("attention.max_alibi_bias", 8.0)])
+def test_attention_of_another_kind_is_refused(tmp_path, key, value):
+    m = manifest(tmp_path, {**META, "qwen3." + key: value})
+    with pytest.raises(UnsupportedError, match=key):
+        attention_plan(m, plan(m))
+    m.metadata["qwen3." + key] = True if value is False else 0.0  # as good as absent
+    assert attention_plan(m, plan(m)).n_heads == 4
