@@ -322,7 +322,7 @@ class QuantizedDecoderLinears:
         q = self.backend.qk_norm_rope(qkv, cache, positions, block_table, rope, q_norm=qn[i], k_norm=kn[i], eps=a.eps,
                                       seqs=seqs, out=q)
         o = self.backend.paged_attention(q, cache, positions, block_table, scale=a.scale, seqs=seqs, out=out)
-        return o.view(o.shape[0], -1)
+        return o.view(o.shape[0], a.n_heads * a.head_dim)
 
     def o(self, i: int, x, rows: int, out) -> None:
         self.backend.linear_dev(self.layers[i]["o"], x, rows, out)

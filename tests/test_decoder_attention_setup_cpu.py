@@ -88,3 +88,8 @@ def test_refused_table_is_tried_again(tmp_path):
         model.attention(0, torch.zeros(1, 6 * 64), None, None, None)
     b.refuse = False
     assert model.attention(0, torch.zeros(1, 6 * 64), None, None, None).shape == (1, 4 * 64)
+
+
+def test_no_rows(tmp_path):
+    _, model = decoder(tmp_path, META, HostBackend())
+    assert model.attention(0, torch.zeros(0, 6 * 64), None, None, None).shape == (0, 4 * 64)
