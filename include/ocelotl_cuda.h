@@ -320,7 +320,8 @@ typedef struct ocl_kv_rows {
  * position * base^(-2i / rot_dim) / factors_host[i] (factors NULL = all 1;
  * GGUF rope_freqs.weight).  interleaved 0: pairs (i, i + rot_dim / 2); 1: pairs
  * (2i, 2i + 1).  rot_dim a multiple of 8, at most 256.  The angle is kept as a
- * 64-bit fixed-point fraction of a revolution, exact at far positions. */
+ * 64-bit fixed-point fraction of a revolution: it wraps exactly, and is as good at far
+ * positions as at near ones (9.4e-8 rad, the rounding of a turn to f32). */
 OCL_API int ocl_rope_create(ocl_ctx* ctx, size_t rot_dim, double base, const float* factors_host, int interleaved,
                             ocl_rope** out);
 OCL_API int ocl_rope_free(ocl_rope* rope);

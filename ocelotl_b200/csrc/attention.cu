@@ -18,7 +18,8 @@
 // (q scaled by a power of two per head, p by 2^14, so that f16's range is enough).
 // The tensor core truncates when it adds; chains are kept short (two chains over
 // head_dim, 32 tokens of p.v) and joined with rounding f32 adds.  Error against the formula
-// in 64 bits: 2e-7 to 4e-7 of the result, below that of f32 matrix products.
+// in 64 bits, by its norm: bf16 1.4e-7 to 3.1e-7 of the result, f16 2.4e-7 to 5.0e-7 (random
+// keys and values, all head_dims, up to 16000 tokens; f32 matrix products 1.3e-7 to 1.3e-6).
 //
 // Work split: the tiles (4 warps of 32 tokens of one row and k/v head) of all rows, in
 // order, are cut into equal runs, one per resident CTA, from the positions in device

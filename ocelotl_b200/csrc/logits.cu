@@ -14,7 +14,7 @@
 // atomics: their order does not show), adds up the biases that do, then applies
 // everything to the registers and stores.  Nothing of the size of the vocabulary is
 // kept between calls.  Bound: one read and one write of the logits; the history is
-// read again by every run of its row, from L2, with eight loads of a thread in flight.
+// read again by every run of its row, from L2, with up to four loads of a thread in flight.
 //
 // The greedy pick is argmax.cu's: one 64-bit key per run, the last run of a row
 // writes the id.

@@ -9,9 +9,12 @@
 // nearest even.
 //
 // The angle: freq_i is held in revolutions as a 64-bit fixed-point fraction, so
-// position * step wraps modulo one revolution exactly and the phase is good to
-// position * 2^-65 revolutions at any 31-bit position; an f32 product loses
-// 2^-24 of the whole angle instead (0.008 rad at position 131072).
+// position * step wraps modulo one revolution exactly.  The step is off by its rounding
+// (2^-65 revolutions) and its evaluation in 64-bit mantissas (a few 2^-64 of it), times the
+// position: 2^-45 revolutions at 131072.  The phase is then rounded to f32, by at most
+// 2^-26 revolutions (9.4e-8 rad), which is the error of the angle that is used at any
+// 31-bit position; an f32 product loses 2^-24 of the whole angle instead (0.008 rad at
+// position 131072).
 //
 // One warp per head, one or more CTAs per row (the host splits the heads of few
 // rows over CTAs); the row's cos and sin are computed once per CTA.
